@@ -31,6 +31,10 @@ void omni_ops_destroy(omni_ops* ctx);
 /* Waits for the context's stream; returns 0, OMNI_ERR_CUDA (-2) or, when a
  * kernel raised the device error word, OMNI_ERR_DEVICE (-3) with the word in *word. */
 int32_t omni_ops_sync(omni_ops* ctx, uint32_t* word);
+/* The stream that the context's calls run on from here: given = 1: `stream`, a cudaStream_t of the context's device (NULL = the
+ * default stream), which the caller may be capturing into a graph if the calls made are those of the 8-bit paged cache below;
+ * given = 0: the context's own again, as after `omni_ops_create`. Calls on the one are not ordered against calls on the other. */
+int32_t omni_ops_stream(omni_ops* ctx, int32_t given, void* stream);
 /* Device time in ms between the two most recent omni_ops_mark calls (CUDA events on the context's stream). */
 int32_t omni_ops_mark(omni_ops* ctx, int32_t which /* 0 = begin, 1 = end */);
 int32_t omni_ops_elapsed_ms(omni_ops* ctx, float* ms);
@@ -210,6 +214,70 @@ int32_t omni_higgs_undelay(const int32_t* rows, int32_t n_rows, int32_t* frames)
 int32_t omni_op_gemm_noalloc(const void* w, int32_t N, int32_t K, const void* x, int32_t rows, void* y, int32_t ldy,
                              int32_t splits, const void* bias, int32_t epilogue, void* stream, char* message,
                              size_t message_len);
+
+/* ---- 8-bit paged cache -----------------------------------------------------------------------------------------------
+ * The operators of a grouped-head stack that keeps its KV in 8 bits. They have no counterpart in the reference, whose KV is
+ * bf16 (crates/omni-qwen3/kernels/qwen3.cu:109-240). One decoder layer of a call:
+ *   omni_op_kv_tables      lengths -> page tables, positions and slots of the call's rows (once for all layers)
+ *   omni_op_qk_norm_rope   norm and rotary embedding of the rows' q and k
+ *   omni_op_kv8_append     the rows' K and V into the pages
+ *   omni_op_kv8_attend     one row a sequence: attention over the pages
+ * Cache of a layer: kv[page][kv_head][K | V][16][head_dim] in E4M3 and scales[page][kv_head][K | V] in f32; an element is its
+ * code times its scale. Heads of 64 or 128. Rows of bf16 are given with a stride in elements (ld), a multiple of 8, so that parts
+ * of wider rows can be passed; base addresses are multiples of 16 bytes (scales: 8). Zero rows are a call that does nothing.
+ * Every call is one kernel, allocates nothing and uses no workspace: it may be captured, and graphs may run side by side.
+ * What device arrays hold (lengths, positions, slots, pages) the host does not see; where the kernels find an index outside
+ * its table they skip it and raise the device error word. */
+
+/* Page tables of n sequences (4096 at most). lens[i]: tokens that sequence i holds; add[i]: tokens that this call appends (0 and
+ * more), or -1: the sequence has ended and its pages come back. table[i][width]: its pages, in order. free_pages[0 .. *free_count):
+ * a stack of free pages with room for free_cap. Pages of ended sequences are laid on top of it in the sequences' order; then, in
+ * the sequences' order, each page that is wanted is taken from its top and entered into the table.
+ *   lens_out[n], *free_count_out   the new lengths (0 for ended sequences) and height; may be lens and free_count themselves
+ *   indptr[n + 1], pages           the tables packed: sequence i has pages[indptr[i] .. indptr[i + 1]); room for page_cap
+ *   row_ptr[n + 1], pos, slot, seq the call's rows, sequence by sequence: position, slot (page * 16 + pos % 16) and sequence of
+ *                                  each; room for row_cap, of which the rows behind the last hold -1
+ *   *status                        0; otherwise nothing was changed (lens_out and *free_count_out say what lens and *free_count
+ *                                  do, pages is untouched, indptr and row_ptr are 0, pos, slot and seq are -1) and it is a sum of
+ *                                  OMNI_TABLES_*. A server's ordinary answer to BUSY is to try again with fewer sequences.
+ * No array may overlap another one but for the two that are named. */
+enum omni_tables_status {
+  OMNI_TABLES_LENGTH = 1,  /* a length below 0, an addition below -1, or more tokens than a table's width holds */
+  OMNI_TABLES_BUSY = 2,    /* fewer pages free than wanted */
+  OMNI_TABLES_ROWS = 4,    /* more rows than row_cap */
+  OMNI_TABLES_PAGES = 8,   /* more pages than page_cap */
+  OMNI_TABLES_FREE = 16    /* *free_count below 0 or above free_cap, or more pages come back than free_cap holds */
+};
+int32_t omni_op_kv_tables(omni_ops* ctx, const int32_t* lens, const int32_t* add, int32_t n, int32_t* table, int32_t width,
+                          int32_t* free_pages, int32_t free_cap, const int32_t* free_count, int32_t* lens_out,
+                          int32_t* free_count_out, int32_t* indptr, int32_t* pages, int32_t page_cap, int32_t* row_ptr,
+                          int32_t* pos, int32_t* slot, int32_t* seq, int32_t row_cap, int32_t* status);
+
+/* The first q_heads + kv_heads heads of every row of x with pos >= 0, normed (x / sqrt(mean x^2 + eps) * gain, q_norm for the
+ * q heads, k_norm for the k heads; NULL: no norm) and rotated: elements i and i + head_dim / 2 by pos * theta^(-2 i / head_dim).
+ * Computed in f32 from an angle in f64 and rounded once (the attention calls above round between the steps as the reference
+ * does). Other rows of out stay as they are. out may be x, with the same stride, and must not overlap it otherwise. */
+int32_t omni_op_qk_norm_rope(omni_ops* ctx, const void* x, int64_t ldx, const void* q_norm, const void* k_norm,
+                             const int32_t* pos, int32_t rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                             float eps, float theta, void* out, int64_t ldo);
+
+/* K and V of every row with slot >= 0 into the cache. A page's scale (one for K, one for V of each head) is the smallest 2^e with
+ * e >= -100 and |x| <= 448 * 2^e for every finite x put into it. A row at a page's first token starts the page anew; rows further in
+ * come behind tokens that the page holds, whose scale then only grows, and whose codes are rounded again when it does. Codes
+ * are the nearest, ties to even; infinities become +-448 * 2^e, a NaN stays one. Rows of one page are neighbours in the call, in
+ * ascending slots without a gap, as omni_op_kv_tables lays them: a page that occurs in two places of a call is written in an
+ * undefined order. */
+int32_t omni_op_kv8_append(omni_ops* ctx, const void* k, int64_t ldk, const void* v, int64_t ldv, const int32_t* slot,
+                           int32_t rows, void* kv, float* scales, int32_t kv_pages, int32_t kv_heads, int32_t head_dim);
+
+/* out[n][h] = softmax(scale * q[n][h] . K) V over tokens 0 .. pos[n] of sequence seq[n] (NULL: sequence n) of n_seqs, whose pages
+ * are pages[indptr[s] .. indptr[s + 1]) out of n_pages. Rows with pos < 0 become zeros. What a page holds behind the row's
+ * last token is not looked at. Scales may be any numbers >= 0 here. A row whose sequence, range or number of pages is wrong becomes
+ * zeros; a page outside the cache is left out. */
+int32_t omni_op_kv8_attend(omni_ops* ctx, const void* q, int64_t ldq, const void* kv, const float* scales, int32_t kv_pages,
+                           const int32_t* pos, const int32_t* seq, const int32_t* indptr, int32_t n_seqs,
+                           const int32_t* pages, int32_t n_pages, int32_t rows, int32_t q_heads, int32_t kv_heads,
+                           int32_t head_dim, float scale, void* out, int64_t ldo);
 
 /* ---- streaming codec decoder: crates/omni-qwen3-tts/kernels/codec.cu, src/codec.rs -------------------------------
  * A per-stream state is `state + lines[s] * stride` bytes plus the entry's own byte offset; `pos[s]` is the number of

@@ -1,0 +1,405 @@
+// Decode attention over pages in 8 bits (kv8.h): one query row a sequence, grouped heads.
+//
+// Bound by HBM: 2 D bytes a token and kv head are read once, for 4 D operations a query head on them. A warp takes every W-th page
+// of a row and kv head, W being the warps of its cluster; its pages travel through a ring of its own in shared memory (cp.async,
+// kStages deep), so warps never wait for one another before the end. There the warps' sums meet in shared memory and the CTAs'
+// in distributed shared memory: one launch, no workspace, sums in a fixed order.
+//
+// Both products run on m16n8k16 with the page as the left operand and the queries as the eight columns, so a group of up to eight
+// heads wastes no rows of it: S^T[16 tokens, 8 queries] = K Q^T and O^T[D, 8 queries] += V^T P^T. E4M3 widens to f16 without loss. The
+// order of the head's elements within a sum is free, so a lane's operands are whole words of a key's row (Q is held in the same
+// order), and those of V^T are bytes of two tokens put side by side. Queries go to f16 under a power of two of their own, which
+// loses nothing above 2^-39 of the largest. With s the score in powers of two and u the log2 of the page's V scale, the
+// weights of a row are 2^(s + u - R), R near the largest s + u: at most 2^8 and rounded to f16 (2^-11 relative, an eighth of what
+// the bf16 result is rounded by). Their sum is taken of 2^(s - r) in f32, r near the largest s.
+#include <cooperative_groups.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "kv8.h"
+#include "sm100.cuh"
+
+namespace omni {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kWarps = 8;
+constexpr float kSlack = 8.f;  // powers of two by which a score may pass its reference before the sums are rescaled
+constexpr float kNegInf = -__builtin_huge_valf();
+
+template <int D>
+constexpr int kStages = D == 128 ? 3 : 4;
+template <int D>
+constexpr int kPageBytes = 32 * D;  // K and V of one head
+
+template <int D, int NT>
+constexpr int smem_bytes() {
+  constexpr int ring = kWarps * kStages<D> * kPageBytes<D>;
+  constexpr int merge = (kWarps + 1) * NT * 8 * D * 4;
+  return ring > merge ? ring : merge;
+}
+
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 u;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(addr));
+  return u;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
+  uint2 u;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(u.x), "=r"(u.y) : "r"(addr));
+  return u;
+}
+
+// Four e4m3 (a word) as f16: bytes 0, 1 in lo, bytes 2, 3 in hi.
+__device__ __forceinline__ void widen(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}" : "=r"(lo), "=r"(hi) : "r"(four));
+}
+
+// An 8 x 8 matrix of 16-bit values, a row's pair a lane, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t half2_of(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Where 16-byte piece `col` of row `row` of a page lies in its stage: neighbouring rows' pieces in different banks.
+template <int D>
+__device__ __forceinline__ uint32_t piece_at(int row, int col) {
+  return (uint32_t)(row * D + ((D == 128 ? col ^ (row & 7) : col ^ ((row >> 1) & 3)) << 4));
+}
+
+struct Part {  // of a query: reference of the scores, of the weights, sum of 2^(s - r)
+  float r, R, l;
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32, 2) kv8_attend_kernel(const __grid_constant__ Kv8Attend a, int subgroups, int per, uint32_t* err) {
+  constexpr int S = kStages<D>, CW = D / 64;  // pieces of a key's row a lane holds
+  constexpr int STEPS = D / 16;               // matrix instructions of K Q^T; as many of V^T P^T
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ Part parts[kWarps][NT * 8], joined[NT * 8];
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, warp = warp_index(), g = lane >> 2, t = lane & 3;
+  const int unit = blockIdx.x / ctas;
+  const int groups = a.kv_heads * subgroups;
+  const int row = unit / groups, kh = unit % groups / subgroups, sub = unit % subgroups;
+  const int group = a.q_heads / a.kv_heads, q0 = sub * per, nq = min(per, group - q0);
+  const int head0 = kh * group + q0;
+  bf16* const out = a.out + row * a.ldo + (int64_t)head0 * D;
+
+  // the row's tokens and pages
+  int len = a.pos[row] + 1, first = 0;
+  if (len > 0) {
+    const int s = a.seq ? a.seq[row] : row;
+    bool ok = s >= 0 && s < a.n_seqs;
+    if (ok) {
+      first = a.indptr[s];
+      const int last = a.indptr[s + 1];
+      ok = first >= 0 && last <= a.n_pages && (int64_t)last - first >= ((int64_t)len + 15) / 16;
+    }
+    if (!ok) {
+      if (tid == 0) raise(err, kErrBadIndex);
+      len = 0;
+    }
+  }
+  if (len <= 0) {  // the same for every CTA of the cluster
+    if (rank == 0)
+      for (int i = tid; i < nq * (D / 8); i += kWarps * 32) *reinterpret_cast<uint4*>(out + i * 8) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const int all = (len >> 4) + ((len & 15) != 0), workers = ctas * kWarps, me = rank * kWarps + warp;
+  const int mine = me < all ? (all - me + workers - 1) / workers : 0;
+  const int32_t* const my_pages = a.pages + first + me;
+
+  // pages and their scales, thirty-two at a time: lane i holds those of this warp's page 32 b + i
+  const auto fetch_id = [&](int b) {
+    const int i = b * 32 + lane;
+    if (i >= mine) return 0;
+    const int id = __ldg(my_pages + (int64_t)i * workers);
+    if (id >= 0 && id < a.kv_pages) return id;
+    raise(err, kErrBadIndex);
+    return -1;
+  };
+  const float2* const scales = reinterpret_cast<const float2*>(a.scales) + kh;
+  int ids = fetch_id(0), ids_next = mine > 32 ? fetch_id(1) : 0;
+  float2 sc = __ldg(scales + (int64_t)max(ids, 0) * a.kv_heads), sc_next = sc;
+  if (ids < 0) sc.x = -1.f;  // no tokens on it
+
+  const uint32_t ring = sm100::smem_addr(smem) + warp * (S * kPageBytes<D>);
+  const auto issue = [&](int i, int stage) {
+    if (i < mine) {
+      if ((i & 31) == 0 && i > 0) {
+        ids = ids_next;
+        sc_next = __ldg(scales + (int64_t)max(ids, 0) * a.kv_heads);
+        if (ids < 0) sc_next.x = -1.f;
+        if (i + 32 < mine) ids_next = fetch_id(i / 32 + 1);
+      }
+      const int64_t id = max(__shfl_sync(0xffffffffu, ids, i & 31), 0);
+      const uint8_t* const src = a.kv + (id * a.kv_heads + kh) * kPageBytes<D>;
+      const uint32_t dst = ring + stage * kPageBytes<D>;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        const int piece = j * 32 + lane;
+        copy16(dst + piece_at<D>(piece / (D / 16), piece % (D / 16)), src + piece * 16);
+      }
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) issue(i, i);
+
+  // queries: column n of a tile is query head head0 + n, lane t holds elements (D / 4) t .. of it
+  uint32_t qf[NT][STEPS][2];
+  float unit_of[NT][2];  // scores of columns 2 t, 2 t + 1 in powers of two
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int n = nt * 8 + g;
+    float x[STEPS * 4];
+    if (n < nq) {
+      const bf16* const src = a.q + row * a.ldq + (int64_t)(head0 + n) * D + t * (D / 4);
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) ld8(src + 8 * j, x + 8 * j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < STEPS * 4; ++j) x[j] = 0.f;
+    }
+    float top = 0.f;
+#pragma unroll
+    for (int j = 0; j < STEPS * 4; ++j) top = fmaxf(top, fabsf(x[j]) < __builtin_huge_valf() ? fabsf(x[j]) : 0.f);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = max((int)(__float_as_uint(top) >> 23) - 127, -112);  // largest in [2^14, 2^15) in f16
+    const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23), down = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) qf[nt][j][0] = half2_of(x[4 * j] * up, x[4 * j + 1] * up), qf[nt][j][1] = half2_of(x[4 * j + 2] * up, x[4 * j + 3] * up);
+    const float f = a.scale * 1.44269504088896340736f * down;
+    unit_of[nt][0] = __shfl_sync(0xffffffffu, f, t * 8), unit_of[nt][1] = __shfl_sync(0xffffffffu, f, t * 8 + 4);
+  }
+
+  float r[NT][2], R[NT][2], l[NT][2], o[NT][STEPS][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    r[nt][0] = r[nt][1] = R[nt][0] = R[nt][1] = kNegInf, l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+  }
+
+  int stage = 0;
+  for (int i = 0; i < mine; ++i) {
+    copy_wait<S - 2>();
+    __syncwarp();  // every lane's pieces are there, and every lane is done with the stage that is filled next
+    if ((i & 31) == 0 && i > 0) sc = sc_next;
+    issue(i + S - 1, stage == 0 ? S - 1 : stage - 1);
+    const uint32_t keys = ring + stage * kPageBytes<D>;
+    stage = stage == S - 1 ? 0 : stage + 1;
+    const float ks = __shfl_sync(0xffffffffu, sc.x, i & 31), vs = __shfl_sync(0xffffffffu, sc.y, i & 31);
+    const int valid = ks < 0.f ? 0 : len - (me + i * workers) * 16;  // tokens from the page's first on
+    if (valid <= 0) continue;
+
+    float s[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+    for (int c = 0; c < CW; ++c) {
+      const uint4 lo = lds16(keys + piece_at<D>(g, t * CW + c)), hi = lds16(keys + piece_at<D>(g + 8, t * CW + c));
+      const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t a0, a1, a2, a3;
+        widen(wl[w], a0, a2), widen(wh[w], a1, a3);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sm100::mma_16816_f16(s[nt], a0, a1, a2, a3, qf[nt][c * 4 + w][0], qf[nt][c * 4 + w][1]);
+      }
+    }
+    const float lvs = __log2f(vs);
+    bool over = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v = s[nt][e] * (ks * unit_of[nt][e & 1]);
+        s[nt][e] = g + (e & 2) * 4 < valid ? v : kNegInf;
+        over |= s[nt][e] > r[nt][e & 1] + kSlack || s[nt][e] + lvs > R[nt][e & 1] + kSlack;
+      }
+    if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float m = fmaxf(s[nt][e], s[nt][e + 2]);
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+          // a reference is a number even where all scores so far are -infinity
+          const float nr = fmaxf(r[nt][e], m), nR = fmaxf(R[nt][e], m + lvs);
+          l[nt][e] *= r[nt][e] == kNegInf ? 0.f : exp2_of(r[nt][e] - nr);
+          const float f = R[nt][e] == kNegInf ? 0.f : exp2_of(R[nt][e] - nR);
+          r[nt][e] = nr, R[nt][e] = nR;
+#pragma unroll
+          for (int j = 0; j < STEPS; ++j) o[nt][j][e] *= f, o[nt][j][e + 2] *= f;
+        }
+    }
+    uint32_t p[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float rr = r[nt][e & 1] == kNegInf ? 0.f : r[nt][e & 1], RR = R[nt][e & 1] == kNegInf ? 0.f : R[nt][e & 1];
+        l[nt][e & 1] += exp2_of(s[nt][e] - rr);
+        w[e] = exp2_of(s[nt][e] + lvs - RR);
+      }
+      p[nt][0] = transpose8(half2_of(w[0], w[1])), p[nt][1] = transpose8(half2_of(w[2], w[3]));
+    }
+    const uint32_t values = keys + 16 * D;
+    constexpr int WORDS = D / 32;  // of a value's row that a lane holds: elements (D / 8) g ..
+    uint32_t u[4][WORDS];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int tok = 2 * t + (k & 1) + (k >> 1) * 8;
+      if constexpr (D == 128) {
+        const uint4 v = lds16(values + piece_at<D>(tok, g));
+        u[k][0] = v.x, u[k][1] = v.y, u[k][2] = v.z, u[k][3] = v.w;
+      } else {
+        const uint2 v = lds8(values + piece_at<D>(tok, g >> 1) + (g & 1) * 8);
+        u[k][0] = v.x, u[k][1] = v.y;
+      }
+      if (tok >= valid) {  // what lies there may be NaN
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) u[k][w] = 0;
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t a0, a1, a2, a3;
+        widen(__byte_perm(u[0][w], u[1][w], half ? 0x7362 : 0x5140), a0, a1), widen(__byte_perm(u[2][w], u[3][w], half ? 0x7362 : 0x5140), a2, a3);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sm100::mma_16816_f16(o[nt][w * 2 + half], a0, a1, a2, a3, p[nt][0], p[nt][1]);
+      }
+  }
+
+  // the warps' sums: o is [D / 8 bytes of lane g][column], a matrix instruction two neighbouring elements
+  copy_wait<0>();
+  __syncthreads();
+  float* const sums = reinterpret_cast<float*>(smem);        // [warp][query][D]
+  float* const total = sums + kWarps * NT * 8 * D;           // [query][D]
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int n = nt * 8 + 2 * t + e;
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
+      if (n < nq) {
+        if (g == 0) parts[warp][n] = Part{r[nt][e], R[nt][e], l[nt][e]};
+        float* const dst = sums + (warp * NT * 8 + n) * D + g * (D / 8);
+#pragma unroll
+        for (int j = 0; j < STEPS; j += 2)
+          *reinterpret_cast<float4*>(dst + 2 * j) = make_float4(o[nt][j][e], o[nt][j][e + 2], o[nt][j + 1][e], o[nt][j + 1][e + 2]);
+      }
+    }
+  __syncthreads();
+  // weights of summands under references x when the largest is `top`
+  const auto weight = [](float x, float top) { return x == kNegInf ? 0.f : exp2_of(x - top); };
+  const auto finish = [&](int n, int d, float4 v, float r_top, float R_top, float l_sum) {
+    const float f = exp2_of((R_top == kNegInf ? 0.f : R_top) - (r_top == kNegInf ? 0.f : r_top)) / l_sum;
+    uint2 w;
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x * f, v.y * f), hi = __floats2bfloat162_rn(v.z * f, v.w * f);
+    w.x = *reinterpret_cast<const uint32_t*>(&lo), w.y = *reinterpret_cast<const uint32_t*>(&hi);
+    *reinterpret_cast<uint2*>(out + n * D + d) = w;
+  };
+  for (int i = tid; i < nq * (D / 4); i += kWarps * 32) {
+    const int n = i / (D / 4), d = i % (D / 4) * 4;
+    float r_top = kNegInf, R_top = kNegInf, l_sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) r_top = fmaxf(r_top, parts[w][n].r), R_top = fmaxf(R_top, parts[w][n].R);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const Part p = parts[w][n];
+      l_sum += p.l * weight(p.r, r_top);
+      const float f = weight(p.R, R_top);
+      const float4 x = *reinterpret_cast<const float4*>(sums + (w * NT * 8 + n) * D + d);
+      v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+    }
+    if (ctas == 1) {
+      finish(n, d, v, r_top, R_top, l_sum);
+    } else {
+      *reinterpret_cast<float4*>(total + n * D + d) = v;
+      if (d == 0) joined[n] = Part{r_top, R_top, l_sum};
+    }
+  }
+  if (ctas == 1) return;
+  cluster.sync();
+  for (int i = rank * (kWarps * 32) + tid; i < nq * (D / 4); i += ctas * (kWarps * 32)) {
+    const int n = i / (D / 4), d = i % (D / 4) * 4;
+    float r_top = kNegInf, R_top = kNegInf, l_sum = 0.f;
+    for (int c = 0; c < ctas; ++c) {
+      const Part p = *cluster.map_shared_rank(&joined[n], c);
+      r_top = fmaxf(r_top, p.r), R_top = fmaxf(R_top, p.R);
+    }
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < ctas; ++c) {
+      const Part p = *cluster.map_shared_rank(&joined[n], c);
+      l_sum += p.l * weight(p.r, r_top);
+      const float f = weight(p.R, R_top);
+      const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(total, c) + n * D + d);
+      v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+    }
+    finish(n, d, v, r_top, R_top, l_sum);
+  }
+  cluster.sync();  // no CTA leaves while another reads its sums
+}
+
+template <int D, int NT>
+cudaError_t go(const Kv8Attend& a, int ctas, int subgroups, int per, uint32_t* err, cudaStream_t s) {
+  constexpr int smem = smem_bytes<D, NT>();
+  const cudaError_t e = cudaFuncSetAttribute(kv8_attend_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.rows * a.kv_heads * subgroups * ctas)), cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = smem, cfg.stream = s;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv8_attend_kernel<D, NT>, a, subgroups, per, err);
+}
+
+}  // namespace
+
+cudaError_t launch_kv8_attend(const Kv8Attend& a, int sm_count, uint32_t* err, cudaStream_t s) {
+  const int group = a.q_heads / a.kv_heads, subgroups = (group + 15) / 16, per = (group + subgroups - 1) / subgroups;
+  const int64_t units = (int64_t)a.rows * a.kv_heads * subgroups;
+  int ctas = 1;
+  while (ctas < 8 && units * ctas < 4 * sm_count) ctas *= 2;
+  if (a.head_dim == 128) return per > 8 ? go<128, 2>(a, ctas, subgroups, per, err, s) : go<128, 1>(a, ctas, subgroups, per, err, s);
+  if (a.head_dim == 64) return per > 8 ? go<64, 2>(a, ctas, subgroups, per, err, s) : go<64, 1>(a, ctas, subgroups, per, err, s);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace omni

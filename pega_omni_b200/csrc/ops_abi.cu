@@ -12,12 +12,14 @@
 #include "gemm.h"
 #include "duplex.h"
 #include "kernels.h"
+#include "kv8.h"
 
 using namespace omni;
 
 struct omni_ops {
   int device = 0, sm_count = 148;
-  cudaStream_t stream = nullptr;
+  cudaStream_t own = nullptr;     // the context's
+  cudaStream_t stream = nullptr;  // what calls run on: `own` or the caller's
   cudaEvent_t ev[2] = {nullptr, nullptr};
   GemmScratch scratch;
   uint32_t* err = nullptr;
@@ -78,7 +80,8 @@ int32_t omni_ops_create(int32_t device, omni_ops** out) {
   OPS_CUDA(c, cudaGetDeviceProperties(&prop, device));
   if (prop.major != 10) return c->fail(OMNI_ERR_UNSUPPORTED, "device is sm_%d%d; this library is sm_100a only", prop.major, prop.minor);
   c->sm_count = prop.multiProcessorCount;
-  OPS_CUDA(c, cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking));
+  OPS_CUDA(c, cudaStreamCreateWithFlags(&c->own, cudaStreamNonBlocking));
+  c->stream = c->own;
   OPS_CUDA(c, cudaEventCreate(&c->ev[0]));
   OPS_CUDA(c, cudaEventCreate(&c->ev[1]));
   if (tc_init() != 0) return c->fail(OMNI_ERR_CUDA, "cuTensorMapEncodeTiled entry point not found");
@@ -97,13 +100,13 @@ int32_t omni_ops_create(int32_t device, omni_ops** out) {
 void omni_ops_destroy(omni_ops* c) {
   if (!c) return;
   cudaSetDevice(c->device);
-  if (c->stream) cudaStreamSynchronize(c->stream);
+  if (c->own) cudaStreamSynchronize(c->own);  // a caller's stream may be gone; cudaFree waits for what it ran
   cudaFree(c->scratch.partials);
   cudaFree(c->scratch.counters);
   cudaFree(c->err);
   if (c->ev[0]) cudaEventDestroy(c->ev[0]);
   if (c->ev[1]) cudaEventDestroy(c->ev[1]);
-  if (c->stream) cudaStreamDestroy(c->stream);
+  if (c->own) cudaStreamDestroy(c->own);
   delete c;
 }
 
@@ -119,6 +122,26 @@ int32_t omni_ops_sync(omni_ops* c, uint32_t* word) {
     cudaMemset(c->err, 0, 4);
     return c->fail(OMNI_ERR_DEVICE, "device error word 0x%x", w);
   }
+  return OMNI_OK;
+}
+
+int32_t omni_ops_stream(omni_ops* c, int32_t given, void* stream) {
+  if (!c) return OMNI_ERR_INVALID;
+  if (!given) {
+    c->stream = c->own;
+    return OMNI_OK;
+  }
+#if CUDART_VERSION >= 12080
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (stream) OPS_CUDA(c, cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture));
+  if (stream && capture == cudaStreamCaptureStatusNone) {  // the question would end a capture; a launch on another device's stream fails
+    int device = c->device;
+    OPS_CUDA(c, cudaStreamGetDevice(static_cast<cudaStream_t>(stream), &device));
+    if (device != c->device)
+      return c->fail(OMNI_ERR_INVALID, "the stream belongs to device %d, the context to device %d", device, c->device);
+  }
+#endif
+  c->stream = static_cast<cudaStream_t>(stream);
   return OMNI_OK;
 }
 
@@ -447,6 +470,99 @@ int32_t omni_higgs_undelay(const int32_t* rows, int32_t n_rows, int32_t* frames)
   for (int t = 0; t < n; ++t)
     for (int b = 0; b < OMNI_HIGGS_BOOKS; ++b) frames[t * OMNI_HIGGS_BOOKS + b] = rows[(t + b) * OMNI_HIGGS_BOOKS + b];
   return n;
+}
+
+// ---- 8-bit paged cache ----------------------------------------------------------------------------------------------
+
+// The context's device for the length of a call.
+struct OnDevice {
+  int before = -1;
+  explicit OnDevice(int device) {
+    if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+    if (before != device) cudaSetDevice(device);
+    else before = -1;
+  }
+  ~OnDevice() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+static bool at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Rows of `width` elements at 16-byte addresses, `ld` elements apart.
+static bool rows_at16(const void* p, int64_t ld, int64_t width) { return at16(p) && ld >= width && ld % 8 == 0; }
+static bool heads_fit(int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
+  return q_heads >= 1 && kv_heads >= 1 && q_heads <= 65535 && q_heads % kv_heads == 0 && (head_dim == 64 || head_dim == 128);
+}
+
+int32_t omni_op_kv_tables(omni_ops* c, const int32_t* lens, const int32_t* add, int32_t n, int32_t* table, int32_t width,
+                          int32_t* free_pages, int32_t free_cap, const int32_t* free_count, int32_t* lens_out,
+                          int32_t* free_count_out, int32_t* indptr, int32_t* pages, int32_t page_cap, int32_t* row_ptr,
+                          int32_t* pos, int32_t* slot, int32_t* seq, int32_t row_cap, int32_t* status) {
+  if (!c) return OMNI_ERR_INVALID;
+  if (n < 0 || width < 1 || free_cap < 0 || page_cap < 0 || row_cap < 0) return c->fail(OMNI_ERR_INVALID, "a negative size, or a table without columns");
+  if (!free_count || !free_count_out || !indptr || !row_ptr || !status || (n > 0 && (!lens || !add || !table || !lens_out)) ||
+      (free_cap > 0 && !free_pages) || (page_cap > 0 && !pages) || (row_cap > 0 && (!pos || !slot || !seq)))
+    return c->fail(OMNI_ERR_INVALID, "a null pointer");
+  if (n > kTablesMaxSeqs || (int64_t)n * width > kTablesMaxEntries)
+    return c->fail(OMNI_ERR_UNSUPPORTED, "%d sequences of %d pages: at most %d, and %lld pages in all", n, width, kTablesMaxSeqs,
+                   (long long)kTablesMaxEntries);
+  const OnDevice on(c->device);
+  const TablesCall call{lens, add, n, table, width, free_pages, free_cap, free_count, lens_out, free_count_out, indptr,
+                        pages, page_cap, row_ptr, pos, slot, seq, row_cap, status};
+  OPS_CUDA(c, launch_kv_tables(call, c->stream));
+  return OMNI_OK;
+}
+
+int32_t omni_op_qk_norm_rope(omni_ops* c, const void* x, int64_t ldx, const void* q_norm, const void* k_norm,
+                             const int32_t* pos, int32_t rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                             float eps, float theta, void* out, int64_t ldo) {
+  if (!c || rows < 0 || !(theta > 0.f)) return c ? c->fail(OMNI_ERR_INVALID, "rows < 0 or theta <= 0") : OMNI_ERR_INVALID;
+  if (q_heads < 0 || kv_heads < 0 || q_heads + (int64_t)kv_heads < 1 || q_heads + (int64_t)kv_heads > 65535 || (head_dim != 64 && head_dim != 128))
+    return c->fail(OMNI_ERR_UNSUPPORTED, "%d + %d heads of %d: heads of 64 or 128", q_heads, kv_heads, head_dim);
+  if (rows == 0) return OMNI_OK;
+  const int64_t width = ((int64_t)q_heads + kv_heads) * head_dim;
+  if (!x || !pos || !out || !rows_at16(x, ldx, width) || !rows_at16(out, ldo, width) || !at16(q_norm) || !at16(k_norm) || (x == out && ldx != ldo))
+    return c->fail(OMNI_ERR_INVALID, "null, rows that are not at 16-byte addresses or overlap, or a row stride below %lld", (long long)width);
+  const OnDevice on(c->device);
+  OPS_CUDA(c, launch_qk_norm_rope((const bf16*)x, ldx, (const bf16*)q_norm, (const bf16*)k_norm, pos, rows, q_heads, kv_heads,
+                                  head_dim, eps, theta, (bf16*)out, ldo, c->stream));
+  return OMNI_OK;
+}
+
+int32_t omni_op_kv8_append(omni_ops* c, const void* k, int64_t ldk, const void* v, int64_t ldv, const int32_t* slot,
+                           int32_t rows, void* kv, float* scales, int32_t kv_pages, int32_t kv_heads, int32_t head_dim) {
+  if (!c || rows < 0 || kv_pages < 1) return c ? c->fail(OMNI_ERR_INVALID, "rows < 0 or no pages") : OMNI_ERR_INVALID;
+  if (!heads_fit(kv_heads, kv_heads, head_dim)) return c->fail(OMNI_ERR_UNSUPPORTED, "%d heads of %d: heads of 64 or 128", kv_heads, head_dim);
+  if (rows == 0) return OMNI_OK;
+  const int64_t width = (int64_t)kv_heads * head_dim;
+  if (!k || !v || !slot || !kv || !scales || !rows_at16(k, ldk, width) || !rows_at16(v, ldv, width) || !at16(kv) ||
+      (reinterpret_cast<uintptr_t>(scales) & 7))
+    return c->fail(OMNI_ERR_INVALID, "null, rows or pages that are not at 16-byte addresses, or a row stride below %lld", (long long)width);
+  const OnDevice on(c->device);
+  OPS_CUDA(c, launch_kv8_append((const bf16*)k, ldk, (const bf16*)v, ldv, slot, rows, (uint8_t*)kv, scales, kv_pages, kv_heads,
+                                head_dim, c->err, c->stream));
+  return OMNI_OK;
+}
+
+int32_t omni_op_kv8_attend(omni_ops* c, const void* q, int64_t ldq, const void* kv, const float* scales, int32_t kv_pages,
+                           const int32_t* pos, const int32_t* seq, const int32_t* indptr, int32_t n_seqs,
+                           const int32_t* pages, int32_t n_pages, int32_t rows, int32_t q_heads, int32_t kv_heads,
+                           int32_t head_dim, float scale, void* out, int64_t ldo) {
+  if (!c || rows < 0 || kv_pages < 1 || n_seqs < 0 || n_pages < 0)
+    return c ? c->fail(OMNI_ERR_INVALID, "a negative size, or no pages") : OMNI_ERR_INVALID;
+  if (!heads_fit(q_heads, kv_heads, head_dim))
+    return c->fail(OMNI_ERR_UNSUPPORTED, "%d query heads over %d of %d: whole groups, heads of 64 or 128", q_heads, kv_heads, head_dim);
+  if ((int64_t)rows * q_heads > (1 << 27)) return c->fail(OMNI_ERR_UNSUPPORTED, "%d rows of %d heads: more than 2^27 in all", rows, q_heads);
+  if (rows == 0) return OMNI_OK;
+  const int64_t width = (int64_t)q_heads * head_dim;
+  if (!q || !kv || !scales || !pos || !indptr || (n_pages > 0 && !pages) || !out || !rows_at16(q, ldq, width) ||
+      !rows_at16(out, ldo, width) || !at16(kv) || (reinterpret_cast<uintptr_t>(scales) & 7))
+    return c->fail(OMNI_ERR_INVALID, "null, rows or pages that are not at 16-byte addresses, or a row stride below %lld", (long long)width);
+  const OnDevice on(c->device);
+  const Kv8Attend a{(const bf16*)q, ldq, (const uint8_t*)kv, scales, kv_pages, pos, seq, indptr, pages, n_seqs, n_pages,
+                    rows, q_heads, kv_heads, head_dim, scale, (bf16*)out, ldo};
+  OPS_CUDA(c, launch_kv8_attend(a, c->sm_count, c->err, c->stream));
+  return OMNI_OK;
 }
 
 // ---- streaming codec decoder ---------------------------------------------------------------------------------------

@@ -142,6 +142,12 @@ SYMBOLS = {
     "omni_op_lm_advance": (I32, [VP, VP, VP, C.c_int64, VP, VP, VP, VP, VP, I32]),
     "omni_op_higgs_frame_embed": (I32, [VP, VP, VP, C.c_int64, VP, VP, I32, I32, I32]),
     "omni_op_higgs_sample": (I32, [VP, VP, I32, C.c_float, I32, VP, VP, VP, VP, C.c_int64, VP, I32]),
+    "omni_ops_stream": (I32, [VP, I32, VP]),
+    "omni_op_kv_tables": (I32, [VP, VP, VP, I32, VP, I32, VP, I32, VP, VP, VP, VP, VP, I32, VP, VP, VP, VP, I32, VP]),
+    "omni_op_qk_norm_rope": (I32, [VP, VP, C.c_int64, VP, VP, VP, I32, I32, I32, I32, C.c_float, C.c_float, VP, C.c_int64]),
+    "omni_op_kv8_append": (I32, [VP, VP, C.c_int64, VP, C.c_int64, VP, I32, VP, VP, I32, I32, I32]),
+    "omni_op_kv8_attend": (I32, [VP, VP, C.c_int64, VP, VP, I32, VP, VP, VP, I32, VP, I32, I32, I32, I32, I32, C.c_float,
+                                 VP, C.c_int64]),
     "omni_op_codec_rvq": (I32, [VP, VP, VP, VP, I32, I32, I32]),
     "omni_op_codec_add_norm": (I32, [VP, VP, C.c_int64, VP, VP, VP, I32, I32, C.c_float]),
     "omni_op_codec_window_attend": (I32, [VP, VP, VP, VP, VP, C.c_int64, C.c_int64, VP, I32, I32, C.c_float]),

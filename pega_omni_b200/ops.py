@@ -3,6 +3,8 @@ from __future__ import annotations
 
 import ctypes as C
 
+import torch
+
 from . import lib as L
 
 
@@ -12,6 +14,21 @@ class OpsError(RuntimeError):
 
 def _p(t):
     return None if t is None else C.c_void_p(t.data_ptr())
+
+
+def _need(ok, what):
+    if not ok:
+        raise OpsError(what)
+
+
+def _i32(*tensors):
+    for t in tensors:
+        _need(t is None or (t.dtype is torch.int32 and t.is_contiguous()), "lengths, positions, slots and pages are contiguous int32")
+
+
+def _rows(*tensors):
+    for t in tensors:
+        _need(t.dtype is torch.bfloat16 and t.dim() == 2 and t.stride(1) == 1, "rows are bf16 [rows, heads * head_dim], each contiguous")
 
 
 class Ops:
@@ -157,6 +174,58 @@ class Ops:
         assert books == 8
         self._check(self._lib.omni_op_higgs_sample(self._h, _p(logits), vocab, temperature, top_k, _p(uniforms),
                                                    _p(force), _p(state), _p(lines), stride, _p(codes), rows))
+
+    # ---- 8-bit paged cache (rows: bf16 [rows, heads * head_dim] with any row stride; kv: one byte an element
+    # [pages, kv_heads, 2, 16, head_dim]; scales: f32 [pages, kv_heads, 2]; everything else contiguous int32) ----
+    def stream(self, stream=None):
+        """Later calls run on `stream` (a cudaStream_t as an int, 0: the default stream); None: on the context's own again."""
+        self._check(self._lib.omni_ops_stream(self._h, stream is not None, stream))
+
+    def kv_tables(self, lens, add, table, free_pages, free_count, lens_out, free_count_out, indptr, pages, row_ptr, pos, slot,
+                  seq, status):
+        n, width = table.shape
+        _i32(lens, add, table, free_pages, free_count, lens_out, free_count_out, indptr, pages, row_ptr, pos, slot, seq, status)
+        _need(len(lens) == len(add) == len(lens_out) == n and len(indptr) == len(row_ptr) == n + 1 and
+              len(pos) == len(slot) == len(seq), "one length, addition and table row a sequence; pos, slot and seq of one size")
+        self._check(self._lib.omni_op_kv_tables(self._h, _p(lens), _p(add), n, _p(table), width, _p(free_pages), len(free_pages),
+                                                _p(free_count), _p(lens_out), _p(free_count_out), _p(indptr), _p(pages),
+                                                len(pages), _p(row_ptr), _p(pos), _p(slot), _p(seq), len(pos), _p(status)))
+
+    def qk_norm_rope(self, x, q_norm, k_norm, pos, q_heads, kv_heads, head_dim, eps, theta, out):
+        rows, width = len(pos), (q_heads + kv_heads) * head_dim
+        _rows(x, out)
+        _i32(pos)
+        _need(x.shape[0] == out.shape[0] == rows and x.shape[1] >= width <= out.shape[1], "a position a row, rows of all q and k heads")
+        for gain in (q_norm, k_norm):
+            _need(gain is None or (gain.dtype is torch.bfloat16 and gain.shape == (head_dim,)), "gains are bf16 [head_dim]")
+        self._check(self._lib.omni_op_qk_norm_rope(self._h, _p(x), x.stride(0), _p(q_norm), _p(k_norm), _p(pos), rows, q_heads,
+                                                   kv_heads, head_dim, eps, theta, _p(out), out.stride(0)))
+
+    def _cache(self, kv, scales):
+        pages, heads, two, page, head_dim = kv.shape
+        _need(kv.element_size() == 1 and (two, page) == (2, L.OMNI_PAGE) and kv.is_contiguous() and scales.is_contiguous() and
+              scales.dtype is torch.float32 and scales.shape == (pages, heads, 2),
+              "a cache is [pages, kv_heads, 2, 16, head_dim] of bytes with f32 scales [pages, kv_heads, 2]")
+        return pages, heads, head_dim
+
+    def kv8_append(self, k, v, slot, kv, scales):
+        pages, heads, head_dim = self._cache(kv, scales)
+        _rows(k, v)
+        _i32(slot)
+        _need(k.shape == v.shape == (len(slot), heads * head_dim), "k and v: a row a slot, all kv heads")
+        self._check(self._lib.omni_op_kv8_append(self._h, _p(k), k.stride(0), _p(v), v.stride(0), _p(slot), len(slot), _p(kv),
+                                                 _p(scales), pages, heads, head_dim))
+
+    def kv8_attend(self, q, kv, scales, pos, indptr, pages, q_heads, scale, out, seq=None):
+        kv_pages, kv_heads, head_dim = self._cache(kv, scales)
+        _rows(q, out)
+        _i32(pos, seq, indptr, pages)
+        rows, n_seqs = len(pos), len(indptr) - 1
+        _need(q.shape == out.shape == (rows, q_heads * head_dim) and n_seqs >= 0 and (len(seq) == rows if seq is not None else n_seqs >= rows),
+              "a query row a position, and a sequence for each")
+        self._check(self._lib.omni_op_kv8_attend(self._h, _p(q), q.stride(0), _p(kv), _p(scales), kv_pages, _p(pos), _p(seq),
+                                                 _p(indptr), n_seqs, _p(pages), len(pages), rows, q_heads, kv_heads, head_dim,
+                                                 scale, _p(out), out.stride(0)))
 
     # ---- streaming codec decoder (state: a byte tensor; lines / pos: int32 tensors, one entry per stream) ----
     def codec_rvq(self, codes, books, out, book_rows):
