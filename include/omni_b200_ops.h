@@ -220,6 +220,7 @@ int32_t omni_op_gemm_noalloc(const void* w, int32_t N, int32_t K, const void* x,
  * bf16 (crates/omni-qwen3/kernels/qwen3.cu:109-240). One decoder layer of a call:
  *   omni_op_kv_tables      lengths -> page tables, positions and slots of the call's rows (once for all layers)
  *   omni_op_qk_norm_rope   norm and rotary embedding of the rows' q and k
+ *   omni_op_packed_attend  whole prompts: causal attention over the call's own rows
  *   omni_op_kv8_append     the rows' K and V into the pages
  *   omni_op_kv8_attend     one row a sequence: attention over the pages
  * Cache of a layer: kv[page][kv_head][K | V][16][head_dim] in E4M3 and scales[page][kv_head][K | V] in f32; an element is its
@@ -260,6 +261,15 @@ int32_t omni_op_kv_tables(omni_ops* ctx, const int32_t* lens, const int32_t* add
 int32_t omni_op_qk_norm_rope(omni_ops* ctx, const void* x, int64_t ldx, const void* q_norm, const void* k_norm,
                              const int32_t* pos, int32_t rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                              float eps, float theta, void* out, int64_t ldo);
+
+/* Causal attention within each of n packed sequences: rows indptr[i] .. indptr[i + 1] of q, k and v, of which row r sees the
+ * sequence's rows up to itself: out[r][h] = softmax(scale * q[r][h] . K) V, h over q_heads and K, V those of kv head
+ * h / (q_heads / kv_heads). scale > 0. indptr ascends from any row on; sequences may be empty. Rows outside of the sequences stay
+ * as they are in out, and nothing of them, of other sequences or of later rows reaches a row, not even as a NaN. out must not
+ * overlap q, k or v. */
+int32_t omni_op_packed_attend(omni_ops* ctx, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
+                              int64_t ldv, const int32_t* indptr, int32_t n, int32_t rows, int32_t q_heads,
+                              int32_t kv_heads, int32_t head_dim, float scale, void* out, int64_t ldo);
 
 /* K and V of every row with slot >= 0 into the cache. A page's scale (one for K, one for V of each head) is the smallest 2^e with
  * e >= -100 and |x| <= 448 * 2^e for every finite x put into it. A row at a page's first token starts the page anew; rows further in

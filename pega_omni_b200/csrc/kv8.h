@@ -73,4 +73,22 @@ struct Kv8Attend {
 };
 cudaError_t launch_kv8_attend(const Kv8Attend& a, int sm_count, uint32_t* err, cudaStream_t s);
 
+// ---- prompts ----------------------------------------------------------------------------------------------------------------
+
+// Causal attention within each of n sequences, rows indptr[i] .. indptr[i + 1] of the packed q, k, v; other rows of out stay.
+struct PackedAttend {
+  const bf16* q;
+  int64_t ldq;
+  const bf16* k;
+  int64_t ldk;
+  const bf16* v;
+  int64_t ldv;
+  const int32_t* indptr;
+  int n, rows, q_heads, kv_heads, head_dim;
+  float scale;
+  bf16* out;
+  int64_t ldo;
+};
+cudaError_t launch_packed_attend(const PackedAttend& a, uint32_t* err, cudaStream_t s);
+
 }  // namespace omni

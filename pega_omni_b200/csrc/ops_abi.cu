@@ -529,6 +529,26 @@ int32_t omni_op_qk_norm_rope(omni_ops* c, const void* x, int64_t ldx, const void
   return OMNI_OK;
 }
 
+int32_t omni_op_packed_attend(omni_ops* c, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
+                              int64_t ldv, const int32_t* indptr, int32_t n, int32_t rows, int32_t q_heads,
+                              int32_t kv_heads, int32_t head_dim, float scale, void* out, int64_t ldo) {
+  if (!c || rows < 0 || n < 0) return c ? c->fail(OMNI_ERR_INVALID, "a negative size") : OMNI_ERR_INVALID;
+  if (!heads_fit(q_heads, kv_heads, head_dim))
+    return c->fail(OMNI_ERR_UNSUPPORTED, "%d query heads over %d of %d: whole groups, heads of 64 or 128", q_heads, kv_heads, head_dim);
+  if (!(scale > 0.f && scale <= 1e38f)) return c->fail(OMNI_ERR_INVALID, "a scale that is not above 0, or not finite");
+  if (((int64_t)rows / 128 + n) * q_heads > (1 << 30)) return c->fail(OMNI_ERR_UNSUPPORTED, "%d rows of %d heads in %d sequences: too many", rows, q_heads, n);
+  if (rows == 0 || n == 0) return OMNI_OK;
+  const int64_t width = (int64_t)q_heads * head_dim, kv_width = (int64_t)kv_heads * head_dim;
+  if (!q || !k || !v || !indptr || !out || !rows_at16(q, ldq, width) || !rows_at16(k, ldk, kv_width) || !rows_at16(v, ldv, kv_width) ||
+      !rows_at16(out, ldo, width) || std::max(std::max(ldq, ldk), ldv) >= (1ll << 38))
+    return c->fail(OMNI_ERR_INVALID, "null, rows that are not at 16-byte addresses, or a row stride below %lld (k, v: %lld)", (long long)width, (long long)kv_width);
+  const OnDevice on(c->device);
+  const PackedAttend a{(const bf16*)q, ldq, (const bf16*)k, ldk, (const bf16*)v, ldv, indptr, n, rows, q_heads, kv_heads,
+                       head_dim, scale, (bf16*)out, ldo};
+  OPS_CUDA(c, launch_packed_attend(a, c->err, c->stream));
+  return OMNI_OK;
+}
+
 int32_t omni_op_kv8_append(omni_ops* c, const void* k, int64_t ldk, const void* v, int64_t ldv, const int32_t* slot,
                            int32_t rows, void* kv, float* scales, int32_t kv_pages, int32_t kv_heads, int32_t head_dim) {
   if (!c || rows < 0 || kv_pages < 1) return c ? c->fail(OMNI_ERR_INVALID, "rows < 0 or no pages") : OMNI_ERR_INVALID;

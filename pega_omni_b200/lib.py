@@ -145,6 +145,8 @@ SYMBOLS = {
     "omni_ops_stream": (I32, [VP, I32, VP]),
     "omni_op_kv_tables": (I32, [VP, VP, VP, I32, VP, I32, VP, I32, VP, VP, VP, VP, VP, I32, VP, VP, VP, VP, I32, VP]),
     "omni_op_qk_norm_rope": (I32, [VP, VP, C.c_int64, VP, VP, VP, I32, I32, I32, I32, C.c_float, C.c_float, VP, C.c_int64]),
+    "omni_op_packed_attend": (I32, [VP, VP, C.c_int64, VP, C.c_int64, VP, C.c_int64, VP, I32, I32, I32, I32, I32, C.c_float,
+                                    VP, C.c_int64]),
     "omni_op_kv8_append": (I32, [VP, VP, C.c_int64, VP, C.c_int64, VP, I32, VP, VP, I32, I32, I32]),
     "omni_op_kv8_attend": (I32, [VP, VP, C.c_int64, VP, VP, I32, VP, VP, VP, I32, VP, I32, I32, I32, I32, I32, C.c_float,
                                  VP, C.c_int64]),

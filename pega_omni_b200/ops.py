@@ -201,6 +201,16 @@ class Ops:
         self._check(self._lib.omni_op_qk_norm_rope(self._h, _p(x), x.stride(0), _p(q_norm), _p(k_norm), _p(pos), rows, q_heads,
                                                    kv_heads, head_dim, eps, theta, _p(out), out.stride(0)))
 
+    def packed_attend(self, q, k, v, indptr, q_heads, kv_heads, head_dim, scale, out):
+        rows, n = q.shape[0], len(indptr) - 1
+        _rows(q, k, v, out)
+        _i32(indptr)
+        _need(q.shape == out.shape == (rows, q_heads * head_dim) and k.shape == v.shape == (rows, kv_heads * head_dim) and n >= 0,
+              "q and out: rows of all q heads; k and v: as many of all kv heads")
+        self._check(self._lib.omni_op_packed_attend(self._h, _p(q), q.stride(0), _p(k), k.stride(0), _p(v), v.stride(0),
+                                                    _p(indptr), n, rows, q_heads, kv_heads, head_dim, scale, _p(out),
+                                                    out.stride(0)))
+
     def _cache(self, kv, scales):
         pages, heads, two, page, head_dim = kv.shape
         _need(kv.element_size() == 1 and (two, page) == (2, L.OMNI_PAGE) and kv.is_contiguous() and scales.is_contiguous() and

@@ -32,6 +32,8 @@ APPEND = dict(k=AT, ldk=1024, v=AT, ldv=1024, slot=AT, rows=3, kv=AT, scales=AT,
 ATTEND = dict(q=AT, ldq=2048, kv=AT, scales=AT, kv_pages=9, pos=AT, seq=AT, indptr=AT, n_seqs=2, pages=AT, n_pages=9, rows=2, q_heads=16,
               kv_heads=8, head_dim=128, scale=0.1, out=AT, ldo=2048)
 
+PACKED = dict(q=AT, ldq=4096, k=AT, ldk=4096, v=AT, ldv=4096, indptr=AT, n=2, rows=9, q_heads=16, kv_heads=8, head_dim=128, scale=0.1, out=AT, ldo=2048)
+
 
 @pytest.mark.parametrize("change,status", [
     *[({k: None}, INVALID) for k in ("lens", "add", "table", "free_pages", "free_count", "lens_out", "free_count_out", "indptr", "pages",
@@ -77,12 +79,25 @@ def test_kv8_attend_refuses(call, change, status):
     assert rc == status and why
 
 
+@pytest.mark.parametrize("change,status", [
+    *[({k: None}, INVALID) for k in ("q", "k", "v", "indptr", "out")], *[({k: ODD}, INVALID) for k in ("q", "k", "v", "out")],
+    ({"rows": -1}, INVALID), ({"n": -1}, INVALID), ({"ldq": 2040}, INVALID), ({"ldk": 1016}, INVALID), ({"ldv": 1028}, INVALID),
+    ({"ldo": 2044}, INVALID), ({"ldq": 1 << 40}, INVALID), ({"q_heads": 9}, UNSUPPORTED), ({"kv_heads": 0}, UNSUPPORTED), ({"head_dim": 96}, UNSUPPORTED),
+    ({"scale": -0.1}, INVALID), ({"scale": 0.0}, INVALID), ({"scale": float("nan")}, INVALID), ({"scale": float("inf")}, INVALID), ({"rows": 2**31 - 1, "q_heads": 128}, UNSUPPORTED),
+    ({"n": 2**31 - 1}, UNSUPPORTED),
+])
+def test_packed_attend_refuses(call, change, status):
+    rc, why = call("omni_op_packed_attend", PACKED, **change)
+    assert rc == status and why
+
+
 def test_null_context_is_refused(built_lib):
-    for name, args in (("kv_tables", TABLES), ("qk_norm_rope", ROPE), ("kv8_append", APPEND), ("kv8_attend", ATTEND)):
+    for name, args in (("kv_tables", TABLES), ("qk_norm_rope", ROPE), ("kv8_append", APPEND), ("kv8_attend", ATTEND), ("packed_attend", PACKED)):
         assert getattr(built_lib, "omni_op_" + name)(None, *args.values()) == INVALID
     assert built_lib.omni_ops_stream(None, 1, None) == INVALID
 
 
 def test_no_rows_is_no_call(call):
-    for name, args in (("qk_norm_rope", ROPE), ("kv8_append", APPEND), ("kv8_attend", ATTEND)):
+    for name, args in (("qk_norm_rope", ROPE), ("kv8_append", APPEND), ("kv8_attend", ATTEND), ("packed_attend", PACKED)):
         assert call("omni_op_" + name, args, rows=0)[0] == 0
+    assert call("omni_op_packed_attend", PACKED, n=0)[0] == 0
