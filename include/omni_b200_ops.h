@@ -226,7 +226,9 @@ int32_t omni_op_gemm_noalloc(const void* w, int32_t N, int32_t K, const void* x,
  * Cache of a layer: kv[page][kv_head][K | V][16][head_dim] in E4M3 and scales[page][kv_head][K | V] in f32; an element is its
  * code times its scale. Heads of 64 or 128. Rows of bf16 are given with a stride in elements (ld), a multiple of 8, so that parts
  * of wider rows can be passed; base addresses are multiples of 16 bytes (scales: 8). Zero rows are a call that does nothing.
- * Every call is one kernel, allocates nothing and uses no workspace: it may be captured, and graphs may run side by side.
+ * No call waits for the device or keeps anything for the next, and each has what memory it needs to itself (of these only
+ * omni_op_kv8_attend over few long rows, which takes it from the stream's order): calls may be captured, and graphs and streams
+ * may run side by side, a context's calls being made by one thread at a time.
  * What device arrays hold (lengths, positions, slots, pages) the host does not see; where the kernels find an index outside
  * its table they skip it and raise the device error word. */
 

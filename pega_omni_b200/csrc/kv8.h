@@ -8,11 +8,28 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "util.cuh"
 
 namespace omni {
 
 constexpr int kPageTokens = 16;
+
+// Lets a kernel have `bytes` of dynamic shared memory and clusters of sixteen, once a device.
+template <auto kKernel>
+inline cudaError_t allow_large(int bytes) {
+  static std::atomic<bool> done[64];
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  if (device < 0 || device >= 64) return cudaErrorInvalidDevice;
+  if (done[device].load(std::memory_order_acquire)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) done[device].store(true, std::memory_order_release);
+  return e;
+}
 
 // ---- page tables ------------------------------------------------------------------------------------------------------
 
@@ -71,7 +88,8 @@ struct Kv8Attend {
   bf16* out;
   int64_t ldo;
 };
-cudaError_t launch_kv8_attend(const Kv8Attend& a, int sm_count, uint32_t* err, cudaStream_t s);
+// `pool`: where sums of rows in pieces are kept for the length of the call, in the stream's order.
+cudaError_t launch_kv8_attend(const Kv8Attend& a, int sm_count, cudaMemPool_t pool, uint32_t* err, cudaStream_t s);
 
 // ---- prompts ----------------------------------------------------------------------------------------------------------------
 

@@ -18,6 +18,7 @@
 #include <algorithm>
 
 #include "kv8.h"
+#include "pdl.cuh"
 #include "sm100.cuh"
 
 namespace omni {
@@ -25,18 +26,23 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarps = 8;
 constexpr float kSlack = 8.f;  // powers of two by which a score may pass its reference before the sums are rescaled
 constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kNone = __builtin_huge_valf();  // reference of a row that is not attended to
+
+constexpr int kWarps = 4;
 
 template <int D>
-constexpr int kStages = D == 128 ? 3 : 4;
-template <int D>
 constexpr int kPageBytes = 32 * D;  // K and V of one head
+// CTAs that an SM's registers hold, and pages of a warp's ring, which fill its shared memory then
+template <int NT>
+constexpr int kPerSm = NT == 1 ? 4 : 3;
+template <int D, int NT>
+constexpr int kStages = (NT == 1 ? 3 : 4) * (128 / D);
 
 template <int D, int NT>
 constexpr int smem_bytes() {
-  constexpr int ring = kWarps * kStages<D> * kPageBytes<D>;
+  constexpr int ring = kWarps * kStages<D, NT> * kPageBytes<D>;
   constexpr int merge = (kWarps + 1) * NT * 8 * D * 4;
   return ring > merge ? ring : merge;
 }
@@ -91,48 +97,126 @@ __device__ __forceinline__ uint32_t piece_at(int row, int col) {
 }
 
 struct Part {  // of a query: reference of the scores, of the weights, sum of 2^(s - r)
-  float r, R, l;
+  float r, R, l, unused;
 };
+// Weight of summands under reference x when the largest reference is `top`.
+__device__ __forceinline__ float weight_of(float x, float top) { return x == kNegInf ? 0.f : exp2_of(x - top); }
+// The result from sums under their largest references.
+__device__ __forceinline__ uint2 result_of(float4 v, float r_top, float R_top, float l_sum) {
+  const float f = exp2_of((R_top == kNegInf ? 0.f : R_top) - (r_top == kNegInf ? 0.f : r_top)) / l_sum;
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x * f, v.y * f), hi = __floats2bfloat162_rn(v.z * f, v.w * f);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
+
+// How the work of a call is cut. Without pieces: a cluster a row and kv head (or part of its group), its warps taking turns. With
+// pieces: rows are cut into pieces of about as many pages each as `room` CTAs would have if all pages were dealt out evenly
+// (or a part of that); a row of one piece is finished by its CTA, the sums of others go to `parts` and `sums` for the second
+// kernel. The cut follows from the rows' lengths alone, which every CTA adds up for itself.
+struct Cut {
+  int subgroups, per;  // parts of a group of query heads, heads of a part
+  int room;            // 0: no pieces
+  int least;           // pages of a piece
+  Part* parts;         // [piece][kv head and part][per]
+  float* sums;         // [piece][kv head and part][per][D]
+};
+constexpr int kCutRows = 1024;  // rows at most of a call in pieces
+
+__device__ __forceinline__ int pages_of_row(const Kv8Attend& a, int row) {
+  const int pos = a.pos[row];
+  return pos < 0 ? 0 : min((pos >> 4) + 1, a.n_pages);
+}
+
+struct Piece {
+  int row, index, count, pages;  // of the row's pieces, pages of each
+  int before;                    // pieces of the rows in front
+};
+// The piece with this number, or (by_row) the first of this row; row = -1: there is none. Whole block, kWarps warps.
+__device__ __forceinline__ Piece find_piece(const Kv8Attend& a, const Cut& cut, int number, bool by_row) {
+  __shared__ float sh_pages[kWarps];
+  __shared__ int sh_pieces[kWarps];
+  __shared__ Piece found;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (a.rows + kWarps * 32 - 1) / (kWarps * 32), begin = min(a.rows, tid * per), end = min(a.rows, begin + per);
+  float sum = 0.f;
+  for (int r = begin; r < end; ++r) sum += (float)pages_of_row(a, r);
+  sum = warp_add(sum);
+  if (lane == 0) sh_pages[warp] = sum;
+  if (tid == 0) found.row = -1;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) sum += sh_pages[w];
+  // the rounding of the sum is far below the hundredth
+  const unsigned size = max((unsigned)cut.least, (unsigned)(sum * (float)(a.kv_heads * cut.subgroups) * (1.01f / (float)cut.room)) + 1u);
+  const auto pieces_of = [&](int pages) { return pages <= (int)size ? 1 : (int)(((unsigned)pages + size - 1u) / size); };
+  int mine = 0;
+  for (int r = begin; r < end; ++r) mine += pieces_of(pages_of_row(a, r));
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 31) sh_pieces[warp] = incl;
+  __syncthreads();
+  int before = incl - mine;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) before += w < warp ? sh_pieces[w] : 0;
+  if (by_row ? number >= begin && number < end : number >= before && number < before + mine)
+    for (int r = begin; r < end; ++r) {
+      const int pages = pages_of_row(a, r), n = pieces_of(pages);
+      if (by_row ? r == number : number < before + n) {
+        found = Piece{r, by_row ? 0 : number - before, n, (int)(((unsigned)pages + n - 1u) / n), before};
+        break;
+      }
+      before += n;
+    }
+  __syncthreads();
+  return found;
+}
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, 2) kv8_attend_kernel(const __grid_constant__ Kv8Attend a, int subgroups, int per, uint32_t* err) {
-  constexpr int S = kStages<D>, CW = D / 64;  // pieces of a key's row a lane holds
+__global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(const __grid_constant__ Kv8Attend a, const __grid_constant__ Cut cut, uint32_t* err) {
+  constexpr int S = kStages<D, NT>, CW = D / 64;  // pieces of a key's row a lane holds
   constexpr int STEPS = D / 16;               // matrix instructions of K Q^T; as many of V^T P^T
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Part parts[kWarps][NT * 8], joined[NT * 8];
+  grid_trigger();  // of the second kernel, if there is one
   const cg::cluster_group cluster = cg::this_cluster();
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = warp_index(), g = lane >> 2, t = lane & 3;
-  const int unit = blockIdx.x / ctas;
-  const int groups = a.kv_heads * subgroups;
-  const int row = unit / groups, kh = unit % groups / subgroups, sub = unit % subgroups;
-  const int group = a.q_heads / a.kv_heads, q0 = sub * per, nq = min(per, group - q0);
+  const int subgroups = cut.subgroups, groups = a.kv_heads * subgroups;
+  const int unit = blockIdx.x / ctas, part = unit % groups, kh = part / subgroups, sub = part % subgroups;
+  Piece piece{unit / groups, 0, 1, 0, 0};
+  if (cut.room) {
+    piece = find_piece(a, cut, unit / groups, false);
+    if (piece.row < 0) return;
+  }
+  const int row = piece.row;
+  const int group = a.q_heads / a.kv_heads, q0 = sub * cut.per, nq = min(cut.per, group - q0);
   const int head0 = kh * group + q0;
   bf16* const out = a.out + row * a.ldo + (int64_t)head0 * D;
 
   // the row's tokens and pages
-  int len = a.pos[row] + 1, first = 0;
-  if (len > 0) {
-    const int s = a.seq ? a.seq[row] : row;
-    bool ok = s >= 0 && s < a.n_seqs;
-    if (ok) {
-      first = a.indptr[s];
-      const int last = a.indptr[s + 1];
-      ok = first >= 0 && last <= a.n_pages && (int64_t)last - first >= ((int64_t)len + 15) / 16;
-    }
-    if (!ok) {
-      if (tid == 0) raise(err, kErrBadIndex);
-      len = 0;
-    }
+  const int s_of = a.seq ? a.seq[row] : row, pos = a.pos[row];
+  const bool named = s_of >= 0 && s_of < a.n_seqs;
+  const int first = named ? a.indptr[s_of] : 0, last = named ? a.indptr[s_of + 1] : 0;
+  int len = pos < 0 || pos == 0x7fffffff ? 0 : pos + 1;
+  if (pos >= 0 && !(named && len > 0 && first >= 0 && last <= a.n_pages && (int64_t)last - first >= ((int64_t)len + 15) / 16)) {
+    if (tid == 0) raise(err, kErrBadIndex);
+    len = 0;
   }
-  if (len <= 0) {  // the same for every CTA of the cluster
-    if (rank == 0)
+  if (len == 0) {  // the same for every CTA of the cluster and every piece of the row
+    if (rank == 0 && piece.index == 0)
       for (int i = tid; i < nq * (D / 8); i += kWarps * 32) *reinterpret_cast<uint4*>(out + i * 8) = make_uint4(0, 0, 0, 0);
+    if (piece.count > 1 && tid < cut.per) cut.parts[(int64_t)(piece.before + piece.index) * groups * cut.per + part * cut.per + tid] = Part{kNone, 0.f, 0.f, 0.f};
     return;
   }
-  const int all = (len >> 4) + ((len & 15) != 0), workers = ctas * kWarps, me = rank * kWarps + warp;
-  const int mine = me < all ? (all - me + workers - 1) / workers : 0;
-  const int32_t* const my_pages = a.pages + first + me;
+  const int all = (len >> 4) + ((len & 15) != 0);
+  const int page0 = piece.index * piece.pages, pages_n = piece.count > 1 ? max(0, min(piece.pages, all - page0)) : all;
+  const int workers = ctas * kWarps, me = rank * kWarps + warp;
+  const int mine = me < pages_n ? (pages_n - me + workers - 1) / workers : 0;
+  const int32_t* const my_pages = a.pages + first + page0 + me;
 
   // pages and their scales, thirty-two at a time: lane i holds those of this warp's page 32 b + i
   const auto fetch_id = [&](int b) {
@@ -216,7 +300,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv8_attend_kernel(const __grid
     const uint32_t keys = ring + stage * kPageBytes<D>;
     stage = stage == S - 1 ? 0 : stage + 1;
     const float ks = __shfl_sync(0xffffffffu, sc.x, i & 31), vs = __shfl_sync(0xffffffffu, sc.y, i & 31);
-    const int valid = ks < 0.f ? 0 : len - (me + i * workers) * 16;  // tokens from the page's first on
+    const int valid = ks < 0.f ? 0 : len - (page0 + me + i * workers) * 16;  // tokens from the page's first on
     if (valid <= 0) continue;
 
     float s[NT][4];
@@ -323,15 +407,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv8_attend_kernel(const __grid
       }
     }
   __syncthreads();
-  // weights of summands under references x when the largest is `top`
-  const auto weight = [](float x, float top) { return x == kNegInf ? 0.f : exp2_of(x - top); };
-  const auto finish = [&](int n, int d, float4 v, float r_top, float R_top, float l_sum) {
-    const float f = exp2_of((R_top == kNegInf ? 0.f : R_top) - (r_top == kNegInf ? 0.f : r_top)) / l_sum;
-    uint2 w;
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x * f, v.y * f), hi = __floats2bfloat162_rn(v.z * f, v.w * f);
-    w.x = *reinterpret_cast<const uint32_t*>(&lo), w.y = *reinterpret_cast<const uint32_t*>(&hi);
-    *reinterpret_cast<uint2*>(out + n * D + d) = w;
-  };
   for (int i = tid; i < nq * (D / 4); i += kWarps * 32) {
     const int n = i / (D / 4), d = i % (D / 4) * 4;
     float r_top = kNegInf, R_top = kNegInf, l_sum = 0.f;
@@ -341,16 +416,20 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv8_attend_kernel(const __grid
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const Part p = parts[w][n];
-      l_sum += p.l * weight(p.r, r_top);
-      const float f = weight(p.R, R_top);
+      l_sum += p.l * weight_of(p.r, r_top);
+      const float f = weight_of(p.R, R_top);
       const float4 x = *reinterpret_cast<const float4*>(sums + (w * NT * 8 + n) * D + d);
       v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
     }
-    if (ctas == 1) {
-      finish(n, d, v, r_top, R_top, l_sum);
+    if (piece.count > 1) {
+      const int64_t at = ((int64_t)(piece.before + piece.index) * groups + part) * cut.per + n;
+      *reinterpret_cast<float4*>(cut.sums + at * D + d) = v;
+      if (d == 0) cut.parts[at] = Part{r_top, R_top, l_sum, 0.f};
+    } else if (ctas == 1) {
+      *reinterpret_cast<uint2*>(out + n * D + d) = result_of(v, r_top, R_top, l_sum);
     } else {
       *reinterpret_cast<float4*>(total + n * D + d) = v;
-      if (d == 0) joined[n] = Part{r_top, R_top, l_sum};
+      if (d == 0) joined[n] = Part{r_top, R_top, l_sum, 0.f};
     }
   }
   if (ctas == 1) return;
@@ -365,40 +444,124 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv8_attend_kernel(const __grid
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c = 0; c < ctas; ++c) {
       const Part p = *cluster.map_shared_rank(&joined[n], c);
-      l_sum += p.l * weight(p.r, r_top);
-      const float f = weight(p.R, R_top);
+      l_sum += p.l * weight_of(p.r, r_top);
+      const float f = weight_of(p.R, R_top);
       const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(total, c) + n * D + d);
       v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
     }
-    finish(n, d, v, r_top, R_top, l_sum);
+    *reinterpret_cast<uint2*>(out + n * D + d) = result_of(v, r_top, R_top, l_sum);
   }
   cluster.sync();  // no CTA leaves while another reads its sums
 }
 
+// The sums of a row's pieces, in an order of their own. A CTA a row and query head; D / 4 lanes a piece, as many pieces at a time
+// as there are such groups of lanes.
+template <int D>
+__global__ void __launch_bounds__(kWarps * 32) kv8_join_kernel(const __grid_constant__ Kv8Attend a, const __grid_constant__ Cut cut) {
+  constexpr int LANES = D / 4, GROUPS = kWarps * 32 / LANES;
+  __shared__ float top[2][kWarps];
+  __shared__ float4 v_of[GROUPS][LANES];
+  __shared__ float l_of[GROUPS];
+  const int tid = threadIdx.x, group = a.q_heads / a.kv_heads;
+  const int row = blockIdx.x / a.q_heads, head = blockIdx.x % a.q_heads, kh = head / group, n = head % group % cut.per;
+  const int groups = a.kv_heads * cut.subgroups, part = kh * cut.subgroups + head % group / cut.per;
+  const Piece piece = find_piece(a, cut, row, true);
+  if (piece.count < 2) return;
+  grid_wait();
+  const int64_t step = (int64_t)groups * cut.per, at = (piece.before * (int64_t)groups + part) * cut.per + n;
+  const float4* const parts = reinterpret_cast<const float4*>(cut.parts) + at;
+  float r_top = kNegInf, R_top = kNegInf;
+  for (int c = tid; c < piece.count; c += kWarps * 32) {
+    const float4 p = __ldcg(parts + c * step);
+    r_top = fmaxf(r_top, p.x), R_top = fmaxf(R_top, p.y);
+  }
+  r_top = warp_fmax(r_top), R_top = warp_fmax(R_top);
+  if ((tid & 31) == 0) top[0][tid >> 5] = r_top, top[1][tid >> 5] = R_top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) r_top = fmaxf(r_top, top[0][w]), R_top = fmaxf(R_top, top[1][w]);
+  if (r_top == kNone) return;  // a row that is not attended to: its zeros are there
+  const int g = tid / LANES, d = tid % LANES;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 4
+  for (int c = g; c < piece.count; c += GROUPS) {
+    const float4 p = __ldcg(parts + c * step), x = __ldcg(reinterpret_cast<const float4*>(cut.sums + (at + c * step) * D) + d);
+    l += p.z * weight_of(p.x, r_top);
+    const float f = weight_of(p.y, R_top);
+    v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+  }
+  v_of[g][d] = v;
+  if (d == 0) l_of[g] = l;
+  __syncthreads();
+  if (g > 0) return;
+#pragma unroll
+  for (int i = 1; i < GROUPS; ++i) {
+    const float4 x = v_of[i][d];
+    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w, l += l_of[i];
+  }
+  *reinterpret_cast<uint2*>(a.out + row * a.ldo + (int64_t)head * D + d * 4) = result_of(v, r_top, R_top, l);
+}
+
 template <int D, int NT>
-cudaError_t go(const Kv8Attend& a, int ctas, int subgroups, int per, uint32_t* err, cudaStream_t s) {
+cudaError_t go(const Kv8Attend& a, Cut cut, int ctas, int sm_count, cudaMemPool_t pool, uint32_t* err, cudaStream_t s) {
   constexpr int smem = smem_bytes<D, NT>();
-  const cudaError_t e = cudaFuncSetAttribute(kv8_attend_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_large<kv8_attend_kernel<D, NT>>(smem);
   if (e != cudaSuccess) return e;
+  const int groups = a.kv_heads * cut.subgroups;
+  unsigned units = (unsigned)a.rows * groups;
+  void* scratch = nullptr;
+  if (cut.room) {
+    const int64_t pieces = a.rows + cut.room / groups + 1;
+    const size_t parts = (size_t)pieces * groups * cut.per;
+    e = cudaMallocFromPoolAsync(&scratch, parts * (sizeof(Part) + D * sizeof(float)), pool, s);
+    if (e != cudaSuccess) return e;
+    cut.parts = static_cast<Part*>(scratch), cut.sums = reinterpret_cast<float*>(cut.parts + parts);
+    units = (unsigned)(pieces * groups);
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.rows * a.kv_heads * subgroups * ctas)), cfg.blockDim = dim3(kWarps * 32);
-  cfg.dynamicSmemBytes = smem, cfg.stream = s;
+  cfg.gridDim = dim3(units * ctas), cfg.blockDim = dim3(kWarps * 32), cfg.dynamicSmemBytes = smem, cfg.stream = s;
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = ctas, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
   cfg.attrs = &attr, cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv8_attend_kernel<D, NT>, a, subgroups, per, err);
+  e = cudaLaunchKernelEx(&cfg, kv8_attend_kernel<D, NT>, a, cut, err);
+  if (cut.room) {
+    if (e == cudaSuccess) e = launch_pdl(kv8_join_kernel<D>, dim3((unsigned)a.rows * a.q_heads), dim3(kWarps * 32), 0, s, a, cut);
+    const cudaError_t done = cudaFreeAsync(scratch, s);
+    if (e == cudaSuccess) e = done;
+  }
+  return e;
 }
 
 }  // namespace
 
-cudaError_t launch_kv8_attend(const Kv8Attend& a, int sm_count, uint32_t* err, cudaStream_t s) {
-  const int group = a.q_heads / a.kv_heads, subgroups = (group + 15) / 16, per = (group + subgroups - 1) / subgroups;
-  const int64_t units = (int64_t)a.rows * a.kv_heads * subgroups;
+cudaError_t launch_kv8_attend(const Kv8Attend& a, int sm_count, cudaMemPool_t pool, uint32_t* err, cudaStream_t s) {
+  const int group = a.q_heads / a.kv_heads;
+  Cut cut = {};
+  cut.subgroups = (group + 15) / 16, cut.per = (group + cut.subgroups - 1) / cut.subgroups;
+  const int64_t units = (int64_t)a.rows * a.kv_heads * cut.subgroups;
+  const int64_t held = a.n_pages / std::max(a.n_seqs, 1);  // pages a sequence, as far as the host knows
+  const int64_t at_once = (int64_t)sm_count * (cut.per > 8 ? kPerSm<2> : kPerSm<1>);
+  // Either more CTAs a row as long as all run at once, to a page a warp; or, where they do not, as many as leave each some 40 pages
+  // of 4 KB; or, where clusters of eight leave the machine half empty, pieces. Measured, us, cluster of 1 / 2 / 4 / 8 | pieces:
+  //   rows x kv heads, tokens (heads of 128, groups of 2)
+  //   1 x 8,   777            9.3 /  7.9 /  6.5 /  6.0 |  8
+  //   1 x 8,   60,000         456 /  231 /  119 /   63 | 32
+  //   20 x 8,  500 - 5,000     48 /   32 /   29 /   32 | 28
+  //   64 x 8,  2,000 - 8,000  136 /  129 /  118 /  121 | 120
+  //   128 x 8, 500 - 8,000    200 /  181 /  176 /  206 | 179
+  //   256 x 8, 100 - 2,000    101 /  104 /  137 /  213 | 105
   int ctas = 1;
-  while (ctas < 8 && units * ctas < 4 * sm_count) ctas *= 2;
-  if (a.head_dim == 128) return per > 8 ? go<128, 2>(a, ctas, subgroups, per, err, s) : go<128, 1>(a, ctas, subgroups, per, err, s);
-  if (a.head_dim == 64) return per > 8 ? go<64, 2>(a, ctas, subgroups, per, err, s) : go<64, 1>(a, ctas, subgroups, per, err, s);
+  if (a.rows <= kCutRows && units * 8 <= at_once && held >= 256) {
+    cut.room = (int)(at_once - units), cut.least = 32;
+  } else {
+    while (ctas < 8 && ((units * 2 * ctas <= at_once && held >= 16 && held >= 8 * ctas) || held * a.head_dim >= 80 * 128 * ctas)) ctas *= 2;
+  }
+  const auto run = [&](auto d, auto nt) { return go<decltype(d)::value, decltype(nt)::value>(a, cut, ctas, sm_count, pool, err, s); };
+  using std::integral_constant;
+  if (a.head_dim == 128) return cut.per > 8 ? run(integral_constant<int, 128>(), integral_constant<int, 2>()) : run(integral_constant<int, 128>(), integral_constant<int, 1>());
+  if (a.head_dim == 64) return cut.per > 8 ? run(integral_constant<int, 64>(), integral_constant<int, 2>()) : run(integral_constant<int, 64>(), integral_constant<int, 1>());
   return cudaErrorInvalidValue;
 }
 

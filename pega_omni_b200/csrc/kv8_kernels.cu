@@ -18,7 +18,8 @@ namespace cg = cooperative_groups;
 // the sums for itself (they are a few KB): one launch, no workspace, and the cluster's barrier stands between the last read of
 // the lengths and their overwriting, so a captured step can keep its lengths in place.
 
-constexpr int kTablesThreads = 512;
+constexpr int kTablesThreads = 1024;  // at most
+constexpr int kChunk = 256;            // pages
 
 struct Sums {
   int v[4];
@@ -28,7 +29,7 @@ struct Sums {
   }
 };
 
-// Index i of the prefix array p[0..n] with p[i] <= x < p[i + 1], for 0 <= x < p[n].
+// Index i of the prefix array p[0..n] with p[i] <= x < p[i + 1], which is there.
 __device__ __forceinline__ int owner_of(const int* p, int n, int x) {
   int lo = 0, hi = n - 1;
   while (lo < hi) {
@@ -44,6 +45,7 @@ __device__ __forceinline__ int pages_of(int tokens) { return (tokens >> 4) + ((t
 __global__ void __launch_bounds__(kTablesThreads) kv_tables_kernel(const TablesCall c) {
   extern __shared__ int tables_smem[];
   __shared__ Sums warp_sums[kTablesThreads / 32];
+  const int block = blockDim.x, warps = block >> 5;
   const cg::cluster_group cluster = cg::this_cluster();
   const int n = c.n, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int* const want = tables_smem;        // [n + 1] pages of the sequences in front
@@ -53,7 +55,7 @@ __global__ void __launch_bounds__(kTablesThreads) kv_tables_kernel(const TablesC
   int* const held = back + n + 1;       // [n] tokens held
   const int count = *c.free_count;
 
-  const int per = (n + kTablesThreads - 1) / kTablesThreads, begin = min(n, tid * per), end = min(n, begin + per);
+  const int per = (n + block - 1) / block, begin = min(n, tid * per), end = min(n, begin + per);
   bool bad = false;
   Sums mine = {};
   for (int pass = 0; pass < 2; ++pass) {
@@ -71,8 +73,10 @@ __global__ void __launch_bounds__(kTablesThreads) kv_tables_kernel(const TablesC
       __syncthreads();
       at = incl;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) at.v[i] -= mine.v[i];
-      for (int w = 0; w < warp; ++w) at += warp_sums[w];
+      for (int i = 0; i < 4; ++i) {
+        const int in_front = lane < warp ? warp_sums[lane].v[i] : 0;  // every warp adds them up for itself
+        at.v[i] += __reduce_add_sync(0xffffffffu, in_front) - mine.v[i];
+      }
     }
     for (int s = begin; s < end; ++s) {
       int len, add;
@@ -94,7 +98,7 @@ __global__ void __launch_bounds__(kTablesThreads) kv_tables_kernel(const TablesC
       if (pass) at += one;
       else mine += one;
     }
-    if (pass && tid == kTablesThreads - 1) want[n] = at.v[0], rows[n] = at.v[1], need[n] = at.v[2], back[n] = at.v[3];
+    if (pass && tid == block - 1) want[n] = at.v[0], rows[n] = at.v[1], need[n] = at.v[2], back[n] = at.v[3];
   }
   bad = __syncthreads_or(bad);
   cg::cluster_group::arrival_token all_read = cluster.barrier_arrive();  // this CTA has read the lengths and the count
@@ -106,38 +110,41 @@ __global__ void __launch_bounds__(kTablesThreads) kv_tables_kernel(const TablesC
   if (rows_n > c.row_cap) status |= kTablesRows;
   if (pages_n > c.page_cap) status |= kTablesPages;
   const bool ok = status == 0;
-  const int first = cluster.block_rank() * kTablesThreads + tid, threads = cluster.num_blocks() * kTablesThreads;
+  const int first = cluster.block_rank() * block + tid, threads = cluster.num_blocks() * block;
 
   const auto returned = [&](int k) {  // the k-th page given back
     const int s = owner_of(back, n, k);
     return c.table[(int64_t)s * c.width + (k - back[s])];
   };
-  const auto page_of = [&](int s, int p) {  // page p of sequence s, which is not gone: its own, or one from the top of the stack
-    const int had = pages_of(held[s]);
-    if (p < had) return c.table[(int64_t)s * c.width + p];
-    const int i = count + back_n - 1 - (need[s] + p - had);
+  const auto taken = [&](int j) {  // the j-th page from the top of the stack
+    const int i = count + back_n - 1 - j;
     return i >= count ? returned(i - count) : c.free_pages[i];
   };
-
-  for (int r = first; r < c.row_cap; r += threads) {
-    int pos = -1, slot = -1, seq = -1;
-    if (ok && r < rows_n) {
-      seq = owner_of(rows, n, r);
-      pos = held[seq] + (r - rows[seq]);
-      slot = (int)((uint32_t)page_of(seq, pos >> 4) * kPageTokens + (pos & 15));
+  // a warp takes kChunk pages and rows of a sequence at a time, so a long one among many is shared
+  const int chunks = ok ? (c.width + kChunk - 1) / kChunk : 0;
+  for (int task = cluster.block_rank() * warps + warp; task < n * chunks; task += cluster.num_blocks() * warps) {
+    const int chunk = task / n, s = task - chunk * n, len = held[s], had = pages_of(len), total = want[s + 1] - want[s];
+    const int32_t* const mine = c.table + (int64_t)s * c.width;
+    const int p0 = chunk * kChunk, p1 = min(total, p0 + kChunk), own = min(had, p1);
+#pragma unroll 4
+    for (int p = p0 + lane; p < own; p += 32) c.pages[want[s] + p] = mine[p];
+    for (int p = max(p0, had) + lane; p < p1; p += 32) {
+      const int page = taken(need[s] + p - had);
+      c.pages[want[s] + p] = page, c.table[(int64_t)s * c.width + p] = page;
     }
-    c.pos[r] = pos, c.slot[r] = slot, c.seq[r] = seq;
+    __syncwarp();  // the rows' pages are those that this warp has just entered
+    const int32_t* const pages_of_s = c.pages + want[s];
+    const int pos1 = min(len + (rows[s + 1] - rows[s]), p1 * kPageTokens), to_row = rows[s] - len;
+#pragma unroll 4
+    for (int pos = max(len, p0 * kPageTokens) + lane; pos < pos1; pos += 32) {
+      c.slot[pos + to_row] = (int)((uint32_t)pages_of_s[pos >> 4] * kPageTokens + (pos & 15));
+      c.pos[pos + to_row] = pos, c.seq[pos + to_row] = s;
+    }
   }
-  if (ok) {
-    for (int e = first; e < pages_n; e += threads) {
-      const int s = owner_of(want, n, e), p = e - want[s];
-      const int page = page_of(s, p);
-      c.pages[e] = page;
-      if (p >= pages_of(held[s])) c.table[(int64_t)s * c.width + p] = page;
-    }
-    // what comes back and is not taken again goes on top of the stack, behind the entries that page_of reads
+  for (int r = (ok ? rows_n : 0) + first; r < c.row_cap; r += threads) c.pos[r] = c.slot[r] = c.seq[r] = -1;
+  // what comes back and is not taken again goes on top of the stack, behind the entries that are taken from it
+  if (ok)
     for (int k = first; k < back_n - need_n; k += threads) c.free_pages[count + k] = returned(k);
-  }
   for (int s = first; s <= n; s += threads) c.indptr[s] = ok ? want[s] : 0, c.row_ptr[s] = ok ? rows[s] : 0;
   cluster.barrier_wait(std::move(all_read));
   for (int s = first; s < n; s += threads) {
@@ -151,78 +158,130 @@ __global__ void __launch_bounds__(kTablesThreads) kv_tables_kernel(const TablesC
 }
 
 // ---- norm + rotary embedding --------------------------------------------------------------------------------------------
-// Bound by HBM: every q and k element is read and written once, 16 bytes an access. A thread holds eight pairs (i, i + D / 2) of
-// a head, D / 16 neighbouring lanes a head. The angle of a pair is the same for all heads of a row, so a block makes it once a
-// row: in turns and in f64, since f32 would be off by 2^-24 of a far position's whole angle, and only what is left of a turn
-// goes to f32 and sincospi. All else is f32 with one rounding.
+// Bound by HBM: every q and k element is read and written once, 16 bytes an access. A lane holds eight pairs (i, i + D / 2) of a
+// head, D / 16 neighbouring lanes a head, and a warp takes up to kRopeBatch such loads of one row at a time, all under way before
+// the first is used. The angle of a pair is the same for all heads of a row, so a warp makes each once, under its loads, and a
+// lane keeps its eight: in turns and in f64, since f32 would be off by 2^-24 of a far position's whole angle, and only what is left
+// of a turn goes to f32 and sincospi. All else is f32 with one rounding.
 
 struct Turns {
   double per_pos[64];
 };
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeWarps = 4, kRopeBatch = 2;
 
-template <int D, int ROWS>
-__global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const bf16* x, int64_t ldx, const bf16* __restrict__ q_norm,
-                                                                    const bf16* __restrict__ k_norm, const int32_t* __restrict__ pos,
-                                                                    int rows, int hq, int heads, float eps, const __grid_constant__ Turns turns,
-                                                                    bf16* out, int64_t ldo) {
-  constexpr int LANES = D / 16;  // of a head
-  __shared__ float2 rot[ROWS][D / 2];
-  const int row0 = blockIdx.x * ROWS;
-  for (int i = threadIdx.x; i < ROWS * (D / 2); i += kRopeThreads) {
-    const int r = i / (D / 2), p = i % (D / 2);
-    if (row0 + r < rows) {
-      const double t = (double)pos[row0 + r] * turns.per_pos[p];
-      float2 f;
-      sincospif(2.f * (float)(t - rint(t)), &f.y, &f.x);
-      rot[r][p] = f;
+// Two f32 an instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\nfma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ void pairs_of(const uint4& u, float2 (&v)[4]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+__device__ __forceinline__ uint4 packed_of(const float2 (&v)[4]) {
+  uint4 u;
+  uint32_t* const w = &u.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[i].x, v[i].y);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return u;
+}
+
+// Block y of a row's y_blocks: heads of q where y < q_blocks, otherwise of k.
+template <int D>
+__global__ void __launch_bounds__(kRopeWarps * 32, 7) qk_norm_rope_kernel(const bf16* x, int64_t ldx, const bf16* __restrict__ q_norm,
+                                                                       const bf16* __restrict__ k_norm, const int32_t* __restrict__ pos,
+                                                                       int rows, int hq, int heads, int q_blocks, int y_blocks, float eps,
+                                                                       const __grid_constant__ Turns turns, bf16* out, int64_t ldo) {
+  constexpr int LANES = D / 16, HEADS = 32 / LANES;  // lanes of a head, heads of a warp's access
+  __shared__ float2 rot[kRopeWarps][D / 2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)(blockIdx.x / y_blocks) * kRopeWarps + warp;
+  const int y = blockIdx.x % y_blocks;
+  if (row >= rows) return;
+  const bool is_q = y < q_blocks;
+  const int end = is_q ? hq : heads, at = lane % LANES * 8;
+  const int head0 = (is_q ? y : y - q_blocks) * (HEADS * kRopeBatch) + (is_q ? 0 : hq) + lane / LANES;
+  const int my_pos = pos[row];
+  const bf16* const src = x + row * ldx + head0 * D + at;
+  uint4 lo_raw[kRopeBatch], hi_raw[kRopeBatch];
+#pragma unroll
+  for (int b = 0; b < kRopeBatch; ++b) {
+    lo_raw[b] = hi_raw[b] = make_uint4(0, 0, 0, 0);
+    if (head0 + b * HEADS < end) {
+      lo_raw[b] = *reinterpret_cast<const uint4*>(src + b * HEADS * D), hi_raw[b] = *reinterpret_cast<const uint4*>(src + b * HEADS * D + D / 2);
     }
   }
-  __syncthreads();
-  const int per_row = heads * LANES, tasks = ROWS * per_row;
-  const int at = (threadIdx.x % LANES) * 8;  // a step of the loop is a whole number of heads
-  for (int i = threadIdx.x; i < (tasks + 31) / 32 * 32; i += kRopeThreads) {  // whole warps
-    const int r = i / per_row, head = (i - r * per_row) / LANES;
-    const bool live = i < tasks && row0 + r < rows && pos[row0 + r] >= 0;
-    float lo[8] = {}, hi[8] = {};
-    if (live) {
-      const bf16* src = x + (int64_t)(row0 + r) * ldx + head * D + at;
-      ld8(src, lo), ld8(src + D / 2, hi);
+  const bf16* const gain = is_q ? q_norm : k_norm;
+  uint4 lo_gain = {}, hi_gain = {};
+  if (gain) lo_gain = __ldg(reinterpret_cast<const uint4*>(gain + at)), hi_gain = __ldg(reinterpret_cast<const uint4*>(gain + D / 2 + at));
+  if (my_pos < 0) return;
+#pragma unroll
+  for (int p = lane; p < D / 2; p += 32) {
+    const double t = (double)my_pos * turns.per_pos[p];
+    float2 f;
+    sincospif(2.f * (float)(t - rint(t)), &f.y, &f.x);
+    rot[warp][p] = f;
+  }
+  __syncwarp();
+  // (lo, hi) -> (lo * lc - hi * hs, hi * hc + lo * ls), the gains in the angles
+  float2 lc[4], ls[4], hc[4], hs[4];
+  pairs_of(lo_gain, lc), pairs_of(hi_gain, hc);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float4 f = *reinterpret_cast<const float4*>(&rot[warp][at + 2 * e]);
+    const float2 cs = make_float2(f.x, f.z), sn = make_float2(f.y, f.w), minus = make_float2(-f.y, -f.w);
+    if (gain) ls[e] = mul2(lc[e], sn), hs[e] = mul2(hc[e], minus), lc[e] = mul2(lc[e], cs), hc[e] = mul2(hc[e], cs);
+    else ls[e] = sn, hs[e] = minus, lc[e] = cs, hc[e] = cs;
+  }
+  bf16* const dst = out + row * ldo + head0 * D + at;
+#pragma unroll
+  for (int b = 0; b < kRopeBatch; ++b) {
+    float2 lo[4], hi[4];
+    pairs_of(lo_raw[b], lo), pairs_of(hi_raw[b], hi);
+    float2 rn = make_float2(1.f, 1.f);
+    if (gain) {
+      float2 ss = mul2(lo[0], lo[0]);
+#pragma unroll
+      for (int e = 1; e < 4; ++e) ss = fma2(lo[e], lo[e], ss);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ss = fma2(hi[e], hi[e], ss);
+      float sum = ss.x + ss.y;
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      rn.x = rn.y = rsqrtf(sum * (1.f / D) + eps);
     }
-    const bf16* gain = head < hq ? q_norm : k_norm;
-    float rn = 1.f;
-    float ss = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss += lo[e] * lo[e] + hi[e] * hi[e];
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (live) {
-      if (gain) {
-        rn = rsqrtf(ss / D + eps);
-        float wl[8], wh[8];
-        ld8(gain + at, wl), ld8(gain + D / 2 + at, wh);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) lo[e] = lo[e] * rn * wl[e], hi[e] = hi[e] * rn * wh[e];
-      }
-      float a[8], b[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float2 f = rot[r][at + e];
-        a[e] = lo[e] * f.x - hi[e] * f.y;
-        b[e] = hi[e] * f.x + lo[e] * f.y;
-      }
-      bf16* dst = out + (int64_t)(row0 + r) * ldo + head * D + at;
-      st8(dst, a), st8(dst + D / 2, b);
+    for (int e = 0; e < 4; ++e) {
+      const float2 l = mul2(lo[e], rn), h = mul2(hi[e], rn);
+      lo[e] = fma2(l, lc[e], mul2(h, hs[e])), hi[e] = fma2(h, hc[e], mul2(l, ls[e]));
+    }
+    if (head0 + b * HEADS < end) {
+      *reinterpret_cast<uint4*>(dst + b * HEADS * D) = packed_of(lo);
+      *reinterpret_cast<uint4*>(dst + b * HEADS * D + D / 2) = packed_of(hi);
     }
   }
 }
 
 // ---- append ---------------------------------------------------------------------------------------------------------------
-// A run is what a call puts into one page: neighbouring rows in ascending slots. A block takes the runs that begin in 16 rows
-// (up to 31 rows then: sixteen and what the last run has behind them), of one kv head, K and V; a thread holds eight elements of
-// two rows. Rows of a prompt give one run a block, those of a decode step sixteen of one row: both fill it. The runs' largest
-// magnitudes meet in shared memory, then each run has its scale, and what the page held before is rounded again if that grew.
+// A run is what a call puts into one page: neighbouring rows in ascending slots. A warp takes the runs that begin in 16 rows (up to
+// 31 rows then: sixteen and what the last run has behind them), of K or V of one kv head, and holds their elements in
+// registers: rows of a prompt make one run of them, those of a decode step sixteen of one row, and no warp waits for another. Lane r
+// keeps what there is to know of row r: its slot, the row that begins its run, that run's largest magnitude and scale.
 
 // The smallest 2^e >= 2^-100 with amax <= 448 * 2^e; amax finite, not negative. 448 = 1.75 * 2^8.
 __device__ __forceinline__ float page_scale(float amax) {
@@ -241,101 +300,141 @@ __device__ __forceinline__ uint2 e4m3_of8(const float* v, float mul) {
   return make_uint2(e4m3_of4(v[0] * mul, v[1] * mul, v[2] * mul, v[3] * mul), e4m3_of4(v[4] * mul, v[5] * mul, v[6] * mul, v[7] * mul));
 }
 
+// The largest magnitude of eight bf16 in each half, infinities and (unless there is nothing else) no NaN among them.
+__device__ __forceinline__ __nv_bfloat162 abs_max(const uint4& u) {
+  __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
+  m = __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u.y)));
+  m = __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u.z)));
+  return __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u.w)));
+}
+
+constexpr int kAppendWarps = 4;
+
 template <int D>
-__global__ void __launch_bounds__(2 * D) kv8_append_kernel(const bf16* __restrict__ k, int64_t ldk, const bf16* __restrict__ v,
-                                                           int64_t ldv, const int32_t* __restrict__ slot, int rows, uint8_t* kv,
-                                                           float* scales, int kv_pages, int hk, uint32_t* err) {
-  constexpr int LANES = D / 8;
-  constexpr int kNone = -2;
-  __shared__ int sl[33];             // slots of the row in front of the window and of 32 rows from its first
-  __shared__ uint32_t amax[16][2];   // of the run that begins at a row of the window
-  __shared__ float mul[16][2], ratio[16][2];  // 1 / scale; old scale / new, where it grew over a page that holds tokens
-  const int base = blockIdx.x * 16, head = blockIdx.y, tid = threadIdx.x;
-  if (tid < 33) {
-    const int r = base - 1 + tid;
-    int s = r >= 0 && r < rows ? slot[r] : kNone;
-    if (s >= 0 && (s >> 4) >= kv_pages) {
-      s = kNone;
-      if (head == 0) raise(err, kErrBadIndex);
-    }
-    sl[tid] = s < 0 ? kNone : s;
-    if (tid < 32) amax[tid >> 1][tid & 1] = 0, ratio[tid >> 1][tid & 1] = 1.f;
-  }
-  __syncthreads();
-  const auto leads = [&](int i) { return sl[i + 1] >= 0 && ((sl[i + 1] & 15) == 0 || sl[i] + 1 != sl[i + 1]); };  // row base + i begins a run
-  const int i0 = tid / LANES, at = tid % LANES * 8;
-  float x[2][2][8];  // [row][K | V]
-  int run[2];
+__global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(const bf16* __restrict__ k, int64_t ldk, const bf16* __restrict__ v,
+                                                                       int64_t ldv, const int32_t* __restrict__ slot, int rows, uint8_t* kv,
+                                                                       float* scales, int kv_pages, int hk, int head_blocks, uint32_t* err) {
+  constexpr int LANES = D / 8, TOGETHER = 32 / LANES, STEPS = 16 / TOGETHER;  // lanes of a row, rows of an access, accesses of 16 rows
+  constexpr float kInf = __builtin_huge_valf();
+  __shared__ float row_max[kAppendWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // blocks of the same rows follow one another: neighbouring heads are neighbours in DRAM
+  const int base = blockIdx.x / head_blocks * 16, what = blockIdx.x % head_blocks * kAppendWarps + warp, head = what >> 1, w = what & 1;
+  if (head >= hk) return;
+  const int sub = lane / LANES, at = lane % LANES * 8;
+  const bf16* const src = (w ? v : k) + head * D + at;
+  const int64_t ld = w ? ldv : ldk;
+  // x[pass][i]: row base + 16 pass + i * TOGETHER + sub; the first sixteen are under way before the slots are known
+  uint4 x[2][STEPS];
+  const auto load = [&](int pass, int i) {
+    const int r = base + 16 * pass + i * TOGETHER + sub;
+    x[pass][i] = r < rows ? __ldg(reinterpret_cast<const uint4*>(src + r * ld)) : make_uint4(0, 0, 0, 0);
+  };
 #pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {
-    const int i = i0 + 16 * pass;
-    int l = -1;
-    if (i < 31 && sl[i + 1] >= 0) {
-      l = i;
-      while (l >= 0 && !leads(l)) --l;  // at most 15 rows back, since a run lies in one page
-      if (l >= 16) l = -1;
-    }
-    run[pass] = l;
-    if (l >= 0) {
-      ld8(k + (int64_t)(base + i) * ldk + head * D + at, x[pass][0]);
-      ld8(v + (int64_t)(base + i) * ldv + head * D + at, x[pass][1]);
-    }
-  }
+  for (int i = 0; i < STEPS; ++i) load(0, i);
+  const int64_t limit = (int64_t)kv_pages * 16;
+  const auto slot_of = [&](int r) {  // -2: none
+    const int s = r >= 0 && r < rows ? slot[r] : -2;
+    if (s >= limit) raise(err, kErrBadIndex);
+    return s < 0 || s >= limit ? -2 : s;
+  };
+  const int s = slot_of(base + lane), edge = lane == 0 ? slot_of(base - 1) : -2;
+  int before = __shfl_up_sync(0xffffffffu, s, 1);
+  if (lane == 0) before = edge;
+  const uint32_t leaders = __ballot_sync(0xffffffffu, s >= 0 && ((s & 15) == 0 || before + 1 != s));
+  const int l = 31 - __clz(leaders & (2u << lane) - 1u);  // that begins no later; -1 where the run begins in front of the window
+  const int run = s >= 0 && lane < 31 && l < 16 ? l : -1;
+  const bool mine = run == lane;  // this lane's row begins a run of this warp
+  float* const at_scale = scales + ((int64_t)(max(s, 0) >> 4) * hk + head) * 2 + w;
+  const bool held = mine && (s & 15);  // the page holds tokens of this sequence
+  const float old = held ? *at_scale : 0.f;
+  const uint32_t ours = __ballot_sync(0xffffffffu, run >= 0);
+  const auto skipped = [&](int pass, int i) { return (ours >> (16 * pass + i * TOGETHER) & ((1u << TOGETHER) - 1)) == 0; };  // rows of nobody or of another warp
 #pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {
+  for (int i = 0; i < STEPS; ++i)
+    if (!skipped(1, i)) load(1, i);
+  // the largest magnitudes: of the warp's one run as a prompt gives it, otherwise row by row and run by run
+  const uint32_t runs = leaders & 0xffffu;
+  const bool one = (runs & (runs - 1)) == 0;
+  float m = 0.f;
+  __nv_bfloat162 m2 = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      float m = 0.f;
-      if (run[pass] >= 0) {
+  for (int pass = 0; pass < 2; ++pass)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float a = fabsf(x[pass][w][e]);
-          m = fmaxf(m, a < __int_as_float(0x7f800000) ? a : 0.f);
-        }
+    for (int i = 0; i < STEPS; ++i) {
+      const int r = 16 * pass + i * TOGETHER + sub;
+      if (skipped(pass, i)) continue;
+      const __nv_bfloat162 its = ours >> r & 1 ? abs_max(x[pass][i]) : __floats2bfloat162_rn(0.f, 0.f);
+      m2 = one ? __hmax2(m2, its) : its;
+      if (!one) {
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) m2 = __hmax2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
+        if (at == 0) row_max[warp][r] = fmaxf(__low2float(m2), __high2float(m2));
       }
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      if (run[pass] >= 0 && at == 0) atomicMax(&amax[run[pass]][w], __float_as_uint(m));  // magnitudes order as their bits do
     }
-  }
-  __syncthreads();
-  if (tid < 32 && leads(tid >> 1)) {
-    const int l = tid >> 1, w = tid & 1, s = sl[l + 1];
-    float* const at_scale = scales + ((int64_t)(s >> 4) * hk + head) * 2 + w;
-    float sc = page_scale(__uint_as_float(amax[l][w]));
-    if (s & 15) {  // the page holds tokens of this sequence
-      const float old = *at_scale;
-      sc = fmaxf(sc, old);
-      ratio[l][w] = old / sc;
-    }
-    *at_scale = sc;
-    mul[l][w] = 1.f / sc;
-  }
-  __syncthreads();
+  if (one) {
 #pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {
-    const int l = run[pass];
-    if (l >= 0) {
-      const int s = sl[i0 + 16 * pass + 1];
-      uint8_t* const dst = kv + (((int64_t)(s >> 4) * hk + head) * 32 + (s & 15)) * D + at;
-      *reinterpret_cast<uint2*>(dst) = e4m3_of8(x[pass][0], mul[l][0]);
-      *reinterpret_cast<uint2*>(dst + 16 * D) = e4m3_of8(x[pass][1], mul[l][1]);
-    }
+    for (int o = 16; o > 0; o >>= 1) m2 = __hmax2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
+    m = fmaxf(__low2float(m2), __high2float(m2));
+  } else {
+    __syncwarp();
+    if (run >= 0) m = row_max[warp][lane];
   }
-  for (int l = 0; l < 16; ++l) {
-    if (!leads(l)) continue;
-    const int s = sl[l + 1];
+  if (__any_sync(0xffffffffu, m == kInf)) {  // infinities do not count: once more without
+    __syncwarp();
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const float f = ratio[l][w];
-      if (f != 1.f && i0 < (s & 15)) {
-        uint2* const word = reinterpret_cast<uint2*>(kv + (((int64_t)(s >> 4) * hk + head) * 32 + w * 16 + i0) * D + at);
-        const uint2 u = *word;
-        const float4 a = static_cast<float4>(*reinterpret_cast<const __nv_fp8x4_e4m3*>(&u.x));
-        const float4 b = static_cast<float4>(*reinterpret_cast<const __nv_fp8x4_e4m3*>(&u.y));
-        const float old[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        *word = e4m3_of8(old, f);
+    for (int pass = 0; pass < 2; ++pass)
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        if (skipped(pass, i)) continue;
+        float f[8], its = 0.f;
+        unpack8v(x[pass][i], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) its = fabsf(f[e]) < kInf ? fmaxf(its, fabsf(f[e])) : its;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) its = fmaxf(its, __shfl_xor_sync(0xffffffffu, its, o));
+        if (at == 0) row_max[warp][16 * pass + i * TOGETHER + sub] = its;
       }
+    __syncwarp();
+    m = run >= 0 ? row_max[warp][lane] : 0.f;
+    if (one) m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+  }
+  const uint32_t my_max = __float_as_uint(fmaxf(m, 0.f));  // magnitudes order as their bits do; a row of NaN: 0
+  uint32_t top = my_max;
+  for (uint32_t left = one ? 0 : runs; left; left &= left - 1) {
+    const int r = __ffs(left) - 1;
+    const uint32_t its = __reduce_max_sync(0xffffffffu, run == r ? my_max : 0);
+    if (lane == r) top = its;
+  }
+  float scale = page_scale(__uint_as_float(top)), ratio = 1.f;  // old scale / new, where it grew over a page that holds tokens
+  if (held) scale = fmaxf(scale, old), ratio = old / scale;
+  if (mine) *at_scale = scale;
+  const float mul = __shfl_sync(0xffffffffu, 1.f / scale, max(run, 0));
+  const int64_t to = (((int64_t)(max(s, 0) >> 4) * hk + head) * 32 + w * 16 + (s & 15)) * D;  // of lane r's row
+#pragma unroll
+  for (int pass = 0; pass < 2; ++pass)
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      if (skipped(pass, i)) continue;
+      const int r = 16 * pass + i * TOGETHER + sub;
+      const float by = __shfl_sync(0xffffffffu, mul, r);
+      uint8_t* const dst = kv + (__shfl_sync(0xffffffffu, to, r) + at);
+      if (ours >> r & 1) {
+        float f[8];
+        unpack8v(x[pass][i], f);
+        *reinterpret_cast<uint2*>(dst) = e4m3_of8(f, by);
+      }
+    }
+  for (uint32_t left = __ballot_sync(0xffffffffu, mine && ratio != 1.f); left; left &= left - 1) {
+    const int r = __ffs(left) - 1, its_slot = __shfl_sync(0xffffffffu, s, r);
+    const float by = __shfl_sync(0xffffffffu, ratio, r);
+    for (int t = sub; t < (its_slot & 15); t += TOGETHER) {
+      uint2* const word = reinterpret_cast<uint2*>(kv + (((int64_t)(its_slot >> 4) * hk + head) * 32 + w * 16 + t) * D + at);
+      const uint2 u = *word;
+      const float4 a = static_cast<float4>(*reinterpret_cast<const __nv_fp8x4_e4m3*>(&u.x));
+      const float4 b = static_cast<float4>(*reinterpret_cast<const __nv_fp8x4_e4m3*>(&u.y));
+      const float codes[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      *word = e4m3_of8(codes, by);
     }
   }
 }
@@ -344,13 +443,15 @@ __global__ void __launch_bounds__(2 * D) kv8_append_kernel(const bf16* __restric
 
 cudaError_t launch_kv_tables(const TablesCall& c, cudaStream_t s) {
   const size_t smem = (size_t)(5 * c.n + 4) * sizeof(int);
-  const cudaError_t e = cudaFuncSetAttribute(kv_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (5 * kTablesMaxSeqs + 4) * 4);
+  const cudaError_t e = allow_large<kv_tables_kernel>((5 * kTablesMaxSeqs + 4) * 4);
   if (e != cudaSuccess) return e;
-  // a CTA for every two thousand entries that there may be, eight at most (the portable cluster size)
-  const int64_t entries = (int64_t)c.page_cap + c.row_cap;
-  const unsigned ctas = entries > 16384 ? 8 : entries > 4096 ? 4 : entries > 2048 ? 2 : 1;
+  // a warp for every sequence and for every 128 pages and rows that there may be: sixteen CTAs at most (the largest cluster)
+  const int64_t warps = std::max<int64_t>(c.n, ((int64_t)c.page_cap + c.row_cap) / 128);
+  unsigned ctas = 1;
+  while (ctas < 16 && warps > (int64_t)ctas * 16) ctas *= 2;
+  const unsigned block = warps > 16 * 16 ? kTablesThreads : kTablesThreads / 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(kTablesThreads), cfg.dynamicSmemBytes = smem, cfg.stream = s;
+  cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(block), cfg.dynamicSmemBytes = smem, cfg.stream = s;
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = ctas, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
@@ -362,25 +463,35 @@ cudaError_t launch_qk_norm_rope(const bf16* x, int64_t ldx, const bf16* q_norm, 
                                 int q_heads, int kv_heads, int head_dim, float eps, float theta, bf16* out, int64_t ldo,
                                 cudaStream_t s) {
   Turns turns;
-  for (int i = 0; i < head_dim / 2; ++i)
-    turns.per_pos[i] = std::pow((double)theta, -2.0 * i / head_dim) / 6.283185307179586476925286766559;
-  const auto go = [&](auto kernel, int per) {
-    kernel<<<(rows + per - 1) / per, kRopeThreads, 0, s>>>(x, ldx, q_norm, k_norm, pos, rows, q_heads, q_heads + kv_heads, eps, turns, out, ldo);
+  double low[8];  // theta^(-2 i / head_dim) as a product of two powers
+  for (int i = 0; i < 8; ++i) low[i] = std::pow((double)theta, -2.0 * i / head_dim);
+  for (int i = 0; i < head_dim / 2; i += 8) {
+    const double high = std::pow((double)theta, -2.0 * i / head_dim) / 6.283185307179586476925286766559;
+    for (int j = 0; j < 8; ++j) turns.per_pos[i + j] = high * low[j];
+  }
+  const int per_warp = 32 / (head_dim / 16) * kRopeBatch;  // heads
+  const int q_blocks = (q_heads + per_warp - 1) / per_warp, k_blocks = (kv_heads + per_warp - 1) / per_warp;
+  const unsigned grid = (unsigned)((rows + kRopeWarps - 1) / kRopeWarps) * (q_blocks + k_blocks);
+  const auto go = [&](auto kernel) {
+    kernel<<<grid, kRopeWarps * 32, 0, s>>>(x, ldx, q_norm, k_norm, pos, rows, q_heads, q_heads + kv_heads, q_blocks, q_blocks + k_blocks, eps, turns, out, ldo);
     return cudaGetLastError();
   };
-  const bool many = rows >= 1024;  // rows enough for every SM at four a block
-  if (head_dim == 128) return many ? go(qk_norm_rope_kernel<128, 4>, 4) : go(qk_norm_rope_kernel<128, 1>, 1);
-  if (head_dim == 64) return many ? go(qk_norm_rope_kernel<64, 4>, 4) : go(qk_norm_rope_kernel<64, 1>, 1);
+  if (head_dim == 128) return go(qk_norm_rope_kernel<128>);
+  if (head_dim == 64) return go(qk_norm_rope_kernel<64>);
   return cudaErrorInvalidValue;
 }
 
 cudaError_t launch_kv8_append(const bf16* k, int64_t ldk, const bf16* v, int64_t ldv, const int32_t* slot, int rows, uint8_t* kv,
                               float* scales, int kv_pages, int kv_heads, int head_dim, uint32_t* err, cudaStream_t s) {
-  const dim3 grid((rows + 15) / 16, kv_heads);
-  if (head_dim == 128) kv8_append_kernel<128><<<grid, 256, 0, s>>>(k, ldk, v, ldv, slot, rows, kv, scales, kv_pages, kv_heads, err);
-  else if (head_dim == 64) kv8_append_kernel<64><<<grid, 128, 0, s>>>(k, ldk, v, ldv, slot, rows, kv, scales, kv_pages, kv_heads, err);
-  else return cudaErrorInvalidValue;
-  return cudaGetLastError();
+  const int head_blocks = (2 * kv_heads + kAppendWarps - 1) / kAppendWarps;
+  const unsigned grid = (unsigned)((rows + 15) / 16) * head_blocks;
+  const auto go = [&](auto kernel) {
+    kernel<<<grid, kAppendWarps * 32, 0, s>>>(k, ldk, v, ldv, slot, rows, kv, scales, kv_pages, kv_heads, head_blocks, err);
+    return cudaGetLastError();
+  };
+  if (head_dim == 128) return go(kv8_append_kernel<128>);
+  if (head_dim == 64) return go(kv8_append_kernel<64>);
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace omni

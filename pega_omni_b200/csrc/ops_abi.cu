@@ -23,6 +23,7 @@ struct omni_ops {
   cudaEvent_t ev[2] = {nullptr, nullptr};
   GemmScratch scratch;
   uint32_t* err = nullptr;
+  cudaMemPool_t pool = nullptr;  // what a call needs for its own length, in its stream's order
   std::string error;
   int fail(int code, const char* fmt, ...) {
     char buf[512];
@@ -94,6 +95,12 @@ int32_t omni_ops_create(int32_t device, omni_ops** out) {
   OPS_CUDA(c, cudaMemset(c->scratch.counters, 0, (size_t)c->scratch.counter_slots * 4));
   OPS_CUDA(c, cudaMalloc((void**)&c->err, 256));
   OPS_CUDA(c, cudaMemset(c->err, 0, 256));
+  cudaMemPoolProps props = {};
+  props.allocType = cudaMemAllocationTypePinned;
+  props.location.type = cudaMemLocationTypeDevice, props.location.id = device;
+  OPS_CUDA(c, cudaMemPoolCreate(&c->pool, &props));
+  uint64_t keep = ~0ull;  // freed blocks stay for the next call
+  OPS_CUDA(c, cudaMemPoolSetAttribute(c->pool, cudaMemPoolAttrReleaseThreshold, &keep));
   return OMNI_OK;
 }
 
@@ -104,6 +111,7 @@ void omni_ops_destroy(omni_ops* c) {
   cudaFree(c->scratch.partials);
   cudaFree(c->scratch.counters);
   cudaFree(c->err);
+  if (c->pool) cudaMemPoolDestroy(c->pool);
   if (c->ev[0]) cudaEventDestroy(c->ev[0]);
   if (c->ev[1]) cudaEventDestroy(c->ev[1]);
   if (c->own) cudaStreamDestroy(c->own);
@@ -581,7 +589,7 @@ int32_t omni_op_kv8_attend(omni_ops* c, const void* q, int64_t ldq, const void* 
   const OnDevice on(c->device);
   const Kv8Attend a{(const bf16*)q, ldq, (const uint8_t*)kv, scales, kv_pages, pos, seq, indptr, pages, n_seqs, n_pages,
                     rows, q_heads, kv_heads, head_dim, scale, (bf16*)out, ldo};
-  OPS_CUDA(c, launch_kv8_attend(a, c->sm_count, c->err, c->stream));
+  OPS_CUDA(c, launch_kv8_attend(a, c->sm_count, c->pool, c->err, c->stream));
   return OMNI_OK;
 }
 

@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attend_kernel(const __grid
 
 template <int D>
 cudaError_t go(const PackedAttend& p, const CUtensorMap* maps, const Args& a, uint32_t* err, cudaStream_t s) {
-  const cudaError_t e = cudaFuncSetAttribute(packed_attend_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
+  const cudaError_t e = allow_large<packed_attend_kernel<D>>(Shape<D>::kSmem);
   if (e != cudaSuccess) return e;
   const unsigned units = p.q_heads >> a.tiles_apart;
   packed_attend_kernel<D><<<a.slots * units, kThreads, Shape<D>::kSmem, s>>>(maps[0], maps[1], maps[2], a, err);

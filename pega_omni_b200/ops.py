@@ -13,7 +13,10 @@ class OpsError(RuntimeError):
 
 
 def _p(t):
-    return None if t is None else C.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
+
+
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 
 
 def _need(ok, what):
@@ -21,14 +24,21 @@ def _need(ok, what):
         raise OpsError(what)
 
 
-def _i32(*tensors):
+def _ints(*tensors):
+    """Their addresses: contiguous int32."""
     for t in tensors:
-        _need(t is None or (t.dtype is torch.int32 and t.is_contiguous()), "lengths, positions, slots and pages are contiguous int32")
+        if t.dtype is not _I32 or not t.is_contiguous():
+            raise OpsError("lengths, positions, slots and pages are contiguous int32")
+    return [t.data_ptr() for t in tensors]
 
 
-def _rows(*tensors):
-    for t in tensors:
-        _need(t.dtype is torch.bfloat16 and t.dim() == 2 and t.stride(1) == 1, "rows are bf16 [rows, heads * head_dim], each contiguous")
+def _rows(t, rows, width, at_least=False):
+    """(address, row stride) of bf16 rows, each contiguous."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not _BF16 or len(shape) != 2 or shape[0] != rows or not (shape[1] == width or at_least and shape[1] > width) or \
+            (stride[1] != 1 and width > 1):
+        raise OpsError(f"rows are bf16 [{rows}, {width}], each contiguous: got {t.dtype} {tuple(shape)} with strides {stride}")
+    return t.data_ptr(), stride[0] if rows > 1 else shape[1] + 7 & ~7
 
 
 class Ops:
@@ -184,58 +194,47 @@ class Ops:
     def kv_tables(self, lens, add, table, free_pages, free_count, lens_out, free_count_out, indptr, pages, row_ptr, pos, slot,
                   seq, status):
         n, width = table.shape
-        _i32(lens, add, table, free_pages, free_count, lens_out, free_count_out, indptr, pages, row_ptr, pos, slot, seq, status)
-        _need(len(lens) == len(add) == len(lens_out) == n and len(indptr) == len(row_ptr) == n + 1 and
-              len(pos) == len(slot) == len(seq), "one length, addition and table row a sequence; pos, slot and seq of one size")
-        self._check(self._lib.omni_op_kv_tables(self._h, _p(lens), _p(add), n, _p(table), width, _p(free_pages), len(free_pages),
-                                                _p(free_count), _p(lens_out), _p(free_count_out), _p(indptr), _p(pages),
-                                                len(pages), _p(row_ptr), _p(pos), _p(slot), _p(seq), len(pos), _p(status)))
+        at = _ints(lens, add, table, free_pages, free_count, lens_out, free_count_out, indptr, pages, row_ptr, pos, slot, seq, status)
+        row_cap = pos.numel()
+        _need(lens.numel() == add.numel() == lens_out.numel() == n and indptr.numel() == row_ptr.numel() == n + 1 and
+              slot.numel() == seq.numel() == row_cap, "one length, addition and table row a sequence; pos, slot and seq of one size")
+        self._check(self._lib.omni_op_kv_tables(self._h, at[0], at[1], n, at[2], width, at[3], free_pages.numel(), at[4], at[5],
+                                                at[6], at[7], at[8], pages.numel(), at[9], at[10], at[11], at[12], row_cap, at[13]))
 
     def qk_norm_rope(self, x, q_norm, k_norm, pos, q_heads, kv_heads, head_dim, eps, theta, out):
-        rows, width = len(pos), (q_heads + kv_heads) * head_dim
-        _rows(x, out)
-        _i32(pos)
-        _need(x.shape[0] == out.shape[0] == rows and x.shape[1] >= width <= out.shape[1], "a position a row, rows of all q and k heads")
+        rows, width = pos.numel(), (q_heads + kv_heads) * head_dim
         for gain in (q_norm, k_norm):
-            _need(gain is None or (gain.dtype is torch.bfloat16 and gain.shape == (head_dim,)), "gains are bf16 [head_dim]")
-        self._check(self._lib.omni_op_qk_norm_rope(self._h, _p(x), x.stride(0), _p(q_norm), _p(k_norm), _p(pos), rows, q_heads,
-                                                   kv_heads, head_dim, eps, theta, _p(out), out.stride(0)))
+            _need(gain is None or (gain.dtype is _BF16 and gain.shape == (head_dim,) and gain.is_contiguous()), "gains are bf16 [head_dim]")
+        self._check(self._lib.omni_op_qk_norm_rope(self._h, *_rows(x, rows, width, True), _p(q_norm), _p(k_norm), *_ints(pos), rows,
+                                                   q_heads, kv_heads, head_dim, eps, theta, *_rows(out, rows, width, True)))
 
     def packed_attend(self, q, k, v, indptr, q_heads, kv_heads, head_dim, scale, out):
-        rows, n = q.shape[0], len(indptr) - 1
-        _rows(q, k, v, out)
-        _i32(indptr)
-        _need(q.shape == out.shape == (rows, q_heads * head_dim) and k.shape == v.shape == (rows, kv_heads * head_dim) and n >= 0,
-              "q and out: rows of all q heads; k and v: as many of all kv heads")
-        self._check(self._lib.omni_op_packed_attend(self._h, _p(q), q.stride(0), _p(k), k.stride(0), _p(v), v.stride(0),
-                                                    _p(indptr), n, rows, q_heads, kv_heads, head_dim, scale, _p(out),
-                                                    out.stride(0)))
+        rows, width, kv_width = q.shape[0], q_heads * head_dim, kv_heads * head_dim
+        self._check(self._lib.omni_op_packed_attend(self._h, *_rows(q, rows, width), *_rows(k, rows, kv_width), *_rows(v, rows, kv_width),
+                                                    *_ints(indptr), indptr.numel() - 1, rows, q_heads, kv_heads, head_dim, scale,
+                                                    *_rows(out, rows, width)))
 
     def _cache(self, kv, scales):
         pages, heads, two, page, head_dim = kv.shape
-        _need(kv.element_size() == 1 and (two, page) == (2, L.OMNI_PAGE) and kv.is_contiguous() and scales.is_contiguous() and
-              scales.dtype is torch.float32 and scales.shape == (pages, heads, 2),
+        _need(kv.element_size() == 1 and two == 2 and page == L.OMNI_PAGE and kv.is_contiguous() and scales.is_contiguous() and
+              scales.dtype is _F32 and scales.shape == (pages, heads, 2),
               "a cache is [pages, kv_heads, 2, 16, head_dim] of bytes with f32 scales [pages, kv_heads, 2]")
         return pages, heads, head_dim
 
     def kv8_append(self, k, v, slot, kv, scales):
         pages, heads, head_dim = self._cache(kv, scales)
-        _rows(k, v)
-        _i32(slot)
-        _need(k.shape == v.shape == (len(slot), heads * head_dim), "k and v: a row a slot, all kv heads")
-        self._check(self._lib.omni_op_kv8_append(self._h, _p(k), k.stride(0), _p(v), v.stride(0), _p(slot), len(slot), _p(kv),
-                                                 _p(scales), pages, heads, head_dim))
+        rows, width = slot.numel(), heads * head_dim
+        self._check(self._lib.omni_op_kv8_append(self._h, *_rows(k, rows, width), *_rows(v, rows, width), *_ints(slot), rows,
+                                                 kv.data_ptr(), scales.data_ptr(), pages, heads, head_dim))
 
     def kv8_attend(self, q, kv, scales, pos, indptr, pages, q_heads, scale, out, seq=None):
         kv_pages, kv_heads, head_dim = self._cache(kv, scales)
-        _rows(q, out)
-        _i32(pos, seq, indptr, pages)
-        rows, n_seqs = len(pos), len(indptr) - 1
-        _need(q.shape == out.shape == (rows, q_heads * head_dim) and n_seqs >= 0 and (len(seq) == rows if seq is not None else n_seqs >= rows),
-              "a query row a position, and a sequence for each")
-        self._check(self._lib.omni_op_kv8_attend(self._h, _p(q), q.stride(0), _p(kv), _p(scales), kv_pages, _p(pos), _p(seq),
-                                                 _p(indptr), n_seqs, _p(pages), len(pages), rows, q_heads, kv_heads, head_dim,
-                                                 scale, _p(out), out.stride(0)))
+        at_pos, at_indptr, at_pages = _ints(pos, indptr, pages)
+        rows, width, n_seqs = pos.numel(), q_heads * head_dim, indptr.numel() - 1
+        _need(n_seqs >= rows if seq is None else seq.numel() == rows, "a sequence for each row")
+        self._check(self._lib.omni_op_kv8_attend(self._h, *_rows(q, rows, width), kv.data_ptr(), scales.data_ptr(), kv_pages, at_pos,
+                                                 None if seq is None else _ints(seq)[0], at_indptr, n_seqs, at_pages, pages.numel(),
+                                                 rows, q_heads, kv_heads, head_dim, scale, *_rows(out, rows, width)))
 
     # ---- streaming codec decoder (state: a byte tensor; lines / pos: int32 tensors, one entry per stream) ----
     def codec_rvq(self, codes, books, out, book_rows):

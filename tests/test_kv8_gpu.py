@@ -467,6 +467,30 @@ def test_attend_every_split(ops, rows):
     check_attend(ops, 4, 2, 128, rng.integers(0, 700, rows).tolist(), seed=rows)
 
 
+@pytest.mark.parametrize("hq,hk,d,lens", [
+    (2, 1, 128, [5000]), (9, 1, 64, [4096, 4097]), (17, 1, 128, [9000, 0, 3]), (6, 3, 64, [0, 12001, 1, 0, 700]), (5, 1, 128, [40000]),
+    (4, 4, 64, [6000, 5999, 16, 8192]), (16, 8, 128, [4500, 4111]),
+])
+def test_attend_long_rows_in_pieces(ops, hq, hk, d, lens):
+    """Few rows of many tokens, which are cut into pieces and joined; short and empty rows between them."""
+    check_attend(ops, hq, hk, d, lens, seed=hq + len(lens), loud=3.0)
+
+
+def test_attend_pieces_of_rows_that_are_wrong(ops):
+    """A long row that ends outside its pages is reported and becomes zeros; a page outside the cache is left out; the others stand."""
+    from pega_omni_b200.ops import OpsError
+    hq, hk, d, lens = 4, 2, 64, [9000, 5000, 7000]
+    kv, scales, pages, indptr, q = attend_case(hq, hk, d, lens, 61)
+    want, tol = attend_of(q, kv, scales, pages, indptr, lens, hq, hk, d, 0.1)
+    pages[int(indptr[1]) + 200] = kv.shape[0]
+    out = torch.full((3, hq * d), 3.0, dtype=torch.bfloat16, device="cuda")
+    ops.kv8_attend(q, kv, scales, i32([9010, 4999, 6999]), i32(indptr), i32(pages), hq, 0.1, out)
+    with pytest.raises(OpsError, match="0x2"):
+        ops.sync()
+    got = f64(out)
+    assert (got[0] == 0).all() and np.isfinite(got[1]).all() and (np.abs(got[2] - want[2]) <= tol[2]).all()
+
+
 @pytest.mark.parametrize("loud", [0.01, 10.0, 100.0])
 @pytest.mark.parametrize("spread", [0, 8])
 def test_attend_flat_and_peaked(ops, loud, spread):
@@ -570,9 +594,9 @@ def test_attend_and_append_far_into_a_large_cache(ops):
 
 
 def test_calls_on_two_streams_and_from_graphs(ops):
-    """The calls keep no workspace: two graphs of one context replayed side by side give what each gives by itself."""
+    """No two calls share memory: graphs of one context replayed side by side give what each gives by itself."""
     hq, hk, d = 16, 8, 128
-    cases = [attend_case(hq, hk, d, lens, 60 + i) + (lens,) for i, lens in enumerate(([700, 9, 2000], [1500, 1, 64, 333]))]
+    cases = [attend_case(hq, hk, d, lens, 60 + i) + (lens,) for i, lens in enumerate(([700, 9, 2000], [1500, 1, 64, 333], [9000, 4000], [7000]))]
     want = [run_attend(ops, q, kv, sc, pages, indptr, lens, hq, hk, d, 0.1) for kv, sc, pages, indptr, q, lens in cases]
     held, graphs, streams, outs = [], [], [], []
     for kv, sc, pages, indptr, q, lens in cases:
