@@ -17,6 +17,7 @@
 
 #include <algorithm>
 
+#include "f32x2.cuh"
 #include "kv8.h"
 #include "pdl.cuh"
 #include "sm100.cuh"
@@ -45,12 +46,6 @@ constexpr int smem_bytes() {
   constexpr int ring = kWarps * kStages<D, NT> * kPageBytes<D>;
   constexpr int merge = (kWarps + 1) * NT * 8 * D * 4;
   return ring > merge ? ring : merge;
-}
-
-__device__ __forceinline__ float exp2_of(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {

@@ -20,6 +20,7 @@
 // take it up at the end.
 #include <algorithm>
 
+#include "f32x2.cuh"
 #include "gemm.h"
 #include "kv8.h"
 #include "sm100.cuh"
@@ -31,6 +32,10 @@ constexpr int kTile = 128;
 constexpr int kThreads = 384;
 constexpr int kCopyWarp = 8, kMmaWarp = 9, kGuardWarp = 10;
 constexpr float kLag = 8.f;  // powers of two
+#ifndef KC
+#define KC 0x24
+#endif
+constexpr int kCubic = KC;
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr int kNever = 0x7fffffff;
 
@@ -52,12 +57,6 @@ struct Args {
 };
 
 using namespace sm100;
-
-__device__ __forceinline__ float exp2_of(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // Thirty-two f32 columns of this thread's lane. The registers hold them only behind tmem_ld_done().
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
@@ -117,8 +116,10 @@ __device__ __forceinline__ uint64_t values_desc(uint32_t smem_byte_addr) {
 }
 constexpr uint32_t kRightTransposed = 1u << 16;  // of an instruction descriptor: B with N contiguous
 
+constexpr int kUsed = 4;
+
 struct Bars {
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], v_full[2], v_clean[2], full[8], empty[8], done;
+  uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], v_full[2], v_clean[2], full[8], used[kUsed], done;
 };
 
 template <int D>
@@ -145,15 +146,6 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attend_kernel(const __grid
   for (int i = tid; i < a.n; i += kThreads)
     if (a.indptr[i] / span + i <= slot) atomicMax(&found, i);
   for (int i = tid; i < 3 * D; i += kThreads) (&odd_row[0][0])[i] = kNever;
-  if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_addr(&bars.q_full[i]), 1), mbar_init(smem_addr(&bars.s_full[i]), 1), mbar_init(smem_addr(&bars.p_full[i]), 4);
-      mbar_init(smem_addr(&bars.o_full[i]), 1), mbar_init(smem_addr(&bars.v_full[i]), 1), mbar_init(smem_addr(&bars.v_clean[i]), 2);
-    }
-    mbar_init(smem_addr(&bars.done), 1);
-    for (int i = 0; i < SLOTS; ++i) mbar_init(smem_addr(&bars.full[i]), 1), mbar_init(smem_addr(&bars.empty[i]), 1);
-    mbar_init_fence();
-  }
   __syncthreads();
   const int seq = found;
   if (seq < 0) return;
@@ -177,6 +169,19 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attend_kernel(const __grid
   const int kv_head = head[0] / group, all = max(blocks[0], blocks[1]);
   const int seen_by_all = row0 / kTile;  // blocks of keys before this one are; one block or two are not
 
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_addr(&bars.q_full[i]), 1), mbar_init(smem_addr(&bars.s_full[i]), 1);
+      mbar_init(smem_addr(&bars.p_full[i][0]), 4), mbar_init(smem_addr(&bars.p_full[i][1]), 4);
+      mbar_init(smem_addr(&bars.o_full[i]), 1);
+      mbar_init(smem_addr(&bars.v_full[i]), 1), mbar_init(smem_addr(&bars.v_clean[i]), 2);
+    }
+    for (int i = 0; i < SLOTS; ++i) mbar_init(smem_addr(&bars.full[i]), 1);
+    for (int i = 0; i < kUsed; ++i) mbar_init(smem_addr(&bars.used[i]), 1);
+    mbar_init(smem_addr(&bars.done), 1);
+    mbar_init_fence();
+    prefetch_tensormap(&qmap), prefetch_tensormap(&kmap), prefetch_tensormap(&vmap);
+  }
   if (warp == kMmaWarp) tmem_alloc(smem_addr(&tmem_slot), 512);
   tc_fence_before_sync();
   __syncthreads();
@@ -212,48 +217,66 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attend_kernel(const __grid
 #pragma unroll
         for (int c = 0; c < kTile; ++c) s[c] = c <= limit ? s[c] : kNegInf;
       }
-      float top[4] = {s[0], s[1], s[2], s[3]};
+      // The weights' first half is made under the reference as it is, with the row's maximum beside it, and once more where that turns
+      // out to be too far off. In front of all a maximum comes first.
+      const auto largest = [&] {
+        float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int c = 4; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
-      const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale;
-      const bool over = now > m + kLag;
-      if (__any_sync(0xffffffffu, over)) {
-        const float next = over ? now : m;
-        const float f = m == next ? 1.f : m == kNegInf ? 0.f : exp2_of(m - next);
-        m = next, l *= f;
-        if (j > 0) {
+        for (int c = 4; c + 7 < kTile; c += 8)
 #pragma unroll
-          for (int c = 0; c < D; c += 32) {
-            float o[32];
-            tmem_ld32(o_at + c, o);
-            tmem_ld_done<32>(o);
-            uint32_t r[32];
+          for (int t = 0; t < 4; ++t) top[t] = max3_nan(top[t], s[c + t], s[c + 4 + t]);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(o[e] * f);
-            tmem_st32(o_at + c, r);
-          }
-        }
-      }
-      const float ref = m == kNegInf ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t p[32];
+        for (int t = 0; t < 4; ++t) top[t] = max3_nan(top[t], s[kTile - 4 + t], s[kTile - 4 + t]);
+        return max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3])) * a.scale;
+      };
+      float2 sum[2];
+      uint32_t p[32];
+      const auto weights = [&](int half) {
+        const float2 scale = both(a.scale), minus_ref = both(m == kNegInf ? 0.f : -m);
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           const int c = half * 64 + 2 * e;
-          const float x = exp2_of(fmaf(s[c], a.scale, -ref)), y = exp2_of(fmaf(s[c + 1], a.scale, -ref));
-          sum[(2 * e) & 3] += x, sum[(2 * e + 1) & 3] += y;
-          const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+          const float2 x = fma2(make_float2(s[c], s[c + 1]), scale, minus_ref);
+          const float2 w = kCubic >> (e & 7) & 1 ? exp2_cubic(x) : make_float2(exp2_of(x.x), exp2_of(x.y));
+          sum[e & 1] = add2(sum[e & 1], w);
+          const __nv_bfloat162 h = __floats2bfloat162_rn(w.x, w.y);
           p[e] = *reinterpret_cast<const uint32_t*>(&h);
         }
+      };
+      const auto give = [&](int half) {
         tmem_st32(s_at + half * 32, p);
+        tmem_st_done();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(bars.p_full[i][half]));
+      };
+      if (j == 0) m = largest();
+      sum[0] = sum[1] = both(0.f);
+      weights(0);
+      const float now = largest();
+      if (__any_sync(0xffffffffu, now > m + kLag)) {
+        const float next = now > m + kLag ? now : m;
+        const float f = m == next ? 1.f : m == kNegInf ? 0.f : exp2_of(m - next);
+        m = next, l *= f;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          tmem_ld32(o_at + c, o);
+          tmem_ld_done<32>(o);
+          uint32_t r[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(o[e] * f);
+          tmem_st32(o_at + c, r);
+        }
+        sum[0] = sum[1] = both(0.f);
+        weights(0);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st_done();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(bars.p_full[i]));
+      give(0);
+      weights(1);
+      give(1);
+      sum[0] = add2(sum[0], sum[1]);
+      // a score that is no number, or infinite: neither is the sum
+      l += sum[0].x + sum[0].y + (now == kNegInf ? 0.f : now - now);
     }
     if (ok && blocks_i) ok = mbar_wait(bar(bars.o_full[i]), 0, err);
     for (int j = seen_by_all; j < all && ok && blocks_i; ++j) ok = mbar_wait(bar(bars.v_clean[j - seen_by_all]), 0, err);
@@ -294,10 +317,13 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attend_kernel(const __grid
         mbar_expect_tx(bar(bars.q_full[i]), BYTES);
         tma_load_3d(q_at + i * BYTES, &qmap, bar(bars.q_full[i]), 0, first + begin[i], head[i] * (D / 64), kEvictFirst);
       }
-      for (int item = 0; item < 2 * all && ok; ++item) {
-        const int s = item % SLOTS, round = item / SLOTS;
-        if (round > 0) ok = mbar_wait(bar(bars.empty[s]), (round - 1) & 1, err);
-        if (!ok) break;
+      for (int item = 0; item < 2 * all; ++item) {
+        if (item >= SLOTS) {  // what the slot held was used up in this turn
+          const int turn = (item - SLOTS - 1) / 2;
+          ok = mbar_wait(bar(bars.used[turn % kUsed]), (turn / kUsed) & 1, err);
+          if (!ok) break;
+        }
+        const int s = item % SLOTS;
         const uint32_t full = filling(item);
         mbar_expect_tx(full, BYTES);
         tma_load_3d(ring + s * BYTES, item & 1 ? &vmap : &kmap, full, 0, first + (item >> 1) * kTile, kv_head * (D / 64), kEvictLast);
@@ -310,9 +336,9 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attend_kernel(const __grid
       }
     }
   } else if (warp == kMmaWarp) {
+    // one thread for both tiles, in turns: it keeps them apart, so that one's products run under the other's exponentials
     if (elect_one()) {
       constexpr uint32_t kScores = idesc_bf16_f32(kTile, kTile), kSums = idesc_bf16_f32(kTile, D) | kRightTransposed;
-      bool ok = true;
       const auto scores = [&](int i, int j) {  // S of tile i against keys j
         const uint32_t q = q_at + i * BYTES, k = ring + (2 * j % SLOTS) * BYTES;
 #pragma unroll
@@ -322,41 +348,50 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attend_kernel(const __grid
         }
         mma_commit(bar(bars.s_full[i]));
       };
-      ok = filled(0);
+      // Turn j: P V(j) and S(j + 1) of both tiles. What it needs of the ring was waited for in the turn before, between the tiles.
+      const auto ready = [&](int j) {
+        const bool v = j < seen_by_all ? filled(2 * j + 1) : mbar_wait(bar(bars.v_clean[j - seen_by_all]), 0, err);
+        return v && (j + 1 >= all || filled(2 * j + 2));
+      };
+      bool ok = filled(0);
       for (int i = 0; i < 2 && ok; ++i) {
         if (!blocks[i]) continue;
         ok = mbar_wait(bar(bars.q_full[i]), 0, err);
+        if (!ok) break;
         tc_fence_after_sync();
-        if (ok) scores(i, 0);
+        scores(i, 0);
       }
-      const auto release = [&](int item) {
-        if (item + SLOTS < 2 * all) mma_commit(bar(bars.empty[item % SLOTS]));
-      };
-      if (ok) release(0);
+      ok = ok && ready(0);
+      uint32_t v = ring + BYTES;
       for (int j = 0; j < all && ok; ++j) {
-        ok = j < seen_by_all ? filled(2 * j + 1) : mbar_wait(bar(bars.v_clean[j - seen_by_all]), 0, err);
-        if (ok && j + 1 < all) ok = filled(2 * j + 2);
         for (int i = 0; i < 2 && ok; ++i) {
-          if (j >= blocks[i]) continue;
-          ok = mbar_wait(bar(bars.p_full[i]), j & 1, err);
-          if (!ok) break;
-          tc_fence_after_sync();
-          const uint32_t v = ring + ((2 * j + 1) % SLOTS) * BYTES;
+          if (j < blocks[i]) {
+            for (int half = 0; half < 2 && ok; ++half) {  // of the block's keys, whose weights come in turn
+              ok = mbar_wait(bar(bars.p_full[i][half]), j & 1, err);
+              if (!ok) break;
+              tc_fence_after_sync();
 #pragma unroll
-          for (int x = 0; x < kTile / 16; ++x)
-            mma_bf16_ta(tmem + 256 + i * kTile, tmem + i * kTile + x * 8, values_desc(v + x * 2048), kSums, j > 0 || x > 0);
-          if (j + 1 < blocks[i]) scores(i, j + 1);
-          else mma_commit(bar(bars.o_full[i]));
+              for (int x = 0; x < kTile / 32; ++x) {
+                const int k = half * (kTile / 32) + x;
+                mma_bf16_ta(tmem + 256 + i * kTile, tmem + i * kTile + k * 8, values_desc(v + k * 2048), kSums, j > 0 || k > 0);
+              }
+            }
+            if (!ok) break;
+            if (j + 1 < blocks[i]) scores(i, j + 1);
+            else mma_commit(bar(bars.o_full[i]));
+          }
+          if (i == 0 && j + 1 < all) ok = ready(j + 1);
         }
         if (!ok) break;
-        release(2 * j + 1), release(2 * j + 2);
+        if (2 * j + SLOTS < 2 * all) mma_commit(bar(bars.used[j % kUsed]));  // items wait for it
+        v = v + 2 * BYTES >= ring + SLOTS * BYTES ? v + 2 * BYTES - SLOTS * BYTES : v + 2 * BYTES;
       }
       if (!ok) {  // what is under way uses shared memory and TMEM
         mma_commit(bar(bars.done));
         mbar_wait(bar(bars.done), 0, err);
       }
     }
-  } else if (warp >= kGuardWarp) {
+  } else {
     const int t = tid - kGuardWarp * 32;
     for (int j = seen_by_all; j < all; ++j) {
       const int item = 2 * j + 1;
