@@ -40,16 +40,4 @@ __device__ __forceinline__ float exp2_of(float x) {
   return y;
 }
 
-// 2^x on the pipe that multiplies, to 1.02e-4 of the value: x = n + f with n whole and |f| <= 1/2, and 2^f from the cubic with value 1
-// at 0 whose largest relative error there is smallest. 0 from -127 down; x below 128. A NaN comes out as a number.
-__device__ __forceinline__ float2 exp2_cubic(float2 x) {
-  const float kWhole = 12582912.f;  // 1.5 * 2^23: a sum with it has n in its low bits
-  const float2 y = make_float2(fmaxf(x.x, -127.f), fmaxf(x.y, -127.f));
-  const float2 t = add2(y, both(kWhole)), f = fma2(add2(t, both(-kWhole)), both(-1.f), y);
-  float2 p = fma2(f, both(0.05500905960798264f), both(0.2422109693288803f));
-  p = fma2(p, f, both(0.6932829022407532f));
-  p = fma2(p, f, both(1.f));
-  return make_float2(__int_as_float((__float_as_int(t.x) << 23) + __float_as_int(p.x)), __int_as_float((__float_as_int(t.y) << 23) + __float_as_int(p.y)));
-}
-
 }  // namespace omni

@@ -107,6 +107,6 @@ struct PackedAttend {
   bf16* out;
   int64_t ldo;
 };
-cudaError_t launch_packed_attend(const PackedAttend& a, uint32_t* err, cudaStream_t s);
+cudaError_t launch_packed_attend(const PackedAttend& a, int sm_count, uint32_t* err, cudaStream_t s);
 
 }  // namespace omni

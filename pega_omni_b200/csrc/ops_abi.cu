@@ -553,7 +553,7 @@ int32_t omni_op_packed_attend(omni_ops* c, const void* q, int64_t ldq, const voi
   const OnDevice on(c->device);
   const PackedAttend a{(const bf16*)q, ldq, (const bf16*)k, ldk, (const bf16*)v, ldv, indptr, n, rows, q_heads, kv_heads,
                        head_dim, scale, (bf16*)out, ldo};
-  OPS_CUDA(c, launch_packed_attend(a, c->err, c->stream));
+  OPS_CUDA(c, launch_packed_attend(a, c->sm_count, c->err, c->stream));
   return OMNI_OK;
 }
 

@@ -1,18 +1,27 @@
 // Causal attention over packed prompts on the tensor cores (kv8.h).
 //
-// Bound by the tensor cores, next to it by the exponentials: a block of 128 queries and 128 keys is two products of
-// 128 x 128 x D and 16,384 exponentials, which an SM makes 16 a clock. A CTA works on two tiles of 128 queries that share their keys
-// - two heads of one group where the group is even, otherwise 256 rows of one head - so a block of K and V is fetched once for
-// both, and one tile's products run under the other tile's softmax.
+// Bound by the tensor cores and the exponentials alike: a block of 128 queries and 128 keys is two products of 128 x 128 x D and
+// 16,384 exponentials, which an SM makes 16 a clock. TMEM holds a tile's 128 columns of scores S, whose first 64 the weights P take
+// over (bf16, the left operand of P V), and D columns of O. A tile's matrix instructions run in their order - S(0) | P V(0) S(1) |
+// P V(1) S(2) .., each group when its P is there - so S(j + 1) having arrived says that P V(j) is done with O, and no other barrier guards it.
+// Softmax has a thread a row of a tile; one warp copies, one issues matrix instructions, two look through values (below).
 //
-// Warps 0-3 and 4-7: the softmax of a tile, a thread a row. Warp 8: copies. Warp 9: matrix instructions. Warps 10 and 11: values
-// behind the diagonal. TMEM: per tile 128 columns of scores S, whose first 64 the weights P take over (bf16, the left operand of
-// P V), and D columns of O. A tile's instructions are issued as S(0) | P V(0) S(1) | P V(1) S(2) ..., each group when its
-// P is there; since they run in order, S(j + 1) having arrived says that P V(j) is done with O, and no other barrier guards it.
+// Two kernels, by the sequences' mean length. Both have two tiles of 128 queries on an SM, one's products under the other's exponentials.
+//  - long_kernel: one CTA, whose tiles share their keys: two heads of a group where the group is even, otherwise 256 rows of one
+//    head. A block of K and V is fetched once for both.
+//  - short_kernel: two CTAs of a tile each, which stay and take items (128 rows of a sequence and head) in turns, the longest first and
+//    back and forth: an item's Q and K are fetched and its first scores made under the end of the one before. It reads K and V
+//    twice as often.
+// us, long | short, 16 heads of 128 over 8: 28 sequences of 32 to 512 tokens 47 | 39, 16 of 512 52 | 44, 8 of 1,024 66 | 59, 4 of 2,048
+// 79 | 84, 2 of 4,096 126 | 141, 1 of 8,192 229 | 274; 64 of 1 to 120, 14 heads of 64 over 2: 38 | 19.
+// Of a turn of long_kernel (a block of keys for both tiles, 2,900 clocks) the tensor cores have work for 2,050, the exponentials' pipe as
+// much; the rest is the way from the last weights to the next scores. The clock is what power leaves at this rate: 8,192 tokens of
+// 32 heads take 480 us, for 1.9 GHz it would be 380. A cubic for every eighth or fourth exponential, two threads a row, an issuing
+// warp a tile (which lets both tiles fall into step) and weights in unequal parts made it no faster.
 //
 // Scores, maxima, sums and O are f32. Weights go to bf16 because V does (one type for both operands): 2^-8 at most of a weight,
 // which averages out over a row's keys and is what the result itself is rounded by. A row's reference is a maximum that may lag by
-// 2^8 behind the true one, so O is rarely rescaled.
+// 2^8 behind the true one, so O is rarely rescaled, and the weights need not wait for the maximum.
 //
 // A weight of 0 does not silence a NaN or an infinity in V. Where a block has keys that some row must not see (the diagonal, the
 // rows behind the sequence's end, which are another sequence's) two warps look through it before it is used: rows behind the end become 0;
@@ -29,34 +38,24 @@ namespace omni {
 namespace {
 
 constexpr int kTile = 128;
-constexpr int kThreads = 384;
-constexpr int kCopyWarp = 8, kMmaWarp = 9, kGuardWarp = 10;
 constexpr float kLag = 8.f;  // powers of two
-#ifndef KC
-#define KC 0x24
-#endif
-constexpr int kCubic = KC;
 constexpr float kNegInf = -__builtin_huge_valf();
-constexpr int kNever = 0x7fffffff;
-
-template <int D>
-struct Shape {
-  static constexpr int kTileBytes = kTile * D * 2;
-  static constexpr int kSlots = D == 128 ? 5 : 8;
-  static constexpr int kSmem = (2 + kSlots) * kTileBytes + 1024;  // and what the ring's alignment costs
-};
 
 struct Args {
   const int32_t* indptr;
   int n, rows, q_heads, kv_heads;
-  int tiles_apart;  // 1: a CTA's tiles are neighbouring heads, 0: neighbouring rows of one head
-  int slots;        // places for blocks of rows in the grid
-  float scale;      // of scores in powers of two
+  float scale;  // of scores in powers of two
   bf16* out;
   int64_t ldo;
+  int apart;  // long_kernel: 1: a CTA's tiles are neighbouring heads, 0: neighbouring rows of one head
+  int shift;  // log2 of a CTA's rows
+  int slots;  // places for blocks of rows in the grid
 };
 
 using namespace sm100;
+
+template <int D>
+constexpr int kTileBytes = kTile * D * 2;
 
 // Thirty-two f32 columns of this thread's lane. The registers hold them only behind tmem_ld_done().
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
@@ -78,15 +77,12 @@ __device__ __forceinline__ void tmem_ld_done(float* v) {
 #pragma unroll
   for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i])::"memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, "
-      "%27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
-      "r"(r[31])
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -116,345 +112,657 @@ __device__ __forceinline__ uint64_t values_desc(uint32_t smem_byte_addr) {
 }
 constexpr uint32_t kRightTransposed = 1u << 16;  // of an instruction descriptor: B with N contiguous
 
-constexpr int kUsed = 4;
+
+// ---- what the kernels share ---------------------------------------------------------------------------------------------
+
+// S of a tile: Q and K as they lie in shared memory.
+template <int D>
+__device__ __forceinline__ void issue_scores(uint32_t s, uint32_t q, uint32_t k) {
+  constexpr uint32_t kShape = idesc_bf16_f32(kTile, kTile);
+#pragma unroll
+  for (int x = 0; x < D / 16; ++x) {
+    const uint32_t at = (x >> 2) * (kTile * 128) + (x & 3) * 32;
+    mma_bf16(s, kmajor_sw128_desc(q + at), kmajor_sw128_desc(k + at), kShape, x > 0);
+  }
+}
+// O (+)= P V for half of a block's keys.
+template <int D>
+__device__ __forceinline__ void issue_sums(uint32_t o, uint32_t p, uint32_t v, int half, bool first) {
+  constexpr uint32_t kShape = idesc_bf16_f32(kTile, D) | kRightTransposed;
+#pragma unroll
+  for (int x = 0; x < kTile / 32; ++x) {
+    const int k = half * (kTile / 32) + x;
+    mma_bf16_ta(o, p + k * 8, values_desc(v + k * 2048), kShape, !first || k > 0);
+  }
+}
+
+// A row's reference and the sum of its weights.
+struct Row {
+  float m = kNegInf, l = 0.f;
+};
+// Weights of a block, whose scores have arrived: give(0) and give(1) when half of them are in TMEM. `first`: there is no O yet;
+// `seen`: the last key that the row sees.
+template <int D, typename Give>
+__device__ __forceinline__ void make_weights(Row& row, uint32_t s_at, uint32_t o_at, float scale_to_2, bool first, bool diagonal, int seen, Give&& give) {
+  float s[kTile];
+#pragma unroll
+  for (int c = 0; c < kTile; c += 32) tmem_ld32(s_at + c, s + c);
+  tmem_ld_done<kTile>(s);
+  if (diagonal) {
+#pragma unroll
+    for (int c = 1; c < kTile; ++c) s[c] = c <= seen ? s[c] : kNegInf;
+  }
+  const auto largest = [&] {
+    float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+    for (int c = 4; c + 7 < kTile; c += 8)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) top[t] = max3_nan(top[t], s[c + t], s[c + 4 + t]);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) top[t] = max3_nan(top[t], s[kTile - 4 + t], s[kTile - 4 + t]);
+    return max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3])) * scale_to_2;
+  };
+  float2 sum[2];
+  const auto weights = [&](int q) {  // of a quarter of the keys
+    const float2 scale = both(scale_to_2), minus_ref = both(row.m == kNegInf ? 0.f : -row.m);
+    uint32_t p[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int c = q * 32 + 2 * e;
+      const float2 x = fma2(make_float2(s[c], s[c + 1]), scale, minus_ref), w = make_float2(exp2_of(x.x), exp2_of(x.y));
+      sum[e & 1] = add2(sum[e & 1], w);
+      const __nv_bfloat162 h = __floats2bfloat162_rn(w.x, w.y);
+      p[e] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    tmem_st16(s_at + q * 16, p);
+  };
+  const auto done = [&](int half) {
+    tmem_st_done();
+    tc_fence_before_sync();
+    __syncwarp();
+    give(half);
+  };
+  // The first half is made under the reference as it is, with the row's maximum beside it, and once more where that turns out to be
+  // too far off. In front of all a maximum comes first.
+  float now;
+  if (first) row.m = now = largest();
+#pragma unroll 1
+  for (;;) {
+    sum[0] = sum[1] = both(0.f);
+    weights(0), weights(1);
+    if (first) break;
+    now = largest();
+    const bool over = now > row.m + kLag;
+    if (!__any_sync(0xffffffffu, over)) break;
+    const float next = over ? now : row.m;
+    const float f = row.m == next ? 1.f : row.m == kNegInf ? 0.f : exp2_of(row.m - next);
+    row.m = next, row.l *= f;
+#pragma unroll 1
+    for (int c = 0; c < D; c += 16) {
+      float o[16];
+      tmem_ld16(o_at + c, o);
+      uint32_t r[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(o[e] * f);
+      tmem_st16(o_at + c, r);
+    }
+  }
+  done(0);
+  weights(2), weights(3);
+  done(1);
+  sum[0] = add2(sum[0], sum[1]);
+  // a score that is no number, or infinite: neither is the sum
+  row.l += sum[0].x + sum[0].y + (now == kNegInf ? 0.f : now - now);
+}
+
+// The warp's rows of O over the sums of their weights, `rows` of them at most, to dst. sees(kind, column): the row takes up
+// a NaN (0), an infinity (1), a negative infinity (2), asked where `odd`. Through 2 KB of shared memory, 16 bytes of a row in an
+// order of its own: the warp then writes 64 bytes of eight rows at a time, not 16 of 32.
+template <int D, typename Sees>
+__device__ __forceinline__ void write_rows(uint32_t o_at, float l, bool odd, Sees&& sees, unsigned char* stage, bf16* dst, int64_t ldo, int rows, int lane) {
+  const float f = 1.f / l;
+#pragma unroll 1
+  for (int c = 0; c < D; c += 32) {
+    float o[32];
+    tmem_ld32(o_at + c, o);
+    tmem_ld_done<32>(o);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o[e] *= f;
+    if (odd) {
+#pragma unroll 1
+      for (int e = 0; e < 32; ++e) {
+        float add = 0.f;
+        if (sees(1, c + e)) add += __builtin_huge_valf();
+        if (sees(2, c + e)) add -= __builtin_huge_valf();
+        if (sees(0, c + e)) add = __int_as_float(0x7fffffff);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] += k == e ? add : 0.f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(stage + lane * 64 + ((e ^ (lane >> 1 & 3)) << 4)) = pack8v(o + 8 * e);
+    __syncwarp();
+    uint4 u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = e * 8 + (lane >> 2);
+      u[e] = *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4));
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = e * 8 + (lane >> 2);
+      if (r < rows) *reinterpret_cast<uint4*>(dst + r * ldo + c + (lane & 3) * 8) = u[e];
+    }
+    __syncwarp();
+  }
+}
+
+// Looks through a block of V, thread t of 64: rows from `keys` on become 0, what is not finite in front of them too, behind
+// note(kind, column, row of the block).
+template <int D, typename Note>
+__device__ __forceinline__ void look_through(unsigned char* v, int keys, int t, Note&& note) {
+  const int own = min(keys, kTile) * 8;  // pieces of 16 bytes of 64 columns
+  __nv_bfloat162 most = __floats2bfloat162_rn(0.f, 0.f);
+  for (int half = 0; half < D / 64; ++half) {
+    uint4* const at = reinterpret_cast<uint4*>(v) + half * (kTile * 8);
+#pragma unroll 4
+    for (int i = t; i < own; i += 64) {
+      const uint4 u = at[i];
+      const __nv_bfloat162* const w = reinterpret_cast<const __nv_bfloat162*>(&u);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) most = __hmax2_nan(most, __habs2(w[e]));
+    }
+    for (int i = own + t; i < kTile * 8; i += 64) at[i] = make_uint4(0, 0, 0, 0);
+  }
+  // infinities and NaN are among the largest magnitudes: once more, piece by piece
+  const float low = __low2float(most), high = __high2float(most);
+  if (!(low < __builtin_huge_valf() && high < __builtin_huge_valf())) {
+#pragma unroll 1
+    for (int i = t; i < D / 64 * own; i += 64) {
+      const int half = i / own, at = i - half * own, r = at >> 3, col = half * 64 + (((at & 7) ^ (r & 7)) << 3);
+      bf16* const w = reinterpret_cast<bf16*>(v + half * (kTile * 128) + at * 16);
+#pragma unroll 1
+      for (int e = 0; e < 8; ++e) {
+        const float x = __bfloat162float(w[e]);
+        if (fabsf(x) < __builtin_huge_valf()) continue;
+        note(x != x ? 0 : x > 0.f ? 1 : 2, col + e, r);
+        w[e] = __float2bfloat16(0.f);
+      }
+    }
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
+
+// ---- long sequences ------------------------------------------------------------------------------------------------------
+
+namespace wide {
+
+constexpr int kThreads = 384;
+constexpr int kCopyWarp = 8, kMmaWarp = 9, kGuardWarp = 10;
+constexpr int kKeys = 2;  // blocks of K in shared memory
+template <int D>
+constexpr int kValues = D == 128 ? 3 : 4;  // of V
+template <int D>
+constexpr int kSmem = (2 + kKeys + kValues<D>) * kTileBytes<D> + 1024;  // and what the tiles' alignment costs
+constexpr uint32_t kColumns = 512;  // of TMEM: S of both tiles, then O
+constexpr int kO = 2 * kTile;
+constexpr int kNever = 0x7fffffff;
 
 struct Bars {
-  uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], v_full[2], v_clean[2], full[8], used[kUsed], done;
+  uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], k_full[4], v_full[4], v_used[4], odd_full[2], odd_clean[2], done;
 };
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, 1) packed_attend_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-                                                                    const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args a,
-                                                                    uint32_t* err) {
-  constexpr int SLOTS = Shape<D>::kSlots, BYTES = Shape<D>::kTileBytes;
+__global__ void __launch_bounds__(kThreads, 1)
+    long_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                         const __grid_constant__ Args a, uint32_t* err) {
+  constexpr int KS = kKeys, VS = kValues<D>, BYTES = kTileBytes<D>;
   extern __shared__ unsigned char raw[];
   __shared__ Bars bars;
   __shared__ uint32_t tmem_slot;
-  __shared__ int found;
+  __shared__ int found, any_odd;
   __shared__ int odd_row[3][D];  // first row of a NaN, an infinity, a negative infinity in a column of V, where rows must not see all
-  __shared__ int any_odd;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
-  const uint32_t q_at = base, ring = base + 2 * BYTES;
+  const uint32_t q_at = base, k_at = base + 2 * BYTES, v_at = k_at + KS * BYTES;
+  const auto bar = [](uint64_t& b) { return smem_addr(&b); };
 
-  // the block of rows and the heads; the last blocks, which have the most keys, first
-  const int units = a.q_heads >> a.tiles_apart;
-  const int slot = a.slots - 1 - (int)blockIdx.x / units, unit = blockIdx.x % units;
-  const int span = a.tiles_apart ? kTile : 2 * kTile;
-  if (tid == 0) found = -1, any_odd = 0;
-  __syncthreads();
-  for (int i = tid; i < a.n; i += kThreads)
-    if (a.indptr[i] / span + i <= slot) atomicMax(&found, i);
-  for (int i = tid; i < 3 * D; i += kThreads) (&odd_row[0][0])[i] = kNever;
-  __syncthreads();
-  const int seq = found;
-  if (seq < 0) return;
-  const int first = a.indptr[seq], last = a.indptr[seq + 1];
-  if (first < 0 || last > a.rows || first > last) {
-    if (tid == 0) raise(err, kErrBadIndex);
-    return;
-  }
-  const int len = last - first;
-  if ((int64_t)(slot - (first / span + seq)) * span >= len) return;
-  const int row0 = (slot - (first / span + seq)) * span;
-
-  const int group = a.q_heads / a.kv_heads;
-  int head[2], begin[2], blocks[2];  // of the tiles: head, first row, blocks of keys
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    head[i] = a.tiles_apart ? 2 * unit + i : unit;
-    begin[i] = a.tiles_apart ? row0 : row0 + i * kTile;
-    blocks[i] = begin[i] < len ? begin[i] / kTile + 1 : 0;
-  }
-  const int kv_head = head[0] / group, all = max(blocks[0], blocks[1]);
-  const int seen_by_all = row0 / kTile;  // blocks of keys before this one are; one block or two are not
-
-  if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_addr(&bars.q_full[i]), 1), mbar_init(smem_addr(&bars.s_full[i]), 1);
-      mbar_init(smem_addr(&bars.p_full[i][0]), 4), mbar_init(smem_addr(&bars.p_full[i][1]), 4);
-      mbar_init(smem_addr(&bars.o_full[i]), 1);
-      mbar_init(smem_addr(&bars.v_full[i]), 1), mbar_init(smem_addr(&bars.v_clean[i]), 2);
-    }
-    for (int i = 0; i < SLOTS; ++i) mbar_init(smem_addr(&bars.full[i]), 1);
-    for (int i = 0; i < kUsed; ++i) mbar_init(smem_addr(&bars.used[i]), 1);
-    mbar_init(smem_addr(&bars.done), 1);
-    mbar_init_fence();
+  // on their way while the CTA sets itself up
+  int from = tid < a.n ? a.indptr[tid] : 0, to = tid < a.n ? a.indptr[tid + 1] : 0;
+  if (warp == kMmaWarp) tmem_alloc(smem_addr(&tmem_slot), kColumns);
+  if (tid == kCopyWarp * 32) {
     prefetch_tensormap(&qmap), prefetch_tensormap(&kmap), prefetch_tensormap(&vmap);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(bars.q_full[i]), 1), mbar_init(bar(bars.s_full[i]), 1), mbar_init(bar(bars.o_full[i]), 1);
+      mbar_init(bar(bars.p_full[i][0]), 4), mbar_init(bar(bars.p_full[i][1]), 4);
+      mbar_init(bar(bars.odd_full[i]), 1), mbar_init(bar(bars.odd_clean[i]), 2);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(bar(bars.k_full[i]), 1), mbar_init(bar(bars.v_full[i]), 1), mbar_init(bar(bars.v_used[i]), 1);
+    mbar_init(bar(bars.done), 1);
+    mbar_init_fence();
   }
-  if (warp == kMmaWarp) tmem_alloc(smem_addr(&tmem_slot), 512);
+  // the block of rows and the heads; the last blocks, which have the most keys, first
+  const int units = a.q_heads >> a.apart;
+  const int slot = a.slots - 1 - (int)blockIdx.x / units, unit = blockIdx.x % units;
+  if (tid == 0) found = -1, any_odd = 0;
+  for (int i = tid; i < 3 * D; i += kThreads) (&odd_row[0][0])[i] = kNever;
   tc_fence_before_sync();
+  __syncthreads();
+  // A sequence's blocks are behind those that the ones in front can have at most: from place (rows in front >> shift) + their number on.
+  for (int i = tid; i < a.n; i += kThreads) {
+    if (i != tid) from = a.indptr[i], to = a.indptr[i + 1];
+    const int place = slot - ((from >> a.shift) + i);
+    if (from < 0 || to > a.rows || from > to) {
+      if (unit == 0) raise(err, kErrBadIndex);
+    } else if (place >= 0 && ((int64_t)place << a.shift) < to - from) {
+      atomicMax(&found, i);  // there is one, where all ascend
+    }
+  }
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  const auto bar = [](uint64_t& b) { return smem_addr(&b); };
-  // Item 2 j of the ring is block j of K, item 2 j + 1 of V. Blocks of V that are looked through have barriers of their own, since
-  // the warps that do it do not follow the ring; they are the last of V.
-  const auto guarded = [&](int item) { return (item & 1) && (item >> 1) >= seen_by_all; };
-  const auto filling = [&](int item) { return guarded(item) ? bar(bars.v_full[(item >> 1) - seen_by_all]) : bar(bars.full[item % SLOTS]); };
-  const auto filled = [&](int item) { return mbar_wait(filling(item), guarded(item) ? 0 : (item / SLOTS) & 1, err); };
+  const int seq = found;
+  if (seq < 0) {
+    if (warp == kMmaWarp) tmem_dealloc(tmem, kColumns);
+    return;
+  }
+  const int first = a.indptr[seq], len = a.indptr[seq + 1] - first, row0 = (slot - ((first >> a.shift) + seq)) << a.shift;
 
-  // registers: 2 * 128 * 224 + 128 * 56 = 384 * 168, what the launch has
+  const int group = a.q_heads / a.kv_heads;
+  const int head0 = unit << a.apart, kv_head = head0 / group;
+  // tile i: head, first row, blocks of keys
+  const auto head_of = [&](int i) { return head0 + (a.apart ? i : 0); };
+  const auto begin_of = [&](int i) { return row0 + (a.apart ? 0 : i * kTile); };
+  const auto blocks_of = [&](int i) { return begin_of(i) < len ? begin_of(i) / kTile + 1 : 0; };
+  const int last_tile = blocks_of(1) > 0 ? 1 : 0, all = blocks_of(last_tile);
+  const int seen_by_all = row0 / kTile;  // blocks of keys before this one are; one block or two are not
+
+  // Blocks of V that are looked through have barriers of their own, since the warps that do it do not follow the ring.
+  const auto k_filled = [&](int j) { return mbar_wait(bar(bars.k_full[j % KS]), (j / KS) & 1, err); };
+  const auto v_filled = [&](int j) {
+    return j >= seen_by_all ? mbar_wait(bar(bars.odd_full[j - seen_by_all]), 0, err) : mbar_wait(bar(bars.v_full[j % VS]), (j / VS) & 1, err);
+  };
+  const auto v_clean = [&](int j) { return j >= seen_by_all ? mbar_wait(bar(bars.odd_clean[j - seen_by_all]), 0, err) : v_filled(j); };
+
+  // registers: 256 * 224 + 128 * 56 = 384 * 168, what the launch has
   if (warp < kCopyWarp) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int i = warp >> 2, quarter = warp & 3;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t s_at = lanes + i * kTile, o_at = lanes + 256 + i * kTile;
-    const int begin_i = i ? begin[1] : begin[0], blocks_i = i ? blocks[1] : blocks[0], head_i = i ? head[1] : head[0];
-    const int row = begin_i + quarter * 32 + lane;  // of the sequence
-    float m = kNegInf, l = 0.f;
+    const uint32_t s_at = lanes + i * kTile, o_at = lanes + kO + i * kTile;
+    const int begin = begin_of(i), blocks = blocks_of(i);
+    const int row = begin + quarter * 32 + lane;  // of the sequence
+    Row sums;
     bool ok = true;
-    for (int j = 0; j < blocks_i; ++j) {
-      ok = mbar_wait(bar(bars.s_full[i]), j & 1, err);
+    for (int j = 0; j < blocks; ++j) {
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(bars.s_full[i]), j & 1, err));
       if (!ok) break;
       tc_fence_after_sync();
-      float s[kTile];
-#pragma unroll
-      for (int c = 0; c < kTile; c += 32) tmem_ld32(s_at + c, s + c);
-      tmem_ld_done<kTile>(s);
-      if ((j + 1) * kTile > begin_i) {  // the diagonal
-        const int limit = row - j * kTile;
-#pragma unroll
-        for (int c = 0; c < kTile; ++c) s[c] = c <= limit ? s[c] : kNegInf;
-      }
-      // The weights' first half is made under the reference as it is, with the row's maximum beside it, and once more where that turns
-      // out to be too far off. In front of all a maximum comes first.
-      const auto largest = [&] {
-        float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int c = 4; c + 7 < kTile; c += 8)
-#pragma unroll
-          for (int t = 0; t < 4; ++t) top[t] = max3_nan(top[t], s[c + t], s[c + 4 + t]);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) top[t] = max3_nan(top[t], s[kTile - 4 + t], s[kTile - 4 + t]);
-        return max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3])) * a.scale;
-      };
-      float2 sum[2];
-      uint32_t p[32];
-      const auto weights = [&](int half) {
-        const float2 scale = both(a.scale), minus_ref = both(m == kNegInf ? 0.f : -m);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const int c = half * 64 + 2 * e;
-          const float2 x = fma2(make_float2(s[c], s[c + 1]), scale, minus_ref);
-          const float2 w = kCubic >> (e & 7) & 1 ? exp2_cubic(x) : make_float2(exp2_of(x.x), exp2_of(x.y));
-          sum[e & 1] = add2(sum[e & 1], w);
-          const __nv_bfloat162 h = __floats2bfloat162_rn(w.x, w.y);
-          p[e] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-      };
-      const auto give = [&](int half) {
-        tmem_st32(s_at + half * 32, p);
-        tmem_st_done();
-        tc_fence_before_sync();
-        __syncwarp();
+      make_weights<D>(sums, s_at, o_at, a.scale, j == 0, j == blocks - 1, quarter * 32 + lane, [&](int half) {
         if (lane == 0) mbar_arrive(bar(bars.p_full[i][half]));
-      };
-      if (j == 0) m = largest();
-      sum[0] = sum[1] = both(0.f);
-      weights(0);
-      const float now = largest();
-      if (__any_sync(0xffffffffu, now > m + kLag)) {
-        const float next = now > m + kLag ? now : m;
-        const float f = m == next ? 1.f : m == kNegInf ? 0.f : exp2_of(m - next);
-        m = next, l *= f;
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          float o[32];
-          tmem_ld32(o_at + c, o);
-          tmem_ld_done<32>(o);
-          uint32_t r[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(o[e] * f);
-          tmem_st32(o_at + c, r);
-        }
-        sum[0] = sum[1] = both(0.f);
-        weights(0);
-      }
-      give(0);
-      weights(1);
-      give(1);
-      sum[0] = add2(sum[0], sum[1]);
-      // a score that is no number, or infinite: neither is the sum
-      l += sum[0].x + sum[0].y + (now == kNegInf ? 0.f : now - now);
+      });
     }
-    if (ok && blocks_i) ok = mbar_wait(bar(bars.o_full[i]), 0, err);
-    for (int j = seen_by_all; j < all && ok && blocks_i; ++j) ok = mbar_wait(bar(bars.v_clean[j - seen_by_all]), 0, err);
-    if (ok && blocks_i) {
+    ok = ok && blocks > 0 && mbar_wait(bar(bars.o_full[i]), 0, err);
+    for (int j = seen_by_all; j < all && ok; ++j) ok = v_clean(j);
+    if (__all_sync(0xffffffffu, ok)) {
       tc_fence_after_sync();
-      const float f = 1.f / l;
-      const bool odd = *reinterpret_cast<volatile int*>(&any_odd);
-      bf16* const dst = a.out + (int64_t)(first + row) * a.ldo + (int64_t)head_i * D;
-#pragma unroll
-      for (int c = 0; c < D; c += 32) {
-        float o[32];
-        tmem_ld32(o_at + c, o);
-        tmem_ld_done<32>(o);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] *= f;
-        if (odd) {
-          for (int e = 0; e < 32; ++e) {
-            const bool nan = row >= odd_row[0][c + e], pos = row >= odd_row[1][c + e], neg = row >= odd_row[2][c + e];
-            if (pos) o[e] += __builtin_huge_valf();
-            if (neg) o[e] -= __builtin_huge_valf();
-            if (nan) o[e] = __int_as_float(0x7fffffff);
-          }
-        }
-        if (row < len) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) st8(dst + c + e, o + e);
-        }
-      }
+      const int row_w = begin + quarter * 32;
+      // the tile of Q is free now
+      write_rows<D>(o_at, sums.l, *reinterpret_cast<volatile int*>(&any_odd) != 0, [&](int kind, int c) { return row >= odd_row[kind][c]; },
+                    raw + (q_at - smem_addr(raw)) + i * BYTES + quarter * 2048, a.out + (int64_t)(first + row_w) * a.ldo + (int64_t)head_of(i) * D,
+                    a.ldo, len - row_w, lane);
     }
   } else {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-  if (warp == kCopyWarp) {
-    if (elect_one()) {
-      int issued = 0;
-      bool ok = true;
-      for (int i = 0; i < 2; ++i) {
-        if (!blocks[i]) continue;
-        mbar_expect_tx(bar(bars.q_full[i]), BYTES);
-        tma_load_3d(q_at + i * BYTES, &qmap, bar(bars.q_full[i]), 0, first + begin[i], head[i] * (D / 64), kEvictFirst);
-      }
-      for (int item = 0; item < 2 * all; ++item) {
-        if (item >= SLOTS) {  // what the slot held was used up in this turn
-          const int turn = (item - SLOTS - 1) / 2;
-          ok = mbar_wait(bar(bars.used[turn % kUsed]), (turn / kUsed) & 1, err);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == kCopyWarp) {
+      if (elect_one()) {
+        const auto fetch = [&](const CUtensorMap* map, uint32_t to, uint32_t full, int at_row, int at_head, uint64_t hint) {
+          mbar_expect_tx(full, BYTES);
+          tma_load_3d(to, map, full, 0, first + at_row, at_head * (D / 64), hint);
+        };
+        int k_n = 0, v_n = 0;  // blocks asked for
+        bool ok = true;
+        for (int j = 0; j < all; ++j) {
+          // With tile 0's scores against the block in front there, both tiles are done with the one before that, and a tile alone
+          // with this one, too: K's slot is free. V's is when v_used says so.
+          if (j > 0) ok = mbar_wait(bar(bars.s_full[0]), (j - 1) & 1, err);
           if (!ok) break;
+          if (j == 0) fetch(&qmap, q_at, bar(bars.q_full[0]), begin_of(0), head_of(0), kEvictFirst);
+          fetch(&kmap, k_at + j % KS * BYTES, bar(bars.k_full[j % KS]), j * kTile, kv_head, kEvictLast);
+          ++k_n;
+          if (j == 0 && last_tile == 1) fetch(&qmap, q_at + BYTES, bar(bars.q_full[1]), begin_of(1), head_of(1), kEvictFirst);
+          if (j >= VS) ok = mbar_wait(bar(bars.v_used[(j - VS) % 4]), ((j - VS) / 4) & 1, err);
+          if (!ok) break;
+          fetch(&vmap, v_at + j % VS * BYTES, j >= seen_by_all ? bar(bars.odd_full[j - seen_by_all]) : bar(bars.v_full[j % VS]), j * kTile, kv_head, kEvictLast);
+          ++v_n;
         }
-        const int s = item % SLOTS;
-        const uint32_t full = filling(item);
-        mbar_expect_tx(full, BYTES);
-        tma_load_3d(ring + s * BYTES, item & 1 ? &vmap : &kmap, full, 0, first + (item >> 1) * kTile, kv_head * (D / 64), kEvictLast);
-        ++issued;
-      }
-      if (!ok) {
-        for (int item = max(0, issued - SLOTS); item < issued; ++item) filled(item);
-        for (int i = 0; i < 2; ++i)
-          if (blocks[i]) mbar_wait(bar(bars.q_full[i]), 0, err);
-      }
-    }
-  } else if (warp == kMmaWarp) {
-    // one thread for both tiles, in turns: it keeps them apart, so that one's products run under the other's exponentials
-    if (elect_one()) {
-      constexpr uint32_t kScores = idesc_bf16_f32(kTile, kTile), kSums = idesc_bf16_f32(kTile, D) | kRightTransposed;
-      const auto scores = [&](int i, int j) {  // S of tile i against keys j
-        const uint32_t q = q_at + i * BYTES, k = ring + (2 * j % SLOTS) * BYTES;
-#pragma unroll
-        for (int x = 0; x < D / 16; ++x) {
-          const uint32_t at = (x >> 2) * (kTile * 128) + (x & 3) * 32;
-          mma_bf16(tmem + i * kTile, kmajor_sw128_desc(q + at), kmajor_sw128_desc(k + at), kScores, x > 0);
+        if (!ok) {  // the copies under way land in shared memory
+          for (int j = max(0, k_n - KS); j < k_n; ++j) k_filled(j);
+          for (int j = max(0, v_n - VS); j < v_n; ++j) v_filled(j);
+          for (int i = 0; i <= last_tile; ++i) mbar_wait(bar(bars.q_full[i]), 0, err);
         }
-        mma_commit(bar(bars.s_full[i]));
-      };
-      // Turn j: P V(j) and S(j + 1) of both tiles. What it needs of the ring was waited for in the turn before, between the tiles.
-      const auto ready = [&](int j) {
-        const bool v = j < seen_by_all ? filled(2 * j + 1) : mbar_wait(bar(bars.v_clean[j - seen_by_all]), 0, err);
-        return v && (j + 1 >= all || filled(2 * j + 2));
-      };
-      bool ok = filled(0);
-      for (int i = 0; i < 2 && ok; ++i) {
-        if (!blocks[i]) continue;
-        ok = mbar_wait(bar(bars.q_full[i]), 0, err);
-        if (!ok) break;
-        tc_fence_after_sync();
-        scores(i, 0);
       }
-      ok = ok && ready(0);
-      uint32_t v = ring + BYTES;
-      for (int j = 0; j < all && ok; ++j) {
-        for (int i = 0; i < 2 && ok; ++i) {
-          if (j < blocks[i]) {
-            for (int half = 0; half < 2 && ok; ++half) {  // of the block's keys, whose weights come in turn
-              ok = mbar_wait(bar(bars.p_full[i][half]), j & 1, err);
-              if (!ok) break;
-              tc_fence_after_sync();
-#pragma unroll
-              for (int x = 0; x < kTile / 32; ++x) {
-                const int k = half * (kTile / 32) + x;
-                mma_bf16_ta(tmem + 256 + i * kTile, tmem + i * kTile + k * 8, values_desc(v + k * 2048), kSums, j > 0 || k > 0);
+    } else if (warp == kMmaWarp) {
+      // one thread for all tiles, in turns: it keeps two apart, so that one's products run under the other's exponentials
+      if (elect_one()) {
+        const auto scores = [&](int i, int j) {  // S of tile i against keys j
+          issue_scores<D>(tmem + i * kTile, q_at + i * BYTES, k_at + j % KS * BYTES);
+          mma_commit(bar(bars.s_full[i]));
+        };
+        // Turn j: P V(j) and S(j + 1) of the tiles. V was waited for in the turn before, K is between the weights' halves.
+        bool ok = k_filled(0);
+        for (int i = 0; i <= last_tile && ok; ++i) {
+          ok = mbar_wait(bar(bars.q_full[i]), 0, err);
+          if (!ok) break;
+          tc_fence_after_sync();
+          scores(i, 0);
+        }
+        ok = ok && v_clean(0);
+        for (int j = 0; j < all && ok; ++j) {
+          for (int i = 0; i <= last_tile && ok; ++i) {
+            const int blocks = blocks_of(i);
+            if (j < blocks) {
+              const uint32_t v = v_at + j % VS * BYTES;
+              for (int half = 0; half < 2 && ok; ++half) {  // of the block's keys, whose weights come in turn
+                ok = mbar_wait(bar(bars.p_full[i][half]), j & 1, err);
+                if (!ok) break;
+                tc_fence_after_sync();
+                issue_sums<D>(tmem + kO + i * kTile, tmem + i * kTile, v, half, j == 0);
+                if (half == 0 && i == 0 && j + 1 < all) ok = k_filled(j + 1);
               }
+              if (!ok) break;
+              if (i == last_tile && j + VS < all) mma_commit(bar(bars.v_used[j % 4]));
+              if (j + 1 < blocks) scores(i, j + 1);
+              else mma_commit(bar(bars.o_full[i]));
             }
-            if (!ok) break;
-            if (j + 1 < blocks[i]) scores(i, j + 1);
-            else mma_commit(bar(bars.o_full[i]));
+            if (ok && i == 0 && j + 1 < all) ok = v_clean(j + 1);
           }
-          if (i == 0 && j + 1 < all) ok = ready(j + 1);
         }
-        if (!ok) break;
-        if (2 * j + SLOTS < 2 * all) mma_commit(bar(bars.used[j % kUsed]));  // items wait for it
-        v = v + 2 * BYTES >= ring + SLOTS * BYTES ? v + 2 * BYTES - SLOTS * BYTES : v + 2 * BYTES;
+        if (!ok) {  // what is under way uses shared memory and TMEM
+          mma_commit(bar(bars.done));
+          mbar_wait(bar(bars.done), 0, err);
+        }
       }
-      if (!ok) {  // what is under way uses shared memory and TMEM
-        mma_commit(bar(bars.done));
-        mbar_wait(bar(bars.done), 0, err);
+    } else {
+      const int t = tid - kGuardWarp * 32;
+      for (int j = seen_by_all; j < all; ++j) {
+        if (!v_filled(j)) break;
+        look_through<D>(raw + (v_at - smem_addr(raw)) + j % VS * BYTES, len - j * kTile, t, [&](int kind, int c, int r) {
+          atomicMin(&odd_row[kind][c], j * kTile + r);
+          any_odd = 1;
+        });
+        if (lane == 0) mbar_arrive(bar(bars.odd_clean[j - seen_by_all]));
       }
     }
-  } else {
-    const int t = tid - kGuardWarp * 32;
-    for (int j = seen_by_all; j < all; ++j) {
-      const int item = 2 * j + 1;
-      if (!filled(item)) break;
-      unsigned char* const v = raw + (ring - smem_addr(raw)) + (item % SLOTS) * BYTES;
-      const int keys = len - j * kTile;  // rows of the sequence in the block, or more
-      for (int i = t; i < BYTES / 16; i += 64) {
-        uint4* const at = reinterpret_cast<uint4*>(v) + i;
-        const int row = (i >> 3) & (kTile - 1);
-        if (row >= keys) {
-          *at = make_uint4(0, 0, 0, 0);
-          continue;
-        }
-        const uint4 u = *at;
-        const uint32_t mark = 0x7f807f80u, one = 0x00800080u, top = 0x80008000u;  // an exponent of all ones carries into the top bit
-        if ((((u.x & mark) + one) | ((u.y & mark) + one) | ((u.z & mark) + one) | ((u.w & mark) + one)) & top) {
-          const int col = (i / (kTile * 8)) * 64 + (((i & 7) ^ (row & 7)) << 3);
-          uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t h = (w[e >> 1] >> (16 * (e & 1))) & 0xffffu;
-            if ((h & 0x7f80u) == 0x7f80u) {
-              atomicMin(&odd_row[h & 0x7fu ? 0 : h >> 15 ? 2 : 1][col + e], j * kTile + row);
-              w[e >> 1] &= e & 1 ? 0xffffu : 0xffff0000u;
-              any_odd = 1;
-            }
-          }
-          *at = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(bars.v_clean[j - seen_by_all]));
-    }
-  }
   }
   tc_fence_before_sync();
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, kColumns);
   }
 }
 
+}  // namespace wide
+
+// ---- short sequences -------------------------------------------------------------------------------------------------------
+
+namespace narrow {
+
+constexpr int kThreads = 256, kPerSm = 2;
+constexpr int kItemWarp = 4, kMmaWarp = 5, kGuardWarp = 6;
+constexpr uint32_t kColumns = 256;  // of TMEM: S, then O
 template <int D>
-cudaError_t go(const PackedAttend& p, const CUtensorMap* maps, const Args& a, uint32_t* err, cudaStream_t s) {
-  const cudaError_t e = allow_large<packed_attend_kernel<D>>(Shape<D>::kSmem);
-  if (e != cudaSuccess) return e;
-  const unsigned units = p.q_heads >> a.tiles_apart;
-  packed_attend_kernel<D><<<a.slots * units, kThreads, Shape<D>::kSmem, s>>>(maps[0], maps[1], maps[2], a, err);
-  return cudaGetLastError();
+constexpr int kSmem = 3 * kTileBytes<D> + 1024;  // Q, K and V, and what their alignment costs
+
+struct Item {
+  int first, len;  // of the sequence: first row, rows
+  int row0, head;  // of the item; head < 0: there is none any more
+};
+
+// One of each of what an item or a block needs in turn: a barrier's phase is the item's or the block's number.
+struct Bars {
+  uint64_t item_full[2], item_empty[2];
+  uint64_t q_full, o_full, last_full, last_clean;  // by items; the last block of V has barriers of its own
+  uint64_t k_full, s_full, p_full[2], v_used;      // by blocks
+  uint64_t v_full;                                 // by blocks that are not an item's last
+  uint64_t done;
+};
+
+// The items in their order, for one warp: by blocks of keys, the most first, then by sequence and head.
+struct Order {
+  const Args& a;
+  int lane;
+  int level = -1, at_level = 0;  // blocks of the items that come now but one; sequences that have such items
+  int base = 0;         // items in front of them
+
+  __device__ __forceinline__ int blocks(int i) const {  // of sequence i
+    if (i >= a.n) return 0;
+    const int from = a.indptr[i], to = a.indptr[i + 1];
+    return from < 0 || to > a.rows || from > to ? 0 : (to - from + kTile - 1) / kTile;
+  }
+  __device__ __forceinline__ int count() const {
+    int c = 0;
+    for (int i0 = 0; i0 < a.n; i0 += 32) c += __popc(__ballot_sync(0xffffffffu, blocks(i0 + lane) > level));
+    return c;
+  }
+  __device__ __forceinline__ void begin(uint32_t* err) {
+    int most = 0;
+    for (int i = lane; i < a.n; i += 32) {
+      const int from = a.indptr[i], to = a.indptr[i + 1];
+      if ((from < 0 || to > a.rows || from > to) && blockIdx.x == 0) raise(err, kErrBadIndex);
+      most = max(most, blocks(i));
+    }
+    level = (int)__reduce_max_sync(0xffffffffu, (unsigned)most) - 1;
+    at_level = level >= 0 ? count() : 0;
+  }
+  // Item t, not in front of the one asked for before.
+  __device__ __forceinline__ Item item(int t) {
+    while (level >= 0 && t - base >= at_level * a.q_heads) {
+      base += at_level * a.q_heads;
+      --level;
+      if (level >= 0) at_level = count();
+    }
+    if (level < 0) return Item{0, 0, 0, -1};
+    int k = (t - base) / a.q_heads;
+    const int head = t - base - k * a.q_heads;
+    for (int i0 = 0;; i0 += 32) {  // the k-th sequence that has such an item
+      const uint32_t has = __ballot_sync(0xffffffffu, blocks(i0 + lane) > level);
+      const int c = __popc(has);
+      if (k < c) {
+        const int i = i0 + __fns(has, 0, k + 1), from = a.indptr[i];
+        return Item{from, a.indptr[i + 1] - from, level * kTile, head};
+      }
+      k -= c;
+    }
+  }
+};
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, kPerSm)
+    short_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                         const __grid_constant__ Args a, uint32_t* err) {
+  constexpr int BYTES = kTileBytes<D>;
+  extern __shared__ unsigned char raw[];
+  __shared__ Bars bars;
+  __shared__ Item items[2];
+  __shared__ uint32_t tmem_slot;
+  // what is not finite in the last block of V, by items: the item's number + 1, and for each column the item's number * 256 + 127 - the
+  // first such row of the block, of NaN, infinities and negative infinities
+  __shared__ int any_odd[2], odd_row[2][3][D];
+  __shared__ __align__(16) unsigned char stages[4][32 * 64];  // 32 columns of a warp's rows on their way out
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
+  const uint32_t q_at = base, k_at = base + BYTES, v_at = base + 2 * BYTES;
+  const auto bar = [](uint64_t& b) { return smem_addr(&b); };
+  const auto wait = [&](uint64_t& b, int phase) { return mbar_wait(smem_addr(&b), phase & 1, err); };
+
+  if (warp == kMmaWarp) tmem_alloc(smem_addr(&tmem_slot), kColumns);
+  if (tid == kItemWarp * 32) {
+    prefetch_tensormap(&qmap), prefetch_tensormap(&kmap), prefetch_tensormap(&vmap);
+    for (int i = 0; i < 2; ++i) mbar_init(bar(bars.item_full[i]), 1), mbar_init(bar(bars.item_empty[i]), 7), mbar_init(bar(bars.p_full[i]), 4);
+    mbar_init(bar(bars.q_full), 1), mbar_init(bar(bars.o_full), 1), mbar_init(bar(bars.last_full), 1), mbar_init(bar(bars.last_clean), 2);
+    mbar_init(bar(bars.k_full), 1), mbar_init(bar(bars.s_full), 1), mbar_init(bar(bars.v_used), 1), mbar_init(bar(bars.v_full), 1);
+    mbar_init(bar(bars.done), 1);
+    mbar_init_fence();
+  }
+  Order order{a, lane};
+  if (warp == kItemWarp) order.begin(err);
+  for (int i = tid; i < 2 * 3 * D; i += kThreads) (&odd_row[0][0][0])[i] = -1;
+  if (tid < 2) any_odd[tid] = 0;
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+
+  const auto item_there = [&](int n) { return wait(bars.item_full[n & 1], n >> 1) && items[n & 1].head >= 0; };
+  const auto leave_item = [&](int n) { mbar_arrive(bar(bars.item_empty[n & 1])); };
+
+  // registers: 128 * 184 + 128 * 72 = 256 * 128, what the launch has
+  if (warp < kItemWarp) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16), s_at = lanes, o_at = lanes + kTile;
+    int g = 0;  // blocks so far
+    for (int n = 0;; ++n) {
+      bool ok = __all_sync(0xffffffffu, item_there(n));
+      if (!ok) break;
+      const int blocks = items[n & 1].row0 / kTile + 1;
+      Row sums;
+      for (int j = 0; j < blocks; ++j, ++g) {
+        ok = __all_sync(0xffffffffu, wait(bars.s_full, g));
+        if (!ok) break;
+        tc_fence_after_sync();
+        const bool last = j == blocks - 1;
+        make_weights<D>(sums, s_at, o_at, a.scale, j == 0, last, warp * 32 + lane, [&](int half) {
+          // behind the last block's look-through, which P V waits for as well: write_rows() below reads what it found
+          if (half == 1 && last) ok = __all_sync(0xffffffffu, wait(bars.last_clean, n));
+          if (lane == 0) mbar_arrive(bar(bars.p_full[half]));
+        });
+      }
+      ok = ok && wait(bars.o_full, n);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after_sync();
+      const Item it = items[n & 1];
+      const int row_w = it.row0 + warp * 32;
+      const auto sees = [&](int kind, int c) {
+        const int x = odd_row[n & 1][kind][c];
+        return x >> 8 == n && warp * 32 + lane >= 127 - (x & 255);
+      };
+      write_rows<D>(o_at, sums.l, *reinterpret_cast<volatile int*>(&any_odd[n & 1]) == n + 1, sees, stages[warp],
+                    a.out + (int64_t)(it.first + row_w) * a.ldo + (int64_t)it.head * D, a.ldo, it.len - row_w, lane);
+      if (lane == 0) leave_item(n);
+      tc_fence_before_sync();  // O has been read: in front of the next item's first weights
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == kItemWarp) {
+      const int group = a.q_heads / a.kv_heads;
+      const auto fetch = [&](const CUtensorMap* map, uint32_t to, uint64_t& full, int at_row, int at_head, uint64_t hint) {
+        mbar_expect_tx(bar(full), BYTES);
+        tma_load_3d(to, map, bar(full), 0, at_row, at_head * (D / 64), hint);
+      };
+      int g = 0, gv = 0;
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        const Item it = order.item(n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x));
+        if (lane == 0) {
+          ok = n < 2 || wait(bars.item_empty[n & 1], (n >> 1) - 1);
+          if (ok) items[n & 1] = it, mbar_arrive(bar(bars.item_full[n & 1]));
+          const int blocks = it.head < 0 ? 0 : it.row0 / kTile + 1;
+          for (int j = 0; j < blocks && ok; ++j, ++g) {
+            // the scores against the block in front are there: K's slot is free, and with an item's last ones Q's; V's behind P V
+            if (g > 0) ok = wait(bars.s_full, g - 1);
+            if (!ok) break;
+            if (j == 0) fetch(&qmap, q_at, bars.q_full, it.first + it.row0, it.head, kEvictFirst);
+            fetch(&kmap, k_at, bars.k_full, it.first + j * kTile, it.head / group, kEvictLast);
+            if (g > 0) ok = wait(bars.v_used, g - 1);
+            if (ok) fetch(&vmap, v_at, j + 1 == blocks ? bars.last_full : bars.v_full, it.first + j * kTile, it.head / group, kEvictLast);
+            else wait(bars.k_full, g), j == 0 && wait(bars.q_full, n);  // the copies under way land in shared memory
+            if (ok && j + 1 < blocks) ++gv;
+          }
+          if (!ok && g > 0) {  // so does the last V
+            if (gv > 0) wait(bars.v_full, gv - 1);
+            if (n > 0) wait(bars.last_full, n - 1);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (it.head < 0) break;
+      }
+    } else if (warp == kMmaWarp) {
+      if (elect_one()) {
+        const auto scores = [&] {
+          issue_scores<D>(tmem, q_at, k_at);
+          mma_commit(bar(bars.s_full));
+        };
+        int g = 0, gv = 0;
+        bool ok = true;
+        for (int n = 0; ok; ++n) {
+          if (!item_there(n)) break;
+          const int blocks = items[n & 1].row0 / kTile + 1;
+          leave_item(n);
+          ok = wait(bars.q_full, n) && wait(bars.k_full, g);
+          if (!ok) break;
+          tc_fence_after_sync();
+          scores();
+          for (int j = 0; j < blocks && ok; ++j, ++g) {
+            ok = j + 1 == blocks ? wait(bars.last_clean, n) : wait(bars.v_full, gv++);
+            for (int half = 0; half < 2 && ok; ++half) {  // of the block's keys, whose weights come in turn
+              ok = wait(bars.p_full[half], g);
+              if (!ok) break;
+              tc_fence_after_sync();
+              issue_sums<D>(tmem + kTile, tmem, v_at, half, j == 0);
+              if (half == 0 && j + 1 < blocks) ok = wait(bars.k_full, g + 1);
+            }
+            if (!ok) break;
+            mma_commit(bar(bars.v_used));
+            if (j + 1 < blocks) scores();
+            else mma_commit(bar(bars.o_full));
+          }
+        }
+        // what is under way uses shared memory and TMEM
+        mma_commit(bar(bars.done));
+        wait(bars.done, 0);
+      }
+    } else {
+      const int t = tid - kGuardWarp * 32;
+      for (int n = 0;; ++n) {
+        if (!__all_sync(0xffffffffu, item_there(n))) break;
+        const int keys = items[n & 1].len - items[n & 1].row0;
+        __syncwarp();
+        if (lane == 0) leave_item(n);
+        // Nobody looks at what was found two items ago any more: this item's last V is fetched behind the end of the one before it.
+        if (!__all_sync(0xffffffffu, wait(bars.last_full, n))) break;
+        look_through<D>(raw + (v_at - smem_addr(raw)), keys, t, [&](int kind, int c, int r) {
+          atomicMax(&odd_row[n & 1][kind][c], n * 256 + 127 - r);
+          any_odd[n & 1] = n + 1;
+        });
+        if (lane == 0) mbar_arrive(bar(bars.last_clean));
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, kColumns);
+  }
 }
+
+}  // namespace narrow
 
 }  // namespace
 
-cudaError_t launch_packed_attend(const PackedAttend& p, uint32_t* err, cudaStream_t s) {
-  const int group = p.q_heads / p.kv_heads, D = p.head_dim;
+cudaError_t launch_packed_attend(const PackedAttend& p, int sm_count, uint32_t* err, cudaStream_t s) {
+  const int D = p.head_dim;
+  if (D != 64 && D != 128) return cudaErrorInvalidValue;
   Args a;
   a.indptr = p.indptr, a.n = p.n, a.rows = p.rows, a.q_heads = p.q_heads, a.kv_heads = p.kv_heads;
-  a.tiles_apart = group % 2 == 0;
-  a.slots = p.rows / (a.tiles_apart ? kTile : 2 * kTile) + p.n;
   a.scale = p.scale * 1.44269504088896340736f;
   a.out = p.out, a.ldo = p.ldo;
+  a.apart = p.q_heads / p.kv_heads % 2 == 0;
+  a.shift = a.apart ? 7 : 8;
+  a.slots = (p.rows >> a.shift) + p.n;
   CUtensorMap maps[3];
   const bf16* at[3] = {p.q, p.k, p.v};
   const int64_t ld[3] = {p.ldq, p.ldk, p.ldv};
@@ -464,9 +772,22 @@ cudaError_t launch_packed_attend(const PackedAttend& p, uint32_t* err, cudaStrea
     const uint64_t strides[2] = {(uint64_t)ld[i] * 2, 128};
     if (tc_encode_bf16(&maps[i], at[i], 3, dims, strides, box) != 0) return cudaErrorInvalidValue;
   }
-  if (D == 128) return go<128>(p, maps, a, err, s);
-  if (D == 64) return go<64>(p, maps, a, err, s);
-  return cudaErrorInvalidValue;
+  const auto go = [&](auto d) {
+    constexpr int kD = decltype(d)::value;
+    if (p.rows / p.n >= 2048) {
+      const cudaError_t e = allow_large<wide::long_kernel<kD>>(wide::kSmem<kD>);
+      if (e != cudaSuccess) return e;
+      wide::long_kernel<kD><<<(unsigned)a.slots * (a.q_heads >> a.apart), wide::kThreads, wide::kSmem<kD>, s>>>(maps[0], maps[1], maps[2], a, err);
+    } else {
+      const cudaError_t e = allow_large<narrow::short_kernel<kD>>(narrow::kSmem<kD>);
+      if (e != cudaSuccess) return e;
+      const int64_t items = ((int64_t)p.rows / kTile + p.n) * p.q_heads;  // at most
+      const unsigned ctas = (unsigned)std::min<int64_t>(items, (int64_t)sm_count * narrow::kPerSm);
+      narrow::short_kernel<kD><<<ctas, narrow::kThreads, narrow::kSmem<kD>, s>>>(maps[0], maps[1], maps[2], a, err);
+    }
+    return cudaGetLastError();
+  };
+  return D == 128 ? go(std::integral_constant<int, 128>()) : go(std::integral_constant<int, 64>());
 }
 
 }  // namespace omni

@@ -120,6 +120,14 @@ def test_long_prompts(ops, d, n):
     check(ops, 1, 1, d, [n, 3])
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hk", [(1, 1), (2, 1), (3, 1), (4, 2)])
+@pytest.mark.parametrize("lens,before,behind", [([2048], 0, 0), ([2049], 0, 3), ([2175], 1, 0), ([2177], 0, 0), ([2304], 0, 100), ([2431, 0, 4096], 7, 0), ([4099, 1, 2560], 0, 9)])
+def test_prompts_of_thousands(ops, lens, before, behind, hq, hk, d):
+    """Sequences long enough in the mean for the kernel that shares keys between two tiles of queries."""
+    check(ops, hq, hk, d, lens, seed=len(lens), before=before, behind=behind)
+
+
 @pytest.mark.parametrize("scale", [1e-38, 1e-3, 2.0])  # 0 is refused: a hidden score is -infinity before it is scaled
 @pytest.mark.parametrize("loud", [0.05, 3.0])
 def test_flat_and_peaked(ops, scale, loud):
@@ -132,21 +140,23 @@ def test_flat_and_peaked(ops, scale, loud):
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("hq,hk", [(2, 1), (1, 1)])
-def test_other_rows_do_not_reach_a_row(ops, hq, hk, d):
+@pytest.mark.parametrize("lens", [[300, 90, 200], [2300, 2090, 2200]])
+def test_other_rows_do_not_reach_a_row(ops, lens, hq, hk, d):
     """NaN and infinities in rows of no sequence, in the sequence behind and in later rows of the same sequence."""
-    lens, before, behind = [300, 90, 200], 5, 60
+    before, behind = 5, 60
     nan, inf = float("nan"), float("inf")
     q, k, v, ptr = case(hq, hk, d, lens, seed=3, before=before, behind=behind)
     for x in (q, k, v):
         x[:before], x[int(ptr[-1]):] = nan, inf
     k[int(ptr[1]):int(ptr[2])] = nan          # the whole second sequence
     v[int(ptr[1]):int(ptr[2])] = -inf
-    v[int(ptr[0]) + 290, 7] = nan             # late rows of the first: in its last block,
-    v[int(ptr[0]) + 270, 9] = inf
-    v[int(ptr[0]) + 271, 9] = -inf
-    v[int(ptr[0]) + 299, 11] = -inf
+    late = lens[0] // 128 * 128               # rows of the first: in its last block,
+    v[int(ptr[0]) + late + 34, 7] = nan
+    v[int(ptr[0]) + late + 14, 9] = inf
+    v[int(ptr[0]) + late + 15, 9] = -inf
+    v[int(ptr[1]) - 1, 11] = -inf
     v[int(ptr[2]) + 100, 13] = inf            # and in one that later rows see as a whole
-    v[int(ptr[2]) + 199, 3] = nan
+    v[int(ptr[3]) - 1, 3] = nan
     want, tol = attend_of(q, k, v, ptr, hq, hk, d, 0.1)
     want[int(ptr[1]):int(ptr[2])] = nan
     got = run(ops, q, k, v, ptr, hq, hk, d, 0.1)
@@ -180,8 +190,9 @@ def test_sequences_outside_the_rows_are_reported(ops, ptr):
         ops.sync()
 
 
-def test_the_same_every_time_and_from_a_graph(ops):
-    q, k, v, ptr = case(16, 8, 128, [300, 77, 512], seed=8)
+@pytest.mark.parametrize("lens", [[300, 77, 512], [5000]])
+def test_the_same_every_time_and_from_a_graph(ops, lens):
+    q, k, v, ptr = case(16, 8, 128, lens, seed=8)
     want = run(ops, q, k, v, ptr, 16, 8, 128, 0.1).clone()
     stream, graph, at = torch.cuda.Stream(), torch.cuda.CUDAGraph(), i32(ptr)
     out = torch.zeros_like(want)
