@@ -29,6 +29,7 @@ namespace cg = cooperative_groups;
 
 constexpr float kSlack = 8.f;  // powers of two by which a score may pass its reference before the sums are rescaled
 constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kLowest = -1e30f;  // reference in front of all scores: a number, so that no difference is infinite minus infinite
 constexpr float kNone = __builtin_huge_valf();  // reference of a row that is not attended to
 
 constexpr int kWarps = 4;
@@ -95,10 +96,10 @@ struct Part {  // of a query: reference of the scores, of the weights, sum of 2^
   float r, R, l, unused;
 };
 // Weight of summands under reference x when the largest reference is `top`.
-__device__ __forceinline__ float weight_of(float x, float top) { return x == kNegInf ? 0.f : exp2_of(x - top); }
+__device__ __forceinline__ float weight_of(float x, float top) { return exp2_of(x - top); }
 // The result from sums under their largest references.
 __device__ __forceinline__ uint2 result_of(float4 v, float r_top, float R_top, float l_sum) {
-  const float f = exp2_of((R_top == kNegInf ? 0.f : R_top) - (r_top == kNegInf ? 0.f : r_top)) / l_sum;
+  const float f = exp2_of(R_top - r_top) / l_sum;
   const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x * f, v.y * f), hi = __floats2bfloat162_rn(v.z * f, v.w * f);
   return make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
 }
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
   float r[NT][2], R[NT][2], l[NT][2], o[NT][STEPS][4];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    r[nt][0] = r[nt][1] = R[nt][0] = R[nt][1] = kNegInf, l[nt][0] = l[nt][1] = 0.f;
+    r[nt][0] = r[nt][1] = R[nt][0] = R[nt][1] = kLowest, l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
     for (int j = 0; j < STEPS; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
   }
@@ -297,88 +298,94 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
     const float ks = __shfl_sync(0xffffffffu, sc.x, i & 31), vs = __shfl_sync(0xffffffffu, sc.y, i & 31);
     const int valid = ks < 0.f ? 0 : len - (page0 + me + i * workers) * 16;  // tokens from the page's first on
     if (valid <= 0) continue;
-
-    float s[NT][4];
+    const auto page = [&](auto part) {  // `part`: some of its tokens are none of the row's
+      constexpr bool kPart = decltype(part)::value;
+      float s[NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
-    for (int c = 0; c < CW; ++c) {
-      const uint4 lo = lds16(keys + piece_at<D>(g, t * CW + c)), hi = lds16(keys + piece_at<D>(g + 8, t * CW + c));
-      const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+      for (int c = 0; c < CW; ++c) {
+        const uint4 lo = lds16(keys + piece_at<D>(g, t * CW + c)), hi = lds16(keys + piece_at<D>(g + 8, t * CW + c));
+        const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t a0, a1, a2, a3;
-        widen(wl[w], a0, a2), widen(wh[w], a1, a3);
+        for (int w = 0; w < 4; ++w) {
+          uint32_t a0, a1, a2, a3;
+          widen(wl[w], a0, a2), widen(wh[w], a1, a3);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sm100::mma_16816_f16(s[nt], a0, a1, a2, a3, qf[nt][c * 4 + w][0], qf[nt][c * 4 + w][1]);
-      }
-    }
-    const float lvs = __log2f(vs);
-    bool over = false;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float v = s[nt][e] * (ks * unit_of[nt][e & 1]);
-        s[nt][e] = g + (e & 2) * 4 < valid ? v : kNegInf;
-        over |= s[nt][e] > r[nt][e & 1] + kSlack || s[nt][e] + lvs > R[nt][e & 1] + kSlack;
-      }
-    if (__any_sync(0xffffffffu, over)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float m = fmaxf(s[nt][e], s[nt][e + 2]);
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-          // a reference is a number even where all scores so far are -infinity
-          const float nr = fmaxf(r[nt][e], m), nR = fmaxf(R[nt][e], m + lvs);
-          l[nt][e] *= r[nt][e] == kNegInf ? 0.f : exp2_of(r[nt][e] - nr);
-          const float f = R[nt][e] == kNegInf ? 0.f : exp2_of(R[nt][e] - nR);
-          r[nt][e] = nr, R[nt][e] = nR;
-#pragma unroll
-          for (int j = 0; j < STEPS; ++j) o[nt][j][e] *= f, o[nt][j][e + 2] *= f;
+          for (int nt = 0; nt < NT; ++nt) sm100::mma_16816_f16(s[nt], a0, a1, a2, a3, qf[nt][c * 4 + w][0], qf[nt][c * 4 + w][1]);
         }
-    }
-    uint32_t p[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float rr = r[nt][e & 1] == kNegInf ? 0.f : r[nt][e & 1], RR = R[nt][e & 1] == kNegInf ? 0.f : R[nt][e & 1];
-        l[nt][e & 1] += exp2_of(s[nt][e] - rr);
-        w[e] = exp2_of(s[nt][e] + lvs - RR);
       }
-      p[nt][0] = transpose8(half2_of(w[0], w[1])), p[nt][1] = transpose8(half2_of(w[2], w[3]));
-    }
-    const uint32_t values = keys + 16 * D;
-    constexpr int WORDS = D / 32;  // of a value's row that a lane holds: elements (D / 8) g ..
-    uint32_t u[4][WORDS];
+      float lvs;
+      asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lvs) : "f"(vs));
+      bool over = false;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int tok = 2 * t + (k & 1) + (k >> 1) * 8;
-      if constexpr (D == 128) {
-        const uint4 v = lds16(values + piece_at<D>(tok, g));
-        u[k][0] = v.x, u[k][1] = v.y, u[k][2] = v.z, u[k][3] = v.w;
-      } else {
-        const uint2 v = lds8(values + piece_at<D>(tok, g >> 1) + (g & 1) * 8);
-        u[k][0] = v.x, u[k][1] = v.y;
+      for (int nt = 0; nt < NT; ++nt) {
+        // scores above this pass one of their references by more than kSlack
+        const float most[2] = {fminf(r[nt][0], R[nt][0] - lvs) + kSlack, fminf(r[nt][1], R[nt][1] - lvs) + kSlack};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[nt][e] *= ks * unit_of[nt][e & 1];
+          if (kPart && g + (e & 2) * 4 >= valid) s[nt][e] = kNegInf;
+          over |= s[nt][e] > most[e & 1];
+        }
       }
-      if (tok >= valid) {  // what lies there may be NaN
+      if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-        for (int w = 0; w < WORDS; ++w) u[k][w] = 0;
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float m = fmaxf(s[nt][e], s[nt][e + 2]);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+            const float nr = fmaxf(r[nt][e], m), nR = fmaxf(R[nt][e], m + lvs);
+            l[nt][e] *= exp2_of(r[nt][e] - nr);
+            const float f = exp2_of(R[nt][e] - nR);
+            r[nt][e] = nr, R[nt][e] = nR;
+#pragma unroll
+            for (int j = 0; j < STEPS; ++j) o[nt][j][e] *= f, o[nt][j][e + 2] *= f;
+          }
       }
-    }
+      uint32_t p[NT][2];
 #pragma unroll
-    for (int w = 0; w < WORDS; ++w)
+      for (int nt = 0; nt < NT; ++nt) {
+        float w[4];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t a0, a1, a2, a3;
-        widen(__byte_perm(u[0][w], u[1][w], half ? 0x7362 : 0x5140), a0, a1), widen(__byte_perm(u[2][w], u[3][w], half ? 0x7362 : 0x5140), a2, a3);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sm100::mma_16816_f16(o[nt][w * 2 + half], a0, a1, a2, a3, p[nt][0], p[nt][1]);
+        for (int e = 0; e < 4; ++e) {
+          l[nt][e & 1] += exp2_of(s[nt][e] - r[nt][e & 1]);
+          w[e] = exp2_of(s[nt][e] + (lvs - R[nt][e & 1]));
+        }
+        p[nt][0] = transpose8(half2_of(w[0], w[1])), p[nt][1] = transpose8(half2_of(w[2], w[3]));
       }
+      const uint32_t values = keys + 16 * D;
+      constexpr int WORDS = D / 32;  // of a value's row that a lane holds: elements (D / 8) g ..
+      uint32_t u[4][WORDS];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int tok = 2 * t + (k & 1) + (k >> 1) * 8;
+        if constexpr (D == 128) {
+          const uint4 v = lds16(values + piece_at<D>(tok, g));
+          u[k][0] = v.x, u[k][1] = v.y, u[k][2] = v.z, u[k][3] = v.w;
+        } else {
+          const uint2 v = lds8(values + piece_at<D>(tok, g >> 1) + (g & 1) * 8);
+          u[k][0] = v.x, u[k][1] = v.y;
+        }
+        if (kPart && tok >= valid) {  // what lies there may be NaN
+#pragma unroll
+          for (int w = 0; w < WORDS; ++w) u[k][w] = 0;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t a0, a1, a2, a3;
+          widen(__byte_perm(u[0][w], u[1][w], half ? 0x7362 : 0x5140), a0, a1), widen(__byte_perm(u[2][w], u[3][w], half ? 0x7362 : 0x5140), a2, a3);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) sm100::mma_16816_f16(o[nt][w * 2 + half], a0, a1, a2, a3, p[nt][0], p[nt][1]);
+        }
+    };
+    if (valid >= 16) page(std::false_type());
+    else page(std::true_type());
   }
 
   // the warps' sums: o is [D / 8 bytes of lane g][column], a matrix instruction two neighbouring elements
@@ -404,7 +411,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
   __syncthreads();
   for (int i = tid; i < nq * (D / 4); i += kWarps * 32) {
     const int n = i / (D / 4), d = i % (D / 4) * 4;
-    float r_top = kNegInf, R_top = kNegInf, l_sum = 0.f;
+    float r_top = kLowest, R_top = kLowest, l_sum = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) r_top = fmaxf(r_top, parts[w][n].r), R_top = fmaxf(R_top, parts[w][n].R);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -431,7 +438,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
   cluster.sync();
   for (int i = rank * (kWarps * 32) + tid; i < nq * (D / 4); i += ctas * (kWarps * 32)) {
     const int n = i / (D / 4), d = i % (D / 4) * 4;
-    float r_top = kNegInf, R_top = kNegInf, l_sum = 0.f;
+    float r_top = kLowest, R_top = kLowest, l_sum = 0.f;
     for (int c = 0; c < ctas; ++c) {
       const Part p = *cluster.map_shared_rank(&joined[n], c);
       r_top = fmaxf(r_top, p.r), R_top = fmaxf(R_top, p.R);
@@ -465,7 +472,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_join_kernel(const __grid_cons
   grid_wait();
   const int64_t step = (int64_t)groups * cut.per, at = (piece.before * (int64_t)groups + part) * cut.per + n;
   const float4* const parts = reinterpret_cast<const float4*>(cut.parts) + at;
-  float r_top = kNegInf, R_top = kNegInf;
+  float r_top = kLowest, R_top = kLowest;
   for (int c = tid; c < piece.count; c += kWarps * 32) {
     const float4 p = __ldcg(parts + c * step);
     r_top = fmaxf(r_top, p.x), R_top = fmaxf(R_top, p.y);
