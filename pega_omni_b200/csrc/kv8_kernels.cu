@@ -15,9 +15,9 @@ namespace cg = cooperative_groups;
 
 // ---- page tables ------------------------------------------------------------------------------------------------------
 // Four prefix sums over the sequences (pages, rows, pages wanted, pages given back), then every page, row and free entry finds
-// its sequence in them by bisection: nothing depends on the order in which anything runs. A cluster of CTAs, each of which makes
-// the sums for itself (they are a few KB): one launch, no workspace, and the cluster's barrier stands between the last read of
-// the lengths and their overwriting, so a captured step can keep its lengths in place.
+// its sequence in them: nothing depends on the order in which anything runs. Every CTA makes the sums for itself (they are a few
+// KB): one launch, no workspace. Where lengths or height are kept in place, as a captured step does, the CTAs are one cluster, whose
+// barrier stands between the last read of them and their overwriting.
 
 constexpr int kTablesThreads = 1024;  // at most
 constexpr int kChunk = 256;            // pages
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kTablesThreads) kv_tables_kernel(const TablesC
   if (rows_n > c.row_cap) status |= kTablesRows;
   if (pages_n > c.page_cap) status |= kTablesPages;
   const bool ok = status == 0;
-  const int first = cluster.block_rank() * block + tid, threads = cluster.num_blocks() * block;
+  const int first = blockIdx.x * block + tid, threads = gridDim.x * block;
 
   const auto returned = [&](int k) {  // the k-th page given back
     const int s = owner_of(back, n, k);
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kTablesThreads) kv_tables_kernel(const TablesC
   };
   // a warp takes kChunk pages and rows of a sequence at a time, so a long one among many is shared
   const int chunks = ok ? (c.width + kChunk - 1) / kChunk : 0;
-  for (int task = cluster.block_rank() * warps + warp; task < n * chunks; task += cluster.num_blocks() * warps) {
+  for (int task = blockIdx.x * warps + warp; task < n * chunks; task += gridDim.x * warps) {
     const int chunk = task / n, s = task - chunk * n, len = held[s], had = pages_of(len), total = want[s + 1] - want[s];
     const int32_t* const mine = c.table + (int64_t)s * c.width;
     const int p0 = chunk * kChunk, p1 = min(total, p0 + kChunk), own = min(had, p1);
@@ -294,10 +294,10 @@ __device__ __forceinline__ __nv_bfloat162 abs_max(const uint4& u) {
   return __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u.w)));
 }
 
-constexpr int kAppendWarps = 4;
+constexpr int kAppendWarps = 2;
 
 template <int D>
-__global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(const bf16* __restrict__ k, int64_t ldk, const bf16* __restrict__ v,
+__global__ void __launch_bounds__(kAppendWarps * 32, 12) kv8_append_kernel(const bf16* __restrict__ k, int64_t ldk, const bf16* __restrict__ v,
                                                                        int64_t ldv, const int32_t* __restrict__ slot, int rows, uint8_t* kv,
                                                                        float* scales, int kv_pages, int hk, int head_blocks, uint32_t* err) {
   constexpr int LANES = D / 8, TOGETHER = 32 / LANES, STEPS = 16 / TOGETHER;  // lanes of a row, rows of an access, accesses of 16 rows
@@ -431,16 +431,19 @@ cudaError_t launch_kv_tables(const TablesCall& c, cudaStream_t s) {
   const size_t smem = (size_t)(5 * c.n + 4) * sizeof(int);
   const cudaError_t e = allow_large<kv_tables_kernel>((5 * kTablesMaxSeqs + 4) * 4);
   if (e != cudaSuccess) return e;
-  // a warp for every sequence and for every 128 pages and rows that there may be: sixteen CTAs at most (the largest cluster)
+  // a warp for every sequence and for every 128 pages and rows that there may be; in one cluster (of sixteen CTAs at most) where
+  // lengths or height are kept in place, otherwise without one
+  const bool in_place = c.lens == c.lens_out || c.free_count == c.free_count_out;
   const int64_t warps = std::max<int64_t>(c.n, ((int64_t)c.page_cap + c.row_cap) / 128);
+  const unsigned most = in_place ? 16 : 128;
   unsigned ctas = 1;
-  while (ctas < 16 && warps > (int64_t)ctas * 16) ctas *= 2;
-  const unsigned block = warps > 16 * 16 ? kTablesThreads : kTablesThreads / 2;
+  while (ctas < most && warps > (int64_t)ctas * 16) ctas *= 2;
+  const unsigned block = in_place && warps > 16 * 16 ? kTablesThreads : kTablesThreads / 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(block), cfg.dynamicSmemBytes = smem, cfg.stream = s;
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = ctas, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  attr.val.clusterDim.x = in_place ? ctas : 1, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
   cfg.attrs = &attr, cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kv_tables_kernel, c);
 }
