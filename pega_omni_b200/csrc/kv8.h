@@ -41,6 +41,7 @@ enum TablesStatus : int32_t {
   kTablesFree = 16,
 };
 constexpr int kTablesMaxSeqs = 4096;             // five words a sequence in shared memory
+constexpr int kPackedMaxSeqs = 16384;            // a block looks through all of them before its first waits run out
 constexpr int64_t kTablesMaxEntries = 1ll << 26;  // tokens of so many pages still add up within 31 bits
 
 struct TablesCall {

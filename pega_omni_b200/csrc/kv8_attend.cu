@@ -468,8 +468,8 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_join_kernel(const __grid_cons
   const int row = blockIdx.x / a.q_heads, head = blockIdx.x % a.q_heads, kh = head / group, n = head % group % cut.per;
   const int groups = a.kv_heads * cut.subgroups, part = kh * cut.subgroups + head % group / cut.per;
   const Piece piece = find_piece(a, cut, row, true);
+  grid_wait();  // on every path: with this kernel the one in front has ended
   if (piece.count < 2) return;
-  grid_wait();
   const int64_t step = (int64_t)groups * cut.per, at = (piece.before * (int64_t)groups + part) * cut.per + n;
   const float4* const parts = reinterpret_cast<const float4*>(cut.parts) + at;
   float r_top = kLowest, R_top = kLowest;

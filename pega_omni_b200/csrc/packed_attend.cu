@@ -535,47 +535,57 @@ struct Order {
   const Args& a;
   int lane;
   int level = -1, at_level = 0;  // blocks of the items that come now but one; sequences that have such items
-  int base = 0;         // items in front of them
+  int until = 0;                 // as many have items of this level and of those between
+  int base = 0;                  // items in front of them
+  int from_i = 0, from_k = 0;    // sequences that need not be looked at again, and how many of them have such items
 
   __device__ __forceinline__ int blocks(int i) const {  // of sequence i
     if (i >= a.n) return 0;
     const int from = a.indptr[i], to = a.indptr[i + 1];
     return from < 0 || to > a.rows || from > to ? 0 : (to - from + kTile - 1) / kTile;
   }
-  __device__ __forceinline__ int count() const {
-    int c = 0;
-    for (int i0 = 0; i0 < a.n; i0 += 32) c += __popc(__ballot_sync(0xffffffffu, blocks(i0 + lane) > level));
-    return c;
+  __device__ __forceinline__ void count() {
+    at_level = 0;
+    int next = 0;  // blocks of the longest sequence that has no such item
+    for (int i0 = 0; i0 < a.n; i0 += 32) {
+      const int its = blocks(i0 + lane);
+      at_level += __popc(__ballot_sync(0xffffffffu, its > level));
+      if (its <= level) next = max(next, its);
+    }
+    until = (int)__reduce_max_sync(0xffffffffu, (unsigned)next);
   }
   __device__ __forceinline__ void begin(uint32_t* err) {
-    int most = 0;
+    constexpr int kMany = 1 << 25;  // more than there can be
+    int most = 0, sum = 0;
     for (int i = lane; i < a.n; i += 32) {
-      const int from = a.indptr[i], to = a.indptr[i + 1];
+      const int from = a.indptr[i], to = a.indptr[i + 1], its = blocks(i);
       if ((from < 0 || to > a.rows || from > to) && blockIdx.x == 0) raise(err, kErrBadIndex);
-      most = max(most, blocks(i));
+      most = max(most, its), sum = min(sum + its, kMany);
     }
     level = (int)__reduce_max_sync(0xffffffffu, (unsigned)most) - 1;
-    at_level = level >= 0 ? count() : 0;
+    // sequences that overlap, between which an end lies in front of a beginning: an error by now, and no end of work
+    if ((int)__reduce_add_sync(0xffffffffu, (unsigned)sum) > a.rows / kTile + a.n) level = -1;
+    if (level >= 0) count();
   }
   // Item t, not in front of the one asked for before.
   __device__ __forceinline__ Item item(int t) {
     while (level >= 0 && t - base >= at_level * a.q_heads) {
       base += at_level * a.q_heads;
       --level;
-      if (level >= 0) at_level = count();
+      from_i = from_k = 0;
+      if (level < until && level >= 0) count();
     }
-    if (level < 0) return Item{0, 0, 0, -1};
-    int k = (t - base) / a.q_heads;
-    const int head = t - base - k * a.q_heads;
-    for (int i0 = 0;; i0 += 32) {  // the k-th sequence that has such an item
-      const uint32_t has = __ballot_sync(0xffffffffu, blocks(i0 + lane) > level);
+    const int k = (t - base) / a.q_heads, head = t - base - k * a.q_heads;
+    for (; level >= 0 && from_i < a.n; from_i += 32) {  // the k-th sequence that has such an item
+      const uint32_t has = __ballot_sync(0xffffffffu, blocks(from_i + lane) > level);
       const int c = __popc(has);
-      if (k < c) {
-        const int i = i0 + __fns(has, 0, k + 1), from = a.indptr[i];
+      if (k < from_k + c) {
+        const int i = from_i + (int)__fns(has, 0, k - from_k + 1), from = a.indptr[i];
         return Item{from, a.indptr[i + 1] - from, level * kTile, head};
       }
-      k -= c;
+      from_k += c;
     }
+    return Item{0, 0, 0, -1};
   }
 };
 
@@ -607,8 +617,28 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
     mbar_init(bar(bars.done), 1);
     mbar_init_fence();
   }
+  const auto fetch = [&](const CUtensorMap* map, uint32_t to, uint64_t& full, int at_row, int at_head, uint64_t hint) {
+    mbar_expect_tx(bar(full), BYTES);
+    tma_load_3d(to, map, bar(full), 0, at_row, at_head * (D / 64), hint);
+  };
+  const int group = a.q_heads / a.kv_heads;
+  // the first item, and the first of its copies, while the CTA sets itself up
   Order order{a, lane};
-  if (warp == kItemWarp) order.begin(err);
+  Item it{0, 0, 0, -1};  // of the item warp
+  if (warp == kItemWarp) {
+    order.begin(err);
+    it = order.item(blockIdx.x);
+    if (lane == 0) {
+      items[0] = it;
+      mbar_arrive(bar(bars.item_full[0]));
+      if (it.head >= 0) {
+        fetch(&qmap, q_at, bars.q_full, it.first + it.row0, it.head, kEvictFirst);
+        fetch(&kmap, k_at, bars.k_full, it.first, it.head / group, kEvictLast);
+        fetch(&vmap, v_at, it.row0 == 0 ? bars.last_full : bars.v_full, it.first, it.head / group, kEvictLast);
+      }
+    }
+    __syncwarp();
+  }
   for (int i = tid; i < 2 * 3 * D; i += kThreads) (&odd_row[0][0][0])[i] = -1;
   if (tid < 2) any_odd[tid] = 0;
   tc_fence_before_sync();
@@ -657,28 +687,27 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == kItemWarp) {
-      const int group = a.q_heads / a.kv_heads;
-      const auto fetch = [&](const CUtensorMap* map, uint32_t to, uint64_t& full, int at_row, int at_head, uint64_t hint) {
-        mbar_expect_tx(bar(full), BYTES);
-        tma_load_3d(to, map, bar(full), 0, at_row, at_head * (D / 64), hint);
-      };
       int g = 0, gv = 0;
       bool ok = true;
       for (int n = 0; ok; ++n) {
-        const Item it = order.item(n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x));
+        if (n > 0) it = order.item(n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x));
         if (lane == 0) {
-          ok = n < 2 || wait(bars.item_empty[n & 1], (n >> 1) - 1);
-          if (ok) items[n & 1] = it, mbar_arrive(bar(bars.item_full[n & 1]));
+          if (n > 0) {
+            ok = n < 2 || wait(bars.item_empty[n & 1], (n >> 1) - 1);
+            if (ok) items[n & 1] = it, mbar_arrive(bar(bars.item_full[n & 1]));
+          }
           const int blocks = it.head < 0 ? 0 : it.row0 / kTile + 1;
           for (int j = 0; j < blocks && ok; ++j, ++g) {
-            // the scores against the block in front are there: K's slot is free, and with an item's last ones Q's; V's behind P V
-            if (g > 0) ok = wait(bars.s_full, g - 1);
-            if (!ok) break;
-            if (j == 0) fetch(&qmap, q_at, bars.q_full, it.first + it.row0, it.head, kEvictFirst);
-            fetch(&kmap, k_at, bars.k_full, it.first + j * kTile, it.head / group, kEvictLast);
-            if (g > 0) ok = wait(bars.v_used, g - 1);
-            if (ok) fetch(&vmap, v_at, j + 1 == blocks ? bars.last_full : bars.v_full, it.first + j * kTile, it.head / group, kEvictLast);
-            else wait(bars.k_full, g), j == 0 && wait(bars.q_full, n);  // the copies under way land in shared memory
+            if (g > 0) {
+              // the scores against the block in front are there: K's slot is free, and with an item's last ones Q's; V's behind P V
+              ok = wait(bars.s_full, g - 1);
+              if (!ok) break;
+              if (j == 0) fetch(&qmap, q_at, bars.q_full, it.first + it.row0, it.head, kEvictFirst);
+              fetch(&kmap, k_at, bars.k_full, it.first + j * kTile, it.head / group, kEvictLast);
+              ok = wait(bars.v_used, g - 1);
+              if (ok) fetch(&vmap, v_at, j + 1 == blocks ? bars.last_full : bars.v_full, it.first + j * kTile, it.head / group, kEvictLast);
+              else wait(bars.k_full, g), j == 0 && wait(bars.q_full, n);  // the copies under way land in shared memory
+            }
             if (ok && j + 1 < blocks) ++gv;
           }
           if (!ok && g > 0) {  // so does the last V

@@ -190,6 +190,24 @@ def test_sequences_outside_the_rows_are_reported(ops, ptr):
         ops.sync()
 
 
+def test_sequences_over_one_another_end(ops):
+    """Many sequences of all the rows: more work than rows and sequences can make is not begun."""
+    from pega_omni_b200.ops import OpsError
+    q, k, v, _ = case(2, 1, 64, [1000])
+    out = torch.full((1000, 128), 3.0, dtype=torch.bfloat16, device="cuda")
+    ops.packed_attend(q, k, v, i32([0, 1000] * 20), 2, 1, 64, 0.1, out)
+    with pytest.raises(OpsError, match="0x2"):
+        ops.sync()
+    assert (out == 3).all()
+
+
+@pytest.mark.parametrize("hq,hk", [(1, 1), (6, 2)])
+@pytest.mark.parametrize("lens", [[1900, 3, 700, 3, 130, 0, 1400], [3] * 70 + [4000] + [129] * 3, [128] * 300, [4000] + [0] * 40 + [2600]])
+def test_prompts_of_all_lengths(ops, hq, hk, lens):
+    """One long sequence among many short ones, lengths that many have, empty ones between."""
+    check(ops, hq, hk, 64, lens, seed=len(lens))
+
+
 @pytest.mark.parametrize("lens", [[300, 77, 512], [5000]])
 def test_the_same_every_time_and_from_a_graph(ops, lens):
     q, k, v, ptr = case(16, 8, 128, lens, seed=8)
