@@ -264,7 +264,7 @@ int32_t omni_op_qk_norm_rope(omni_ops* ctx, const void* x, int64_t ldx, const vo
                              const int32_t* pos, int32_t rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                              float eps, float theta, void* out, int64_t ldo);
 
-/* Causal attention within each of n packed sequences: rows indptr[i] .. indptr[i + 1] of q, k and v, of which row r sees the
+/* Causal attention within each of n packed sequences (16,384 at most): rows indptr[i] .. indptr[i + 1] of q, k and v, of which row r sees the
  * sequence's rows up to itself: out[r][h] = softmax(scale * q[r][h] . K) V, h over q_heads and K, V those of kv head
  * h / (q_heads / kv_heads). scale > 0. indptr ascends from any row on; sequences may be empty. Rows outside of the sequences stay
  * as they are in out, and nothing of them, of other sequences or of later rows reaches a row, not even as a NaN. out must not
@@ -277,7 +277,8 @@ int32_t omni_op_packed_attend(omni_ops* ctx, const void* q, int64_t ldq, const v
  * e >= -100 and |x| <= 448 * 2^e for every finite x put into it. A row at a page's first token starts the page anew; rows further in
  * come behind tokens that the page holds, whose scale then only grows, and whose codes are rounded again when it does. Codes
  * are the nearest, ties to even; infinities become +-448 * 2^e, a NaN stays one. Rows of one page are neighbours in the call, in
- * ascending slots without a gap, as omni_op_kv_tables lays them: a page that occurs in two places of a call is written in an
+ * ascending slots without a gap, as omni_op_kv_tables lays them: a row that is on the page of the row in front of it but not its
+ * next token is left out and raises the device error word, and a page that occurs in two places further apart is written in an
  * undefined order. */
 int32_t omni_op_kv8_append(omni_ops* ctx, const void* k, int64_t ldk, const void* v, int64_t ldv, const int32_t* slot,
                            int32_t rows, void* kv, float* scales, int32_t kv_pages, int32_t kv_heads, int32_t head_dim);

@@ -324,9 +324,14 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 12) kv8_append_kernel(const
     if (s >= limit) raise(err, kErrBadIndex);
     return s < 0 || s >= limit ? -2 : s;
   };
-  const int s = slot_of(base + lane), edge = lane == 0 ? slot_of(base - 1) : -2;
+  int s = slot_of(base + lane);
+  const int edge = lane == 0 ? slot_of(base - 1) : -2;
   int before = __shfl_up_sync(0xffffffffu, s, 1);
   if (lane == 0) before = edge;
+  if (s >= 0 && before >= 0 && s >> 4 == before >> 4 && s != before + 1) {  // not its page's next token: two runs would write the page
+    raise(err, kErrBadIndex);
+    s = -2;
+  }
   const uint32_t leaders = __ballot_sync(0xffffffffu, s >= 0 && ((s & 15) == 0 || before + 1 != s));
   const int l = 31 - __clz(leaders & (2u << lane) - 1u);  // that begins no later; -1 where the run begins in front of the window
   const int run = s >= 0 && lane < 31 && l < 16 ? l : -1;

@@ -498,6 +498,7 @@ struct OnDevice {
 static bool at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // Rows of `width` elements at 16-byte addresses, `ld` elements apart.
 static bool rows_at16(const void* p, int64_t ld, int64_t width) { return at16(p) && ld >= width && ld % 8 == 0; }
+constexpr int32_t kMostRows = 1 << 30;
 static bool heads_fit(int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
   return q_heads >= 1 && kv_heads >= 1 && q_heads <= 65535 && q_heads % kv_heads == 0 && (head_dim == 64 || head_dim == 128);
 }
@@ -524,6 +525,8 @@ int32_t omni_op_kv_tables(omni_ops* c, const int32_t* lens, const int32_t* add, 
 int32_t omni_op_qk_norm_rope(omni_ops* c, const void* x, int64_t ldx, const void* q_norm, const void* k_norm,
                              const int32_t* pos, int32_t rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                              float eps, float theta, void* out, int64_t ldo) {
+  if (c && (rows > kMostRows || ((int64_t)rows / 4 + 1) * (((int64_t)q_heads + kv_heads) / 8 + 2) > kMostRows))
+    return c->fail(OMNI_ERR_UNSUPPORTED, "%d rows of %d + %d heads: too many", rows, q_heads, kv_heads);
   if (!c || rows < 0 || !(theta > 0.f)) return c ? c->fail(OMNI_ERR_INVALID, "rows < 0 or theta <= 0") : OMNI_ERR_INVALID;
   if (q_heads < 0 || kv_heads < 0 || q_heads + (int64_t)kv_heads < 1 || q_heads + (int64_t)kv_heads > 65535 || (head_dim != 64 && head_dim != 128))
     return c->fail(OMNI_ERR_UNSUPPORTED, "%d + %d heads of %d: heads of 64 or 128", q_heads, kv_heads, head_dim);
@@ -544,7 +547,8 @@ int32_t omni_op_packed_attend(omni_ops* c, const void* q, int64_t ldq, const voi
   if (!heads_fit(q_heads, kv_heads, head_dim))
     return c->fail(OMNI_ERR_UNSUPPORTED, "%d query heads over %d of %d: whole groups, heads of 64 or 128", q_heads, kv_heads, head_dim);
   if (!(scale > 0.f && scale <= 1e38f)) return c->fail(OMNI_ERR_INVALID, "a scale that is not above 0, or not finite");
-  if (((int64_t)rows / 128 + n) * q_heads > (1 << 30)) return c->fail(OMNI_ERR_UNSUPPORTED, "%d rows of %d heads in %d sequences: too many", rows, q_heads, n);
+  if (n > kPackedMaxSeqs || rows > kMostRows || ((int64_t)rows / 128 + n) * q_heads > kMostRows)
+    return c->fail(OMNI_ERR_UNSUPPORTED, "%d rows of %d heads in %d sequences: too many (sequences: at most %d)", rows, q_heads, n, kPackedMaxSeqs);
   if (rows == 0 || n == 0) return OMNI_OK;
   const int64_t width = (int64_t)q_heads * head_dim, kv_width = (int64_t)kv_heads * head_dim;
   if (!q || !k || !v || !indptr || !out || !rows_at16(q, ldq, width) || !rows_at16(k, ldk, kv_width) || !rows_at16(v, ldv, kv_width) ||
@@ -561,6 +565,8 @@ int32_t omni_op_kv8_append(omni_ops* c, const void* k, int64_t ldk, const void* 
                            int32_t rows, void* kv, float* scales, int32_t kv_pages, int32_t kv_heads, int32_t head_dim) {
   if (!c || rows < 0 || kv_pages < 1) return c ? c->fail(OMNI_ERR_INVALID, "rows < 0 or no pages") : OMNI_ERR_INVALID;
   if (!heads_fit(kv_heads, kv_heads, head_dim)) return c->fail(OMNI_ERR_UNSUPPORTED, "%d heads of %d: heads of 64 or 128", kv_heads, head_dim);
+  if (rows > kMostRows || ((int64_t)rows / 16 + 1) * (kv_heads + 1) > kMostRows)
+    return c->fail(OMNI_ERR_UNSUPPORTED, "%d rows of %d heads: too many", rows, kv_heads);
   if (rows == 0) return OMNI_OK;
   const int64_t width = (int64_t)kv_heads * head_dim;
   if (!k || !v || !slot || !kv || !scales || !rows_at16(k, ldk, width) || !rows_at16(v, ldv, width) || !at16(kv) ||

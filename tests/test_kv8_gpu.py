@@ -383,6 +383,24 @@ def test_append_outside_the_cache_is_reported(ops, bad):
     assert torch.equal(kv, before) and torch.equal(scales, scales_before)
 
 
+@pytest.mark.parametrize("front", [0, 13, 15, 31])
+def test_append_leaves_out_rows_that_are_not_their_pages_next(ops, front):
+    """The same slot twice, slots that descend or skip one, behind one another and where the kernel changes warps."""
+    from pega_omni_b200.ops import OpsError
+    given = [16 * (i + 6) for i in range(front)] + [0, 0, 1, 2, 20, 20, 20, 37, 36, 50, 53, 64, 65, 64]
+    out = {front + i for i in (1, 5, 6, 8, 10, 13)}
+    kept = [i for i in range(len(given)) if i not in out]
+    rng = np.random.default_rng(front)
+    kv, scales = cache(40, 2, 64, 2)
+    k, v = bf16(rng.standard_normal((len(given), 128))), bf16(rng.standard_normal((len(given), 128)))
+    want, want_scales = values(kv), f64(scales)
+    append_of(want, want_scales, f64(k)[kept], f64(v)[kept], [given[i] for i in kept])
+    ops.kv8_append(k, v, i32(given), kv, scales)
+    with pytest.raises(OpsError, match="0x2"):
+        ops.sync()
+    assert np.array_equal(f64(scales), want_scales) and np.array_equal(values(kv), want, equal_nan=True)
+
+
 # ---- attention over the pages ---------------------------------------------------------------------------------------------
 
 def attend_case(hq, hk, d, lens, seed, spread=2, extra=3, loud=1.0):

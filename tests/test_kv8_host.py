@@ -51,7 +51,8 @@ def test_kv_tables_refuses(call, change, status):
     ({"rows": -1}, INVALID), ({"theta": 0.0}, INVALID), ({"theta": float("nan")}, INVALID), ({"ldx": 24 * 128 - 8}, INVALID),
     ({"ldx": 4100}, INVALID), ({"ldo": 4092}, INVALID), ({"ldo": 8192}, INVALID),  # in place with another stride
     ({"head_dim": 96}, UNSUPPORTED), ({"q_heads": 0, "kv_heads": 0}, UNSUPPORTED), ({"q_heads": -1}, UNSUPPORTED),
-    ({"q_heads": 65535, "kv_heads": 1}, UNSUPPORTED),
+    ({"q_heads": 65535, "kv_heads": 1}, UNSUPPORTED), ({"rows": 2**31 - 1}, UNSUPPORTED), ({"rows": 2**31 - 1, "q_heads": 1, "kv_heads": 0}, UNSUPPORTED),
+    ({"rows": 1 << 22, "q_heads": 60000}, UNSUPPORTED),
 ])
 def test_qk_norm_rope_refuses(call, change, status):
     rc, why = call("omni_op_qk_norm_rope", ROPE, **change)
@@ -62,6 +63,7 @@ def test_qk_norm_rope_refuses(call, change, status):
     *[({k: None}, INVALID) for k in ("k", "v", "slot", "kv", "scales")], *[({k: ODD}, INVALID) for k in ("k", "v", "kv", "scales")],
     ({"k": OFF8}, INVALID), ({"kv": OFF8}, INVALID), ({"rows": -1}, INVALID), ({"kv_pages": 0}, INVALID), ({"ldk": 1016}, INVALID),
     ({"ldv": 1028}, INVALID), ({"head_dim": 80}, UNSUPPORTED), ({"kv_heads": 0}, UNSUPPORTED), ({"kv_heads": 65536}, UNSUPPORTED),
+    ({"rows": 2**31 - 1}, UNSUPPORTED), ({"rows": 1 << 20, "kv_heads": 60000, "ldk": 60000 * 128, "ldv": 60000 * 128}, UNSUPPORTED),
 ])
 def test_kv8_append_refuses(call, change, status):
     rc, why = call("omni_op_kv8_append", APPEND, **change)
@@ -84,7 +86,7 @@ def test_kv8_attend_refuses(call, change, status):
     ({"rows": -1}, INVALID), ({"n": -1}, INVALID), ({"ldq": 2040}, INVALID), ({"ldk": 1016}, INVALID), ({"ldv": 1028}, INVALID),
     ({"ldo": 2044}, INVALID), ({"ldq": 1 << 40}, INVALID), ({"q_heads": 9}, UNSUPPORTED), ({"kv_heads": 0}, UNSUPPORTED), ({"head_dim": 96}, UNSUPPORTED),
     ({"scale": -0.1}, INVALID), ({"scale": 0.0}, INVALID), ({"scale": float("nan")}, INVALID), ({"scale": float("inf")}, INVALID), ({"rows": 2**31 - 1, "q_heads": 128}, UNSUPPORTED),
-    ({"n": 2**31 - 1}, UNSUPPORTED),
+    ({"n": 2**31 - 1}, UNSUPPORTED), ({"n": 16385}, UNSUPPORTED), ({"rows": 2**31 - 1, "q_heads": 1, "kv_heads": 1}, UNSUPPORTED),
 ])
 def test_packed_attend_refuses(call, change, status):
     rc, why = call("omni_op_packed_attend", PACKED, **change)
