@@ -92,14 +92,14 @@ __device__ __forceinline__ uint32_t piece_at(int row, int col) {
   return (uint32_t)(row * D + ((D == 128 ? col ^ (row & 7) : col ^ ((row >> 1) & 3)) << 4));
 }
 
-struct Part {  // of a query: reference of the scores, of the weights, sum of 2^(s - r)
-  float r, R, l, unused;
+struct Part {  // of a query: reference of the scores, of the weights, sum of 2^(s - r), and what the weights' sums are to be multiplied by
+  float r, R, l, f;
 };
 // Weight of summands under reference x when the largest reference is `top`.
 __device__ __forceinline__ float weight_of(float x, float top) { return exp2_of(x - top); }
-// The result from sums under their largest references.
-__device__ __forceinline__ uint2 result_of(float4 v, float r_top, float R_top, float l_sum) {
-  const float f = exp2_of(R_top - r_top) / l_sum;
+// 0 where nothing was attended to: all of the row's pages lie outside the cache.
+__device__ __forceinline__ Part part_of(float r, float R, float l) { return Part{r, R, l, l == 0.f ? 0.f : exp2_of(R - r) / l}; }
+__device__ __forceinline__ uint2 result_of(float4 v, float f) {
   const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x * f, v.y * f), hi = __floats2bfloat162_rn(v.z * f, v.w * f);
   return make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
 }
@@ -177,6 +177,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
   constexpr int STEPS = D / 16;               // matrix instructions of K Q^T; as many of V^T P^T
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Part parts[kWarps][NT * 8], joined[NT * 8];
+  __shared__ float factor[8][NT * 8];  // of the sums of warps, then of CTAs
   grid_trigger();  // of the second kernel, if there is one
   const cg::cluster_group cluster = cg::this_cluster();
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
@@ -192,6 +193,14 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
   const int group = a.q_heads / a.kv_heads, q0 = sub * cut.per, nq = min(cut.per, group - q0);
   const int head0 = kh * group + q0;
   bf16* const out = a.out + row * a.ldo + (int64_t)head0 * D;
+
+  // queries: column n of a tile is query head head0 + n, lane t holds elements (D / 4) t .. of it; on their way before anything is known
+  uint4 raw[NT][D / 32];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+      raw[nt][j] = __ldg(reinterpret_cast<const uint4*>(a.q + row * a.ldq + (int64_t)(head0 + min(nt * 8 + g, nq - 1)) * D + t * (D / 4)) + j);
 
   // the row's tokens and pages
   const int s_of = a.seq ? a.seq[row] : row, pos = a.pos[row];
@@ -251,21 +260,13 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
 #pragma unroll
   for (int i = 0; i < S - 1; ++i) issue(i, i);
 
-  // queries: column n of a tile is query head head0 + n, lane t holds elements (D / 4) t .. of it
   uint32_t qf[NT][STEPS][2];
   float unit_of[NT][2];  // scores of columns 2 t, 2 t + 1 in powers of two
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int n = nt * 8 + g;
     float x[STEPS * 4];
-    if (n < nq) {
-      const bf16* const src = a.q + row * a.ldq + (int64_t)(head0 + n) * D + t * (D / 4);
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) ld8(src + 8 * j, x + 8 * j);
-    } else {
-#pragma unroll
-      for (int j = 0; j < STEPS * 4; ++j) x[j] = 0.f;
-    }
+    for (int j = 0; j < D / 32; ++j) unpack8v(nt * 8 + g < nq ? raw[nt][j] : make_uint4(0, 0, 0, 0), x + 8 * j);
     float top = 0.f;
 #pragma unroll
     for (int j = 0; j < STEPS * 4; ++j) top = fmaxf(top, fabsf(x[j]) < __builtin_huge_valf() ? fabsf(x[j]) : 0.f);
@@ -401,7 +402,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
       if (n < nq) {
-        if (g == 0) parts[warp][n] = Part{r[nt][e], R[nt][e], l[nt][e]};
+        if (g == 0) parts[warp][n] = Part{r[nt][e], R[nt][e], l[nt][e], 0.f};
         float* const dst = sums + (warp * NT * 8 + n) * D + g * (D / 8);
 #pragma unroll
         for (int j = 0; j < STEPS; j += 2)
@@ -409,49 +410,65 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
       }
     }
   __syncthreads();
-  for (int i = tid; i < nq * (D / 4); i += kWarps * 32) {
-    const int n = i / (D / 4), d = i % (D / 4) * 4;
+  if (tid < nq) {
     float r_top = kLowest, R_top = kLowest, l_sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) r_top = fmaxf(r_top, parts[w][n].r), R_top = fmaxf(R_top, parts[w][n].R);
+    for (int w = 0; w < kWarps; ++w) r_top = fmaxf(r_top, parts[w][tid].r), R_top = fmaxf(R_top, parts[w][tid].R);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) l_sum += parts[w][tid].l * weight_of(parts[w][tid].r, r_top), factor[w][tid] = weight_of(parts[w][tid].R, R_top);
+    joined[tid] = part_of(r_top, R_top, l_sum);
+  }
+  __syncthreads();
+  const int64_t at = ((int64_t)(piece.before + piece.index) * groups + part) * cut.per;
+  if (piece.count > 1 && tid < nq) cut.parts[at + tid] = joined[tid];
+#pragma unroll
+  for (int k = 0; k < NT * 8 * (D / 4) / (kWarps * 32); ++k) {
+    const int i = k * (kWarps * 32) + tid, n = i / (D / 4), d = i % (D / 4) * 4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const Part p = parts[w][n];
-      l_sum += p.l * weight_of(p.r, r_top);
-      const float f = weight_of(p.R, R_top);
+      const float f = factor[w][n];
       const float4 x = *reinterpret_cast<const float4*>(sums + (w * NT * 8 + n) * D + d);
       v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
     }
-    if (piece.count > 1) {
-      const int64_t at = ((int64_t)(piece.before + piece.index) * groups + part) * cut.per + n;
-      *reinterpret_cast<float4*>(cut.sums + at * D + d) = v;
-      if (d == 0) cut.parts[at] = Part{r_top, R_top, l_sum, 0.f};
-    } else if (ctas == 1) {
-      *reinterpret_cast<uint2*>(out + n * D + d) = result_of(v, r_top, R_top, l_sum);
-    } else {
-      *reinterpret_cast<float4*>(total + n * D + d) = v;
-      if (d == 0) joined[n] = Part{r_top, R_top, l_sum, 0.f};
-    }
+    if (n >= nq) continue;
+    if (piece.count > 1) *reinterpret_cast<float4*>(cut.sums + (at + n) * D + d) = v;
+    else if (ctas == 1) *reinterpret_cast<uint2*>(out + n * D + d) = result_of(v, joined[n].f);
+    else *reinterpret_cast<float4*>(total + n * D + d) = v;
   }
   if (ctas == 1) return;
   cluster.sync();
-  for (int i = rank * (kWarps * 32) + tid; i < nq * (D / 4); i += ctas * (kWarps * 32)) {
-    const int n = i / (D / 4), d = i % (D / 4) * 4;
-    float r_top = kLowest, R_top = kLowest, l_sum = 0.f;
-    for (int c = 0; c < ctas; ++c) {
-      const Part p = *cluster.map_shared_rank(&joined[n], c);
-      r_top = fmaxf(r_top, p.r), R_top = fmaxf(R_top, p.R);
-    }
+  const int begin = rank * (kWarps * 32) + tid, end = nq * (D / 4), step = ctas * (kWarps * 32);
+  float4 x[8];
+  const auto fetch = [&](int i) {  // the CTAs' sums, all under way before the first is used
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < ctas && i < end) x[c] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(total, c) + i * 4);
+  };
+  fetch(begin);
+  {
+    const int n = tid >> 3, c = tid & 7;
+    Part p = {kLowest, kLowest, 0.f, 0.f};
+    if (n < nq && c < ctas) p = *cluster.map_shared_rank(&joined[n], c);
+    float r_top = p.r, R_top = p.R;
+#pragma unroll
+    for (int x = 1; x < 8; x <<= 1) r_top = fmaxf(r_top, __shfl_xor_sync(0xffffffffu, r_top, x)), R_top = fmaxf(R_top, __shfl_xor_sync(0xffffffffu, R_top, x));
+    float l_sum = p.l * weight_of(p.r, r_top);
+#pragma unroll
+    for (int x = 1; x < 8; x <<= 1) l_sum += __shfl_xor_sync(0xffffffffu, l_sum, x);
+    if (n < nq) factor[c][n] = part_of(r_top, R_top, l_sum).f * weight_of(p.R, R_top);
+  }
+  __syncthreads();
+  for (int i = begin; i < end; i += step) {
+    if (i != begin) fetch(i);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = 0; c < ctas; ++c) {
-      const Part p = *cluster.map_shared_rank(&joined[n], c);
-      l_sum += p.l * weight_of(p.r, r_top);
-      const float f = weight_of(p.R, R_top);
-      const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(total, c) + n * D + d);
-      v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      if (c >= ctas) break;
+      const float f = factor[c][i / (D / 4)];
+      v.x += x[c].x * f, v.y += x[c].y * f, v.z += x[c].z * f, v.w += x[c].w * f;
     }
-    *reinterpret_cast<uint2*>(out + n * D + d) = result_of(v, r_top, R_top, l_sum);
+    *reinterpret_cast<uint2*>(out + i * 4) = result_of(v, 1.f);
   }
   cluster.sync();  // no CTA leaves while another reads its sums
 }
@@ -502,7 +519,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_join_kernel(const __grid_cons
     const float4 x = v_of[i][d];
     v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w, l += l_of[i];
   }
-  *reinterpret_cast<uint2*>(a.out + row * a.ldo + (int64_t)head * D + d * 4) = result_of(v, r_top, R_top, l);
+  *reinterpret_cast<uint2*>(a.out + row * a.ldo + (int64_t)head * D + d * 4) = result_of(v, part_of(r_top, R_top, l).f);
 }
 
 template <int D, int NT>
@@ -555,7 +572,7 @@ cudaError_t launch_kv8_attend(const Kv8Attend& a, int sm_count, cudaMemPool_t po
   //   128 x 8, 500 - 8,000    200 /  181 /  176 /  206 | 179
   //   256 x 8, 100 - 2,000    101 /  104 /  137 /  213 | 105
   int ctas = 1;
-  if (a.rows <= kCutRows && units * 8 <= at_once && held >= 256) {
+  if (a.rows <= kCutRows && units * 6 <= at_once && held >= 256) {
     cut.room = (int)(at_once - units), cut.least = 32;
   } else {
     while (ctas < 8 && ((units * 2 * ctas <= at_once && held >= 16 && held >= 8 * ctas) || held * a.head_dim >= 80 * 128 * ctas)) ctas *= 2;

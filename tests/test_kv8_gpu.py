@@ -593,6 +593,22 @@ def test_attend_outside_its_tables_is_reported(ops, what):
     assert np.isfinite(got[0]).all() and (what.endswith("page") or (got[0] == 0).all())
 
 
+@pytest.mark.parametrize("hq,hk,d,length", [(4, 2, 64, 9), (16, 1, 128, 700), (4, 2, 128, 9000)])
+def test_attend_without_any_page_is_zero(ops, hq, hk, d, length):
+    """All of a row's pages outside the cache: nothing is left to attend to; the other row does not notice."""
+    from pega_omni_b200.ops import OpsError
+    lens = [length, length]
+    kv, scales, pages, indptr, q = attend_case(hq, hk, d, lens, 77)
+    want = run_attend(ops, q, kv, scales, pages, indptr, lens, hq, hk, d, 0.1)
+    pages = pages.copy()
+    pages[:indptr[1]] = -3
+    out = torch.full((2, hq * d), 7.0, dtype=torch.bfloat16, device="cuda")
+    ops.kv8_attend(q, kv, scales, i32([t - 1 for t in lens]), i32(indptr), i32(pages), hq, 0.1, out)
+    with pytest.raises(OpsError, match="0x2"):
+        ops.sync()
+    assert (out[0] == 0).all() and np.array_equal(f64(out)[1], want[1])
+
+
 def test_attend_and_append_far_into_a_large_cache(ops):
     """Pages whose byte offsets pass 32 bits."""
     hq, hk, d = 4, 2, 128
