@@ -33,7 +33,7 @@ namespace cg = cooperative_groups;
 constexpr float kSlack = 8.f;  // powers of two by which a score may pass its reference before the sums are rescaled
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kLowest = -1e30f;  // reference in front of all scores: a number, so that no difference is infinite minus infinite
-constexpr float kNone = __builtin_huge_valf();  // reference of a row that is not attended to
+constexpr float kNone = -1.f;  // what the sums of a row that is not attended to are to be multiplied by, in the first of its pieces' parts
 
 constexpr int kWarps = 4;
 
@@ -129,13 +129,14 @@ struct Piece {
   int row, index, count, pages;  // of the row's pieces, pages of each
   int before;                    // pieces of the rows in front
 };
-// The piece with this number, or (by_row) the first of this row; row = -1: there is none. Whole block, kWarps warps.
+// The piece with this number, or (by_row) the first of this row; row = -1: there is none. Whole block, W warps.
+template <int W>
 __device__ __forceinline__ Piece find_piece(const Kv8Attend& a, const Cut& cut, int number, bool by_row) {
-  __shared__ float sh_pages[kWarps];
-  __shared__ int sh_pieces[kWarps];
+  __shared__ float sh_pages[W];
+  __shared__ int sh_pieces[W];
   __shared__ Piece found;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (a.rows + kWarps * 32 - 1) / (kWarps * 32), begin = min(a.rows, tid * per), end = min(a.rows, begin + per);
+  const int per = (a.rows + W * 32 - 1) / (W * 32), begin = min(a.rows, tid * per), end = min(a.rows, begin + per);
   float sum = 0.f;
   for (int r = begin; r < end; ++r) sum += (float)pages_of_row(a, r);
   sum = warp_add(sum);
@@ -144,7 +145,7 @@ __device__ __forceinline__ Piece find_piece(const Kv8Attend& a, const Cut& cut, 
   __syncthreads();
   sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) sum += sh_pages[w];
+  for (int w = 0; w < W; ++w) sum += sh_pages[w];
   // the rounding of the sum is far below the hundredth
   const unsigned size = max((unsigned)cut.least, (unsigned)(sum * (float)(a.kv_heads * cut.subgroups) * (1.01f / (float)cut.room)) + 1u);
   const auto pieces_of = [&](int pages) { return pages <= (int)size ? 1 : (int)(((unsigned)pages + size - 1u) / size); };
@@ -160,7 +161,7 @@ __device__ __forceinline__ Piece find_piece(const Kv8Attend& a, const Cut& cut, 
   __syncthreads();
   int before = incl - mine;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) before += w < warp ? sh_pieces[w] : 0;
+  for (int w = 0; w < W; ++w) before += w < warp ? sh_pieces[w] : 0;
   if (by_row ? number >= begin && number < end : number >= before && number < before + mine)
     for (int r = begin; r < end; ++r) {
       const int pages = pages_of_row(a, r), n = pieces_of(pages);
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
   const int unit = blockIdx.x / ctas, part = unit % groups, kh = part / subgroups, sub = part % subgroups;
   Piece piece{unit / groups, 0, 1, 0, 0};
   if (cut.room) {
-    piece = find_piece(a, cut, unit / groups, false);
+    piece = find_piece<kWarps>(a, cut, unit / groups, false);
     if (piece.row < 0) return;
   }
   const int row = piece.row;
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
   if (len == 0) {  // the same for every CTA of the cluster and every piece of the row
     if (rank == 0 && piece.index == 0)
       for (int i = tid; i < nq * (D / 8); i += kWarps * 32) *reinterpret_cast<uint4*>(out + i * 8) = make_uint4(0, 0, 0, 0);
-    if (piece.count > 1 && tid < cut.per) cut.parts[(int64_t)(piece.before + piece.index) * groups * cut.per + part * cut.per + tid] = Part{kNone, 0.f, 0.f, 0.f};
+    if (piece.count > 1 && tid < cut.per) cut.parts[(int64_t)(piece.before + piece.index) * groups * cut.per + part * cut.per + tid] = Part{0.f, 0.f, 0.f, kNone};
     return;
   }
   const int all = (len >> 4) + ((len & 15) != 0);
@@ -476,53 +477,68 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
   cluster.sync();  // no CTA leaves while another reads its sums
 }
 
-// The sums of a row's pieces, in an order of their own. A CTA a row and query head; D / 4 lanes a piece, as many pieces at a time
-// as there are such groups of lanes.
+// The sums of a row's pieces, in an order of their own. A CTA a row and query head; D / 4 lanes a piece, as many pieces at a time as
+// there are such groups of lanes, each with two under way and references of its own. It stands behind the last CTAs of the kernel in
+// front, so it has to be small as well as short. One row of 60,000 tokens, 8 kv heads (74 pieces a row and head), both kernels: 28.2
+// us; with four warps 29.7, with sixteen and four pieces under way 28.8, with which 24 rows in pieces of 2 heads of 64 take 30 us
+// instead of 23.7.
+constexpr int kJoinWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(kWarps * 32) kv8_join_kernel(const __grid_constant__ Kv8Attend a, const __grid_constant__ Cut cut) {
-  constexpr int LANES = D / 4, GROUPS = kWarps * 32 / LANES;
-  __shared__ float top[2][kWarps];
+__global__ void __launch_bounds__(kJoinWarps * 32, 4) kv8_join_kernel(const __grid_constant__ Kv8Attend a, const __grid_constant__ Cut cut) {
+  constexpr int LANES = D / 4, GROUPS = kJoinWarps * 32 / LANES, AHEAD = 2;
   __shared__ float4 v_of[GROUPS][LANES];
-  __shared__ float l_of[GROUPS];
+  __shared__ Part part_of_group[GROUPS];
   const int tid = threadIdx.x, group = a.q_heads / a.kv_heads;
   const int row = blockIdx.x / a.q_heads, head = blockIdx.x % a.q_heads, kh = head / group, n = head % group % cut.per;
   const int groups = a.kv_heads * cut.subgroups, part = kh * cut.subgroups + head % group / cut.per;
-  const Piece piece = find_piece(a, cut, row, true);
+  const Piece piece = find_piece<kJoinWarps>(a, cut, row, true);
   grid_wait();  // on every path: with this kernel the one in front has ended
   if (piece.count < 2) return;
   const int64_t step = (int64_t)groups * cut.per, at = (piece.before * (int64_t)groups + part) * cut.per + n;
   const float4* const parts = reinterpret_cast<const float4*>(cut.parts) + at;
-  float r_top = kLowest, R_top = kLowest;
-  for (int c = tid; c < piece.count; c += kWarps * 32) {
-    const float4 p = __ldcg(parts + c * step);
-    r_top = fmaxf(r_top, p.x), R_top = fmaxf(R_top, p.y);
-  }
-  r_top = warp_fmax(r_top), R_top = warp_fmax(R_top);
-  if ((tid & 31) == 0) top[0][tid >> 5] = r_top, top[1][tid >> 5] = R_top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) r_top = fmaxf(r_top, top[0][w]), R_top = fmaxf(R_top, top[1][w]);
-  if (r_top == kNone) return;  // a row that is not attended to: its zeros are there
   const int g = tid / LANES, d = tid % LANES;
+  Part mine = {kLowest, kLowest, 0.f, 0.f};
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-#pragma unroll 4
-  for (int c = g; c < piece.count; c += GROUPS) {
-    const float4 p = __ldcg(parts + c * step), x = __ldcg(reinterpret_cast<const float4*>(cut.sums + (at + c * step) * D) + d);
-    l += p.z * weight_of(p.x, r_top);
-    const float f = weight_of(p.y, R_top);
-    v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+  const float first = __ldcg(parts).w;
+  for (int c = g; c < piece.count; c += AHEAD * GROUPS) {
+    float4 p[AHEAD], x[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int at_piece = c + k * GROUPS;
+      p[k] = make_float4(kLowest, kLowest, 0.f, 0.f), x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (at_piece < piece.count) p[k] = __ldcg(parts + at_piece * step), x[k] = __ldcg(reinterpret_cast<const float4*>(cut.sums + (at + at_piece * step) * D) + d);
+    }
+    float r = mine.r, R = mine.R;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) r = fmaxf(r, p[k].x), R = fmaxf(R, p[k].y);
+    const float old = weight_of(mine.R, R);
+    mine.l *= weight_of(mine.r, r), mine.r = r, mine.R = R;
+    v.x *= old, v.y *= old, v.z *= old, v.w *= old;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      mine.l += p[k].z * weight_of(p[k].x, r);
+      const float f = weight_of(p[k].y, R);
+      v.x += x[k].x * f, v.y += x[k].y * f, v.z += x[k].z * f, v.w += x[k].w * f;
+    }
   }
+  if (first == kNone) return;  // its zeros are there
   v_of[g][d] = v;
-  if (d == 0) l_of[g] = l;
+  if (d == 0) part_of_group[g] = mine;
   __syncthreads();
   if (g > 0) return;
+  Part all = {kLowest, kLowest, 0.f, 0.f};
 #pragma unroll
-  for (int i = 1; i < GROUPS; ++i) {
+  for (int i = 0; i < GROUPS; ++i) all.r = fmaxf(all.r, part_of_group[i].r), all.R = fmaxf(all.R, part_of_group[i].R);
+  v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    const Part p = part_of_group[i];
     const float4 x = v_of[i][d];
-    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w, l += l_of[i];
+    const float f = weight_of(p.R, all.R);
+    all.l += p.l * weight_of(p.r, all.r);
+    v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
   }
-  *reinterpret_cast<uint2*>(a.out + row * a.ldo + (int64_t)head * D + d * 4) = result_of(v, part_of(r_top, R_top, l).f);
+  *reinterpret_cast<uint2*>(a.out + row * a.ldo + (int64_t)head * D + d * 4) = result_of(v, part_of(all.r, all.R, all.l).f);
 }
 
 template <int D, int NT>
@@ -549,7 +565,7 @@ cudaError_t go(const Kv8Attend& a, Cut cut, int ctas, int sm_count, cudaMemPool_
   cfg.attrs = &attr, cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, kv8_attend_kernel<D, NT>, a, cut, err);
   if (cut.room) {
-    if (e == cudaSuccess) e = launch_pdl(kv8_join_kernel<D>, dim3((unsigned)a.rows * a.q_heads), dim3(kWarps * 32), 0, s, a, cut);
+    if (e == cudaSuccess) e = launch_pdl(kv8_join_kernel<D>, dim3((unsigned)a.rows * a.q_heads), dim3(kJoinWarps * 32), 0, s, a, cut);
     const cudaError_t done = cudaFreeAsync(scratch, s);
     if (e == cudaSuccess) e = done;
   }
@@ -570,7 +586,7 @@ cudaError_t launch_kv8_attend(const Kv8Attend& a, int sm_count, cudaMemPool_t po
   // the CTAs that every row has. Measured, us, cluster of 1 / 2 / 4 / 8 | pieces (heads of 128, groups of 2, the third: of 4):
   //   rows x kv heads, tokens
   //   1 x 8,   777              9.0 /  7.7 /  6.3 /  5.5 | 9.7
-  //   1 x 8,   60,000           451 /  228 /  117 /   61 | 32
+  //   1 x 8,   60,000           451 /  228 /  117 /   61 | 28
   //   12 x 8,  28,000 - 34,000  258 /  164 /  133 /  157 | 130 - 139
   //   20 x 8,  500 - 5,000       44 /   30 /   29 /   31 | 27
   //   64 x 8,  2,000 - 8,000    128 /  123 /  116 /  120 |

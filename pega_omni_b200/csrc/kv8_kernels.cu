@@ -164,14 +164,14 @@ __global__ void __launch_bounds__(kTablesThreads) kv_tables_kernel(const TablesC
 // head, D / 16 neighbouring lanes a head, and a warp takes up to kRopeBatch such loads of one row at a time, all under way before
 // the first is used. The angle of a pair is the same for all heads of a row, so a warp makes each once, under its loads, and a
 // lane keeps its eight: in turns and in f64, since f32 would be off by 2^-24 of a far position's whole angle, and only what is left
-// of a turn goes to f32 and sincospi. All else is f32 with one rounding. 8,192 rows of 40 heads of 128: 33.7 us, 4.98 TB/s, where a
-// plain copy of them takes 27.6 us; angles and norms are 40 % of what the SMs can issue meanwhile. 64 rows of 24 heads: 2.5 us.
+// of a turn goes to f32 and sincospi. All else is f32 with one rounding. 8,192 rows of 40 heads of 128: 32.1 us, 5.2 TB/s, where a
+// plain copy of them takes 27.6 us; angles and norms are 40 % of what the SMs can issue meanwhile. 64 rows of 24 heads: 2.3 us.
 
 struct Turns {
   double per_pos[64];
 };
 
-constexpr int kRopeWarps = 4, kRopeBatch = 2;
+constexpr int kRopeWarps = 2, kRopeBatch = 2;
 
 __device__ __forceinline__ void pairs_of(const uint4& u, float2 (&v)[4]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -191,12 +191,12 @@ __device__ __forceinline__ uint4 packed_of(const float2 (&v)[4]) {
 
 // Block y of a row's y_blocks: heads of q where y < q_blocks, otherwise of k.
 template <int D>
-__global__ void __launch_bounds__(kRopeWarps * 32, 7) qk_norm_rope_kernel(const bf16* x, int64_t ldx, const bf16* __restrict__ q_norm,
+__global__ void __launch_bounds__(kRopeWarps * 32, 14) qk_norm_rope_kernel(const bf16* x, int64_t ldx, const bf16* __restrict__ q_norm,
                                                                        const bf16* __restrict__ k_norm, const int32_t* __restrict__ pos,
                                                                        int rows, int hq, int heads, int q_blocks, int y_blocks, float eps,
                                                                        const __grid_constant__ Turns turns, bf16* out, int64_t ldo) {
   constexpr int LANES = D / 16, HEADS = 32 / LANES;  // lanes of a head, heads of a warp's access
-  __shared__ float2 rot[kRopeWarps][D / 2];
+  __shared__ __align__(16) float2 rot[kRopeWarps][D / 2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = (int64_t)(blockIdx.x / y_blocks) * kRopeWarps + warp;
   const int y = blockIdx.x % y_blocks;
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 7) qk_norm_rope_kernel(const 
     const double t = (double)my_pos * turns.per_pos[p];
     float2 f;
     sincospif(2.f * (float)(t - rint(t)), &f.y, &f.x);
-    rot[warp][p] = f;
+    rot[warp][(((p >> 1) & 3) * LANES + (p >> 3)) * 2 + (p & 1)] = f;  // the lanes' pairs side by side, so that no banks collide
   }
   __syncwarp();
   // (lo, hi) -> (lo * lc - hi * hs, hi * hc + lo * ls), the gains in the angles
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 7) qk_norm_rope_kernel(const 
   pairs_of(lo_gain, lc), pairs_of(hi_gain, hc);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float4 f = *reinterpret_cast<const float4*>(&rot[warp][at + 2 * e]);
+    const float4 f = *reinterpret_cast<const float4*>(&rot[warp][(e * LANES + lane % LANES) * 2]);
     const float2 cs = make_float2(f.x, f.z), sn = make_float2(f.y, f.w), minus = make_float2(-f.y, -f.w);
     if (gain) ls[e] = mul2(lc[e], sn), hs[e] = mul2(hc[e], minus), lc[e] = mul2(lc[e], cs), hc[e] = mul2(hc[e], cs);
     else ls[e] = sn, hs[e] = minus, lc[e] = cs, hc[e] = cs;
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 7) qk_norm_rope_kernel(const 
 // registers: rows of a prompt make one run of them, those of a decode step sixteen of one row, and no warp waits for another. Lane r
 // keeps what there is to know of row r: its slot, the row that begins its run, that run's largest magnitude and scale.
 // Bound by HBM where there are many rows (2 bytes in, 1 out an element), but a warp's page is a chain of load, maximum and store, and
-// registers hold two waves of them: 7,600 rows of 8 heads of 128 take 14.8 us, 3.2 TB/s. 61 rows of as many sequences: 4.9 us.
+// registers hold two waves of them: 7,600 rows of 8 heads of 128 take 14.5 us, 3.2 TB/s. 61 rows of as many sequences: 4.2 us.
 
 // The smallest 2^e >= 2^-100 with amax <= 448 * 2^e; amax finite, not negative. 448 = 1.75 * 2^8.
 __device__ __forceinline__ float page_scale(float amax) {
@@ -288,6 +288,13 @@ __device__ __forceinline__ uint32_t e4m3_of4(float a, float b, float c, float d)
 
 __device__ __forceinline__ uint2 e4m3_of8(const float* v, float mul) {
   return make_uint2(e4m3_of4(v[0] * mul, v[1] * mul, v[2] * mul, v[3] * mul), e4m3_of4(v[4] * mul, v[5] * mul, v[6] * mul, v[7] * mul));
+}
+__device__ __forceinline__ uint2 e4m3_of8(const uint4& u, float mul) {
+  float2 v[4];
+  pairs_of(u, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], make_float2(mul, mul));
+  return make_uint2(e4m3_of4(v[0].x, v[0].y, v[1].x, v[1].y), e4m3_of4(v[2].x, v[2].y, v[3].x, v[3].y));
 }
 
 // The largest magnitude of eight bf16 in each half, infinities and (unless there is nothing else) no NaN among them.
@@ -344,29 +351,35 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 12) kv8_append_kernel(const
   const bool held = mine && (s & 15);  // the page holds tokens of this sequence
   const float old = held ? *at_scale : 0.f;
   const uint32_t ours = __ballot_sync(0xffffffffu, run >= 0);
-  const auto skipped = [&](int pass, int i) { return (ours >> (16 * pass + i * TOGETHER) & ((1u << TOGETHER) - 1)) == 0; };  // rows of nobody or of another warp
+  const uint32_t its_ours = ours >> sub;  // bit 16 pass + i * TOGETHER: the row of x[pass][i] is this warp's
+  const int passes = ours >> 16 ? 2 : 1;
+  const auto is_ours = [&](int pass, int i) { return (its_ours >> (16 * pass + i * TOGETHER) & 1) != 0; };
+  if (passes == 2) {
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i)
-    if (!skipped(1, i)) load(1, i);
+    for (int i = 0; i < STEPS; ++i) {
+      x[1][i] = make_uint4(0, 0, 0, 0);
+      if (is_ours(1, i)) load(1, i);
+    }
+  }
   // the largest magnitudes: of the warp's one run as a prompt gives it, otherwise row by row and run by run
   const uint32_t runs = leaders & 0xffffu;
   const bool one = (runs & (runs - 1)) == 0;
   float m = 0.f;
   __nv_bfloat162 m2 = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll
-  for (int pass = 0; pass < 2; ++pass)
+  for (int pass = 0; pass < 2; ++pass) {
+    if (pass == passes) break;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
-      const int r = 16 * pass + i * TOGETHER + sub;
-      if (skipped(pass, i)) continue;
-      const __nv_bfloat162 its = ours >> r & 1 ? abs_max(x[pass][i]) : __floats2bfloat162_rn(0.f, 0.f);
+      const __nv_bfloat162 its = is_ours(pass, i) ? abs_max(x[pass][i]) : __floats2bfloat162_rn(0.f, 0.f);
       m2 = one ? __hmax2(m2, its) : its;
       if (!one) {
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) m2 = __hmax2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
-        if (at == 0) row_max[warp][r] = fmaxf(__low2float(m2), __high2float(m2));
+        if (at == 0) row_max[warp][16 * pass + i * TOGETHER + sub] = fmaxf(__low2float(m2), __high2float(m2));
       }
     }
+  }
   if (one) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m2 = __hmax2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
@@ -378,10 +391,10 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 12) kv8_append_kernel(const
   if (__any_sync(0xffffffffu, m == kInf)) {  // infinities do not count: once more without
     __syncwarp();
 #pragma unroll
-    for (int pass = 0; pass < 2; ++pass)
+    for (int pass = 0; pass < 2; ++pass) {
+      if (pass == passes) break;
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
-        if (skipped(pass, i)) continue;
         float f[8], its = 0.f;
         unpack8v(x[pass][i], f);
 #pragma unroll
@@ -390,6 +403,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 12) kv8_append_kernel(const
         for (int o = LANES / 2; o > 0; o >>= 1) its = fmaxf(its, __shfl_xor_sync(0xffffffffu, its, o));
         if (at == 0) row_max[warp][16 * pass + i * TOGETHER + sub] = its;
       }
+    }
     __syncwarp();
     m = run >= 0 ? row_max[warp][lane] : 0.f;
     if (one) m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
@@ -404,22 +418,32 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 12) kv8_append_kernel(const
   float scale = page_scale(__uint_as_float(top)), ratio = 1.f;  // old scale / new, where it grew over a page that holds tokens
   if (held) scale = fmaxf(scale, old), ratio = old / scale;
   if (mine) *at_scale = scale;
-  const float mul = __shfl_sync(0xffffffffu, 1.f / scale, max(run, 0));
   const int64_t to = (((int64_t)(max(s, 0) >> 4) * hk + head) * 32 + w * 16 + (s & 15)) * D;  // of lane r's row
+  if (one) {  // one row behind the other
+    const int lead = runs ? __ffs(runs) - 1 : 0;
+    const float by = __shfl_sync(0xffffffffu, 1.f / scale, lead);
+    uint8_t* const dst = kv + (__shfl_sync(0xffffffffu, to, lead) + (sub - lead) * D + at);
 #pragma unroll
-  for (int pass = 0; pass < 2; ++pass)
+    for (int pass = 0; pass < 2; ++pass) {
+      if (pass == passes) break;
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-      if (skipped(pass, i)) continue;
-      const int r = 16 * pass + i * TOGETHER + sub;
-      const float by = __shfl_sync(0xffffffffu, mul, r);
-      uint8_t* const dst = kv + (__shfl_sync(0xffffffffu, to, r) + at);
-      if (ours >> r & 1) {
-        float f[8];
-        unpack8v(x[pass][i], f);
-        *reinterpret_cast<uint2*>(dst) = e4m3_of8(f, by);
+      for (int i = 0; i < STEPS; ++i)
+        if (is_ours(pass, i)) *reinterpret_cast<uint2*>(dst + (16 * pass + i * TOGETHER) * D) = e4m3_of8(x[pass][i], by);
+    }
+  } else {
+    const float mul = __shfl_sync(0xffffffffu, 1.f / scale, max(run, 0));
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+      if (pass == passes) break;
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const int r = 16 * pass + i * TOGETHER + sub;
+        const float by = __shfl_sync(0xffffffffu, mul, r);
+        uint8_t* const dst = kv + (__shfl_sync(0xffffffffu, to, r) + at);
+        if (is_ours(pass, i)) *reinterpret_cast<uint2*>(dst) = e4m3_of8(x[pass][i], by);
       }
     }
+  }
   for (uint32_t left = __ballot_sync(0xffffffffu, mine && ratio != 1.f); left; left &= left - 1) {
     const int r = __ffs(left) - 1, its_slot = __shfl_sync(0xffffffffu, s, r);
     const float by = __shfl_sync(0xffffffffu, ratio, r);

@@ -525,7 +525,7 @@ int32_t omni_op_kv_tables(omni_ops* c, const int32_t* lens, const int32_t* add, 
 int32_t omni_op_qk_norm_rope(omni_ops* c, const void* x, int64_t ldx, const void* q_norm, const void* k_norm,
                              const int32_t* pos, int32_t rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                              float eps, float theta, void* out, int64_t ldo) {
-  if (c && (rows > kMostRows || ((int64_t)rows / 4 + 1) * (((int64_t)q_heads + kv_heads) / 8 + 2) > kMostRows))
+  if (c && (rows > kMostRows || ((int64_t)rows / 2 + 1) * (((int64_t)q_heads + kv_heads) / 8 + 2) > kMostRows))
     return c->fail(OMNI_ERR_UNSUPPORTED, "%d rows of %d + %d heads: too many", rows, q_heads, kv_heads);
   if (!c || rows < 0 || !(theta > 0.f)) return c ? c->fail(OMNI_ERR_INVALID, "rows < 0 or theta <= 0") : OMNI_ERR_INVALID;
   if (q_heads < 0 || kv_heads < 0 || q_heads + (int64_t)kv_heads < 1 || q_heads + (int64_t)kv_heads > 65535 || (head_dim != 64 && head_dim != 128))

@@ -569,6 +569,21 @@ def test_attend_not_a_number(ops):
         assert (np.abs(got[part] - want[part]) <= tol[part]).all()
 
 
+@pytest.mark.parametrize("lens", [[40], [700], [9000], [300, 9000], [600] * 300])
+def test_attend_scores_without_bound(ops, lens):
+    """Infinities in a query: the softmax of that head is no number, however the row is cut, and nothing else notices."""
+    hq, hk, d = 2, 1, 128
+    kv, scales, pages, indptr, q = attend_case(hq, hk, d, lens, 43)
+    want, tol = attend_of(q, kv, scales, pages, indptr, lens, hq, hk, d, 0.1)
+    q[len(lens) - 1, 7] = float("inf")
+    out = torch.full((len(lens), hq * d), 5.0, dtype=torch.bfloat16, device="cuda")
+    ops.kv8_attend(q, kv, scales, i32([t - 1 for t in lens]), i32(indptr), i32(pages), hq, 0.1, out)
+    ops.sync()
+    got = f64(out)
+    assert np.isnan(got[-1, :d]).all()
+    assert (np.abs(got[:-1] - want[:-1]) <= tol[:-1]).all() and (np.abs(got[-1, d:] - want[-1, d:]) <= tol[-1, d:]).all()
+
+
 @pytest.mark.parametrize("what", ["page", "negative page", "sequence", "range", "count"])
 def test_attend_outside_its_tables_is_reported(ops, what):
     from pega_omni_b200.ops import OpsError
