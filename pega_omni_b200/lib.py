@@ -6,6 +6,7 @@ Loading fails loudly when the library is missing: there is no fallback path.
 from __future__ import annotations
 
 import ctypes as C
+import operator
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libomni_b200.so"
@@ -92,6 +93,14 @@ P = C.POINTER
 VP = C.c_void_p
 I32 = C.c_int32
 
+
+class Int:
+    """An int32 of a call whose time counts: ctypes takes a Python int as it is in a tenth of the 0.1 us that c_int32 takes."""
+    from_param = operator.index
+
+
+STRIDE = VP  # an int64 likewise: as wide, and in half the time of c_int64
+
 # name -> (restype, argtypes): every symbol the two headers declare
 SYMBOLS = {
     "omni_talker_create": (I32, [P(TalkerCfg), P(Tensor), I32, I32, P(VP)]),
@@ -142,14 +151,14 @@ SYMBOLS = {
     "omni_op_lm_advance": (I32, [VP, VP, VP, C.c_int64, VP, VP, VP, VP, VP, I32]),
     "omni_op_higgs_frame_embed": (I32, [VP, VP, VP, C.c_int64, VP, VP, I32, I32, I32]),
     "omni_op_higgs_sample": (I32, [VP, VP, I32, C.c_float, I32, VP, VP, VP, VP, C.c_int64, VP, I32]),
-    "omni_ops_stream": (I32, [VP, I32, VP]),
-    "omni_op_kv_tables": (I32, [VP, VP, VP, I32, VP, I32, VP, I32, VP, VP, VP, VP, VP, I32, VP, VP, VP, VP, I32, VP]),
-    "omni_op_qk_norm_rope": (I32, [VP, VP, C.c_int64, VP, VP, VP, I32, I32, I32, I32, C.c_float, C.c_float, VP, C.c_int64]),
-    "omni_op_packed_attend": (I32, [VP, VP, C.c_int64, VP, C.c_int64, VP, C.c_int64, VP, I32, I32, I32, I32, I32, C.c_float,
-                                    VP, C.c_int64]),
-    "omni_op_kv8_append": (I32, [VP, VP, C.c_int64, VP, C.c_int64, VP, I32, VP, VP, I32, I32, I32]),
-    "omni_op_kv8_attend": (I32, [VP, VP, C.c_int64, VP, VP, I32, VP, VP, VP, I32, VP, I32, I32, I32, I32, I32, C.c_float,
-                                 VP, C.c_int64]),
+    "omni_ops_stream": (I32, [VP, Int, VP]),
+    "omni_op_kv_tables": (I32, [VP, VP, VP, Int, VP, Int, VP, Int, VP, VP, VP, VP, VP, Int, VP, VP, VP, VP, Int, VP]),
+    "omni_op_qk_norm_rope": (I32, [VP, VP, STRIDE, VP, VP, VP, Int, Int, Int, Int, C.c_float, C.c_float, VP, STRIDE]),
+    "omni_op_packed_attend": (I32, [VP, VP, STRIDE, VP, STRIDE, VP, STRIDE, VP, Int, Int, Int, Int, Int, C.c_float,
+                                    VP, STRIDE]),
+    "omni_op_kv8_append": (I32, [VP, VP, STRIDE, VP, STRIDE, VP, Int, VP, VP, Int, Int, Int]),
+    "omni_op_kv8_attend": (I32, [VP, VP, STRIDE, VP, VP, Int, VP, VP, VP, Int, VP, Int, Int, Int, Int, Int, C.c_float,
+                                 VP, STRIDE]),
     "omni_op_codec_rvq": (I32, [VP, VP, VP, VP, I32, I32, I32]),
     "omni_op_codec_add_norm": (I32, [VP, VP, C.c_int64, VP, VP, VP, I32, I32, C.c_float]),
     "omni_op_codec_window_attend": (I32, [VP, VP, VP, VP, VP, C.c_int64, C.c_int64, VP, I32, I32, C.c_float]),

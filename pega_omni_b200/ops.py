@@ -26,16 +26,18 @@ def _need(ok, what):
 
 def _ints(*tensors):
     """Their addresses: contiguous int32."""
+    at = []
     for t in tensors:
         if t.dtype is not _I32 or not t.is_contiguous():
             raise OpsError("lengths, positions, slots and pages are contiguous int32")
-    return [t.data_ptr() for t in tensors]
+        at.append(t.data_ptr())
+    return at
 
 
 def _rows(t, rows, width, at_least=False):
     """(address, row stride) of bf16 rows, each contiguous."""
     shape, stride = t.shape, t.stride()
-    if t.dtype is not _BF16 or len(shape) != 2 or shape[0] != rows or not (shape[1] == width or at_least and shape[1] > width) or \
+    if t.dtype is not _BF16 or (shape != (rows, width) and not (at_least and len(shape) == 2 and shape[0] == rows and shape[1] > width)) or \
             (stride[1] != 1 and width > 1):
         raise OpsError(f"rows are bf16 [{rows}, {width}], each contiguous: got {t.dtype} {tuple(shape)} with strides {stride}")
     return t.data_ptr(), stride[0] if rows > 1 else shape[1] + 7 & ~7
