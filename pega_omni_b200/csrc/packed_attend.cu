@@ -9,11 +9,13 @@
 // Two kernels, by the sequences' mean length. Both have two tiles of 128 queries on an SM, one's products under the other's exponentials.
 //  - long_kernel: one CTA, whose tiles share their keys: two heads of a group where the group is even, otherwise 256 rows of one
 //    head. A block of K and V is fetched once for both.
-//  - short_kernel: two CTAs of a tile each, which stay and take items (128 rows of a sequence and head) in turns, the longest first and
+//  - short_kernel: two CTAs of a tile each, which stay and take items (a tile's rows of a sequence) in turns, the longest first and
 //    back and forth: an item's Q and K are fetched and its first scores made under the end of the one before. It reads K and V
-//    twice as often.
-// us, long | short, 16 heads of 128 over 8: 28 sequences of 32 to 512 tokens 47 | 39, 16 of 512 52 | 44, 8 of 1,024 66 | 59, 4 of 2,048
-// 79 | 84, 2 of 4,096 126 | 141, 1 of 8,192 229 | 274; 64 of 1 to 120, 14 heads of 64 over 2: 38 | 19.
+//    twice as often. A tile is 128 rows of one head, or as many fewer of each of 2, 4, 8 or 16 heads of a group as halve its number:
+//    less of the last tile of a sequence is empty then.
+// us, long | short with tiles of one head | short, heads of 128: 28 sequences of 32 to 512 tokens, 16 heads over 8 47 | 37 | 36, 32 over 8
+// - | 64 | 56, 16 over 1 - | 35 | 32; 16 of 512, 16 over 8 52 | 38 | 39, 4 of 2,048 77 | 79 | 80, 1 of 8,192 229 | 274 | -; 64 of 1 to 120,
+// 32 over 8 - | 39 | 27; 43 of 6 to 12, 16 over 1 - | 16 | 8.
 // Of a turn of long_kernel (a block of keys for both tiles, 2,900 clocks) the tensor cores have work for 2,050, the exponentials' pipe as
 // much; the rest is the way from the last weights to the next scores. The clock is what power leaves at this rate: 8,192 tokens of
 // 32 heads take 480 us, for 1.9 GHz it would be 380. A cubic for every eighth or fourth exponential, two threads a row, an issuing
@@ -50,6 +52,7 @@ struct Args {
   int apart;  // long_kernel: 1: a CTA's tiles are neighbouring heads, 0: neighbouring rows of one head
   int shift;  // log2 of a CTA's rows
   int slots;  // places for blocks of rows in the grid
+  int span;   // short_kernel: log2 of a tile's rows of one head, of which it holds 128 >> span
 };
 
 using namespace sm100;
@@ -215,12 +218,15 @@ __device__ __forceinline__ void make_weights(Row& row, uint32_t s_at, uint32_t o
   row.l += sum[0].x + sum[0].y + (now == kNegInf ? 0.f : now - now);
 }
 
-// The warp's rows of O over the sums of their weights, `rows` of them at most, to dst. sees(kind, column): the row takes up
+// The warp's rows of O over the sums of their weights. place(r): where row r goes, null: nowhere; sees(kind, column): the row takes up
 // a NaN (0), an infinity (1), a negative infinity (2), asked where `odd`. Through 2 KB of shared memory, 16 bytes of a row in an
 // order of its own: the warp then writes 64 bytes of eight rows at a time, not 16 of 32.
-template <int D, typename Sees>
-__device__ __forceinline__ void write_rows(uint32_t o_at, float l, bool odd, Sees&& sees, unsigned char* stage, bf16* dst, int64_t ldo, int rows, int lane) {
+template <int D, typename Sees, typename Place>
+__device__ __forceinline__ void write_rows(uint32_t o_at, float l, bool odd, Sees&& sees, unsigned char* stage, Place&& place, int lane) {
   const float f = 1.f / l;
+  bf16* dst[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) dst[e] = place(e * 8 + (lane >> 2));
 #pragma unroll 1
   for (int c = 0; c < D; c += 32) {
     float o[32];
@@ -249,10 +255,8 @@ __device__ __forceinline__ void write_rows(uint32_t o_at, float l, bool odd, See
       u[e] = *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4));
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = e * 8 + (lane >> 2);
-      if (r < rows) *reinterpret_cast<uint4*>(dst + r * ldo + c + (lane & 3) * 8) = u[e];
-    }
+    for (int e = 0; e < 4; ++e)
+      if (dst[e]) *reinterpret_cast<uint4*>(dst[e] + c + (lane & 3) * 8) = u[e];
     __syncwarp();
   }
 }
@@ -410,8 +414,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int row_w = begin + quarter * 32;
       // the tile of Q is free now
       write_rows<D>(o_at, sums.l, *reinterpret_cast<volatile int*>(&any_odd) != 0, [&](int kind, int c) { return row >= odd_row[kind][c]; },
-                    raw + (q_at - smem_addr(raw)) + i * BYTES + quarter * 2048, a.out + (int64_t)(first + row_w) * a.ldo + (int64_t)head_of(i) * D,
-                    a.ldo, len - row_w, lane);
+                    raw + (q_at - smem_addr(raw)) + i * BYTES + quarter * 2048,
+                    [&](int r) { return row_w + r < len ? a.out + (int64_t)(first + row_w + r) * a.ldo + (int64_t)head_of(i) * D : nullptr; }, lane);
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -518,7 +522,7 @@ constexpr int kSmem = 3 * kTileBytes<D> + 1024;  // Q, K and V, and what their a
 
 struct Item {
   int first, len;  // of the sequence: first row, rows
-  int row0, head;  // of the item; head < 0: there is none any more
+  int row0, head;  // of the item: its first row, its first head; head < 0: there is none any more
 };
 
 // One of each of what an item or a block needs in turn: a barrier's phase is the item's or the block's number.
@@ -530,35 +534,44 @@ struct Bars {
   uint64_t done;
 };
 
-// The items in their order, for one warp: by blocks of keys, the most first, then by sequence and head.
+// The items in their order, for one warp: by blocks of keys, the most first, then by sequence, row and heads.
 struct Order {
   const Args& a;
   int lane;
-  int level = -1, at_level = 0;  // blocks of the items that come now but one; sequences that have such items
-  int until = 0;                 // as many have items of this level and of those between
-  int base = 0;                  // items in front of them
-  int from_i = 0, from_k = 0;    // sequences that need not be looked at again, and how many of them have such items
+  int units = a.q_heads >> (7 - a.span);  // items of the same rows
+  int level = -1;               // blocks of the items that come now but one
+  int at_level = 0, longer = 0; // tiles of them; sequences that have any
+  int until = 0;                // no sequence ends between this level and the one last counted
+  int base = 0;                 // items in front of them
+  int from_i = 0, from_k = 0;   // sequences that need not be looked at again, and their tiles
 
-  __device__ __forceinline__ int blocks(int i) const {  // of sequence i
+  __device__ __forceinline__ int rows(int i) const {  // of sequence i
     if (i >= a.n) return 0;
     const int from = a.indptr[i], to = a.indptr[i + 1];
-    return from < 0 || to > a.rows || from > to ? 0 : (to - from + kTile - 1) / kTile;
+    return from < 0 || to > a.rows || from > to ? 0 : to - from;
+  }
+  __device__ __forceinline__ static int blocks(int rows) { return (rows + kTile - 1) / kTile; }
+  __device__ __forceinline__ int tiles(int rows) const {  // of this level, of a sequence with so many rows
+    const int left = min(max(rows - level * kTile, 0), kTile);
+    return (left + (1 << a.span) - 1) >> a.span;
   }
   __device__ __forceinline__ void count() {
-    at_level = 0;
-    int next = 0;  // blocks of the longest sequence that has no such item
+    int sum = 0, next = 0;  // next: blocks of the longest sequence that has no such item
+    longer = 0;
     for (int i0 = 0; i0 < a.n; i0 += 32) {
-      const int its = blocks(i0 + lane);
-      at_level += __popc(__ballot_sync(0xffffffffu, its > level));
-      if (its <= level) next = max(next, its);
+      const int its = rows(i0 + lane);
+      sum += tiles(its);
+      longer += __popc(__ballot_sync(0xffffffffu, blocks(its) > level));
+      if (blocks(its) <= level) next = max(next, blocks(its));
     }
+    at_level = (int)__reduce_add_sync(0xffffffffu, (unsigned)sum);
     until = (int)__reduce_max_sync(0xffffffffu, (unsigned)next);
   }
   __device__ __forceinline__ void begin(uint32_t* err) {
     constexpr int kMany = 1 << 25;  // more than there can be
     int most = 0, sum = 0;
     for (int i = lane; i < a.n; i += 32) {
-      const int from = a.indptr[i], to = a.indptr[i + 1], its = blocks(i);
+      const int from = a.indptr[i], to = a.indptr[i + 1], its = blocks(rows(i));
       if ((from < 0 || to > a.rows || from > to) && blockIdx.x == 0) raise(err, kErrBadIndex);
       most = max(most, its), sum = min(sum + its, kMany);
     }
@@ -569,21 +582,28 @@ struct Order {
   }
   // Item t, not in front of the one asked for before.
   __device__ __forceinline__ Item item(int t) {
-    while (level >= 0 && t - base >= at_level * a.q_heads) {
-      base += at_level * a.q_heads;
+    while (level >= 0 && t - base >= at_level * units) {
+      base += at_level * units;
       --level;
       from_i = from_k = 0;
       if (level < until && level >= 0) count();
+      else at_level = longer << (7 - a.span);  // all of the sequences go on beyond this level
     }
-    const int k = (t - base) / a.q_heads, head = t - base - k * a.q_heads;
-    for (; level >= 0 && from_i < a.n; from_i += 32) {  // the k-th sequence that has such an item
-      const uint32_t has = __ballot_sync(0xffffffffu, blocks(from_i + lane) > level);
-      const int c = __popc(has);
-      if (k < from_k + c) {
-        const int i = from_i + (int)__fns(has, 0, k - from_k + 1), from = a.indptr[i];
-        return Item{from, a.indptr[i + 1] - from, level * kTile, head};
+    const int k = (t - base) / units, unit = t - base - k * units;
+    for (; level >= 0 && from_i < a.n; from_i += 32) {  // the sequence that has the k-th tile
+      const int its = tiles(rows(from_i + lane));
+      int incl = its;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
       }
-      from_k += c;
+      const uint32_t has = __ballot_sync(0xffffffffu, from_k + incl > k);
+      if (has) {
+        const int l = __ffs(has) - 1, i = from_i + l, tile = k - from_k - __shfl_sync(0xffffffffu, incl - its, l), from = a.indptr[i];
+        return Item{from, a.indptr[i + 1] - from, level * kTile + (tile << a.span), unit << (7 - a.span)};
+      }
+      from_k += __shfl_sync(0xffffffffu, incl, 31);
     }
     return Item{0, 0, 0, -1};
   }
@@ -621,6 +641,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
     mbar_expect_tx(bar(full), BYTES);
     tma_load_3d(to, map, bar(full), 0, at_row, at_head * (D / 64), hint);
   };
+  const auto fetch_q = [&](const Item& it) {  // rows of its heads, one head behind the other
+    mbar_expect_tx(bar(bars.q_full), BYTES);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) tma_load_4d(q_at + c * (kTile * 128), &qmap, bar(bars.q_full), 0, it.first + it.row0, it.head, c, kEvictFirst);
+  };
   const int group = a.q_heads / a.kv_heads;
   // the first item, and the first of its copies, while the CTA sets itself up
   Order order{a, lane};
@@ -632,9 +657,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
       items[0] = it;
       mbar_arrive(bar(bars.item_full[0]));
       if (it.head >= 0) {
-        fetch(&qmap, q_at, bars.q_full, it.first + it.row0, it.head, kEvictFirst);
+        fetch_q(it);
         fetch(&kmap, k_at, bars.k_full, it.first, it.head / group, kEvictLast);
-        fetch(&vmap, v_at, it.row0 == 0 ? bars.last_full : bars.v_full, it.first, it.head / group, kEvictLast);
+        fetch(&vmap, v_at, it.row0 < kTile ? bars.last_full : bars.v_full, it.first, it.head / group, kEvictLast);
       }
     }
     __syncwarp();
@@ -653,18 +678,19 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
   if (warp < kItemWarp) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16), s_at = lanes, o_at = lanes + kTile;
+    const int local = (warp * 32 + lane) & ((1 << a.span) - 1);  // row of its head's in the tile
     int g = 0;  // blocks so far
     for (int n = 0;; ++n) {
       bool ok = __all_sync(0xffffffffu, item_there(n));
       if (!ok) break;
-      const int blocks = items[n & 1].row0 / kTile + 1;
+      const int blocks = items[n & 1].row0 / kTile + 1, seen = items[n & 1].row0 % kTile + local;  // the last key in the last block that the row sees
       Row sums;
       for (int j = 0; j < blocks; ++j, ++g) {
         ok = __all_sync(0xffffffffu, wait(bars.s_full, g));
         if (!ok) break;
         tc_fence_after_sync();
         const bool last = j == blocks - 1;
-        make_weights<D>(sums, s_at, o_at, a.scale, j == 0, last, warp * 32 + lane, [&](int half) {
+        make_weights<D>(sums, s_at, o_at, a.scale, j == 0, last, seen, [&](int half) {
           // behind the last block's look-through, which P V waits for as well: write_rows() below reads what it found
           if (half == 1 && last) ok = __all_sync(0xffffffffu, wait(bars.last_clean, n));
           if (lane == 0) mbar_arrive(bar(bars.p_full[half]));
@@ -674,13 +700,15 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after_sync();
       const Item it = items[n & 1];
-      const int row_w = it.row0 + warp * 32;
       const auto sees = [&](int kind, int c) {
         const int x = odd_row[n & 1][kind][c];
-        return x >> 8 == n && warp * 32 + lane >= 127 - (x & 255);
+        return x >> 8 == n && seen >= 127 - (x & 255);
       };
-      write_rows<D>(o_at, sums.l, *reinterpret_cast<volatile int*>(&any_odd[n & 1]) == n + 1, sees, stages[warp],
-                    a.out + (int64_t)(it.first + row_w) * a.ldo + (int64_t)it.head * D, a.ldo, it.len - row_w, lane);
+      const auto place = [&](int r) {
+        const int in_tile = warp * 32 + r, row = it.row0 + (in_tile & ((1 << a.span) - 1)), head = it.head + (in_tile >> a.span);
+        return row < it.len ? a.out + (int64_t)(it.first + row) * a.ldo + (int64_t)head * D : nullptr;
+      };
+      write_rows<D>(o_at, sums.l, *reinterpret_cast<volatile int*>(&any_odd[n & 1]) == n + 1, sees, stages[warp], place, lane);
       if (lane == 0) leave_item(n);
       tc_fence_before_sync();  // O has been read: in front of the next item's first weights
     }
@@ -702,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
               // the scores against the block in front are there: K's slot is free, and with an item's last ones Q's; V's behind P V
               ok = wait(bars.s_full, g - 1);
               if (!ok) break;
-              if (j == 0) fetch(&qmap, q_at, bars.q_full, it.first + it.row0, it.head, kEvictFirst);
+              if (j == 0) fetch_q(it);
               fetch(&kmap, k_at, bars.k_full, it.first + j * kTile, it.head / group, kEvictLast);
               ok = wait(bars.v_used, g - 1);
               if (ok) fetch(&vmap, v_at, j + 1 == blocks ? bars.last_full : bars.v_full, it.first + j * kTile, it.head / group, kEvictLast);
@@ -757,7 +785,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
       const int t = tid - kGuardWarp * 32;
       for (int n = 0;; ++n) {
         if (!__all_sync(0xffffffffu, item_there(n))) break;
-        const int keys = items[n & 1].len - items[n & 1].row0;
+        const int keys = items[n & 1].len - items[n & 1].row0 / kTile * kTile;
         __syncwarp();
         if (lane == 0) leave_item(n);
         // Nobody looks at what was found two items ago any more: this item's last V is fetched behind the end of the one before it.
@@ -792,25 +820,34 @@ cudaError_t launch_packed_attend(const PackedAttend& p, int sm_count, uint32_t* 
   a.apart = p.q_heads / p.kv_heads % 2 == 0;
   a.shift = a.apart ? 7 : 8;
   a.slots = (p.rows >> a.shift) + p.n;
+  // heads of a group share a tile's keys as far as their number halves, up to sixteen (eight rows of each, what a swizzled tile's
+  // pattern repeats after)
+  const int group = p.q_heads / p.kv_heads;
+  a.span = 7 - std::min(4, __builtin_ctz(group));
   CUtensorMap maps[3];
   const bf16* at[3] = {p.q, p.k, p.v};
   const int64_t ld[3] = {p.ldq, p.ldk, p.ldv};
   const uint32_t box[3] = {64, kTile, (uint32_t)(D / 64)};
-  for (int i = 0; i < 3; ++i) {
+  const bool is_long = p.rows / p.n >= 2048;
+  for (int i = is_long ? 0 : 1; i < 3; ++i) {
     const uint64_t dims[3] = {64, (uint64_t)p.rows, (uint64_t)(i ? p.kv_heads : p.q_heads) * (D / 64)};
     const uint64_t strides[2] = {(uint64_t)ld[i] * 2, 128};
     if (tc_encode_bf16(&maps[i], at[i], 3, dims, strides, box) != 0) return cudaErrorInvalidValue;
   }
   const auto go = [&](auto d) {
     constexpr int kD = decltype(d)::value;
-    if (p.rows / p.n >= 2048) {
+    if (is_long) {
       const cudaError_t e = allow_large<wide::long_kernel<kD>>(wide::kSmem<kD>);
       if (e != cudaSuccess) return e;
       wide::long_kernel<kD><<<(unsigned)a.slots * (a.q_heads >> a.apart), wide::kThreads, wide::kSmem<kD>, s>>>(maps[0], maps[1], maps[2], a, err);
     } else {
       const cudaError_t e = allow_large<narrow::short_kernel<kD>>(narrow::kSmem<kD>);
       if (e != cudaSuccess) return e;
-      const int64_t items = ((int64_t)p.rows / kTile + p.n) * p.q_heads;  // at most
+      const uint64_t dims[4] = {64, (uint64_t)p.rows, (uint64_t)p.q_heads, (uint64_t)(kD / 64)};
+      const uint64_t strides[3] = {(uint64_t)p.ldq * 2, (uint64_t)kD * 2, 128};
+      const uint32_t tile[4] = {64, 1u << a.span, (uint32_t)kTile >> a.span, 1};
+      if (tc_encode_bf16(&maps[0], p.q, 4, dims, strides, tile) != 0) return cudaErrorInvalidValue;
+      const int64_t items = (((int64_t)p.rows >> a.span) + p.n) * (p.q_heads >> (7 - a.span));  // at most
       const unsigned ctas = (unsigned)std::min<int64_t>(items, (int64_t)sm_count * narrow::kPerSm);
       narrow::short_kernel<kD><<<ctas, narrow::kThreads, narrow::kSmem<kD>, s>>>(maps[0], maps[1], maps[2], a, err);
     }

@@ -190,6 +190,17 @@ def test_sequences_outside_the_rows_are_reported(ops, ptr):
         ops.sync()
 
 
+@pytest.mark.parametrize("hq,hk,d", [(4, 1, 64), (8, 1, 128), (16, 1, 64), (32, 1, 128), (48, 2, 64), (12, 1, 128), (20, 4, 64), (8, 2, 128)])
+@pytest.mark.parametrize("lens", [[9, 1, 0, 70, 8, 17], [300, 129, 64, 65, 5], [1] * 40, [700, 33]])
+def test_heads_that_share_a_tile(ops, hq, hk, d, lens):
+    """Groups of all sizes, whose heads share tiles: what is not finite reaches the rows behind it in each head alike."""
+    check(ops, hq, hk, d, lens, seed=hq, before=3, behind=5)
+    q, k, v, ptr = case(hq, hk, d, lens, seed=hq + 1)
+    at = int(ptr[1]) - 1 - (15 if lens[0] > 20 else 0)  # of the first sequence
+    v[at, 3], v[at, 5], v[int(ptr[0]), 7] = float("nan"), -float("inf"), float("inf")
+    agree(run(ops, q, k, v, ptr, hq, hk, d, 0.1), *attend_of(q, k, v, ptr, hq, hk, d, 0.1), ptr)
+
+
 def test_sequences_over_one_another_end(ops):
     """Many sequences of all the rows: more work than rows and sequences can make is not begun."""
     from pega_omni_b200.ops import OpsError
