@@ -6,20 +6,18 @@
 // P V(1) S(2) .., each group when its P is there - so S(j + 1) having arrived says that P V(j) is done with O, and no other barrier guards it.
 // Softmax has a thread a row of a tile; one warp copies, one issues matrix instructions, two look through values (below).
 //
-// Two kernels, by the sequences' mean length. Both have two tiles of 128 queries on an SM, one's products under the other's exponentials.
-//  - long_kernel: one CTA, whose tiles share their keys: two heads of a group where the group is even, otherwise 256 rows of one
-//    head. A block of K and V is fetched once for both.
-//  - short_kernel: two CTAs of a tile each, which stay and take items (a tile's rows of a sequence) in turns, the longest first and
-//    back and forth: an item's Q and K are fetched and its first scores made under the end of the one before. It reads K and V
-//    twice as often. A tile is 128 rows of one head, or as many fewer of each of 2, 4, 8 or 16 heads of a group as halve its number:
-//    less of the last tile of a sequence is empty then.
-// us, long | short with tiles of one head | short, heads of 128: 28 sequences of 32 to 512 tokens, 16 heads over 8 47 | 37 | 36, 32 over 8
-// - | 64 | 56, 16 over 1 - | 35 | 32; 16 of 512, 16 over 8 52 | 38 | 39, 4 of 2,048 77 | 79 | 80, 1 of 8,192 229 | 274 | -; 64 of 1 to 120,
-// 32 over 8 - | 39 | 27; 43 of 6 to 12, 16 over 1 - | 16 | 8.
-// Of a turn of long_kernel (a block of keys for both tiles, 2,900 clocks) the tensor cores have work for 2,050, the exponentials' pipe as
-// much; the rest is the way from the last weights to the next scores. The clock is what power leaves at this rate: 8,192 tokens of
-// 32 heads take 480 us, for 1.9 GHz it would be 380. A cubic for every eighth or fourth exponential, two threads a row, an issuing
-// warp a tile (which lets both tiles fall into step) and weights in unequal parts made it no faster.
+// CTAs stay and take items (a tile's or two tiles' rows of a sequence) in turns, the longest first and back and forth: an item's Q and K
+// are fetched and its first scores made under the end of the one before. A tile is 128 rows of one head, or as many fewer of each of 2, 4,
+// 8 or 16 heads of a group as halve its number: less of a sequence's last tile is empty then (43 sequences of 6 to 12 tokens, 16 heads of
+// 128 over one: 8.3 us instead of 16.2, 64 of 1 to 120, 32 over 8: 28 instead of 39; 16 of 512, 16 over 8: 39 instead of 38).
+//
+// Two kernels, chosen below; both have two tiles on an SM, one's products under the other's exponentials.
+//  - paired_kernel: one CTA, whose tiles are other heads of the same group and rows, so that a block of K and V is fetched once for both.
+//  - single_kernel: two CTAs of a tile each, which read K and V twice as often, but are out of step at an item's end, and smaller.
+// Of a turn of paired_kernel (a block of keys for both tiles, 3,400 clocks) the tensor cores have work for 2,050, the exponentials' pipe as
+// much; the rest is the way from the last weights to the next scores, and an item's end. The clock is what power leaves at this rate: 8,192
+// tokens of 32 heads take 450 to 490 us. A cubic for every eighth or fourth exponential, two threads a row, an issuing
+// warp a tile (which lets both tiles fall into step), weights in unequal parts and 32-byte stores of results from registers made it no faster.
 //
 // Scores, maxima, sums and O are f32. Weights go to bf16 because V does (one type for both operands): 2^-8 at most of a weight,
 // which averages out over a row's keys and is what the result itself is rounded by. A row's reference is a maximum that may lag by
@@ -49,10 +47,8 @@ struct Args {
   float scale;  // of scores in powers of two
   bf16* out;
   int64_t ldo;
-  int apart;  // long_kernel: 1: a CTA's tiles are neighbouring heads, 0: neighbouring rows of one head
-  int shift;  // log2 of a CTA's rows
-  int slots;  // places for blocks of rows in the grid
-  int span;   // short_kernel: log2 of a tile's rows of one head, of which it holds 128 >> span
+  int span;   // log2 of a tile's rows of one head, of which it holds 128 >> span
+  int share;  // log2 of an item's heads
 };
 
 using namespace sm100;
@@ -298,247 +294,18 @@ __device__ __forceinline__ void look_through(unsigned char* v, int keys, int t, 
   __syncwarp();
 }
 
-// ---- long sequences ------------------------------------------------------------------------------------------------------
-
-namespace wide {
-
-constexpr int kThreads = 384;
-constexpr int kCopyWarp = 8, kMmaWarp = 9, kGuardWarp = 10;
-constexpr int kKeys = 2;  // blocks of K in shared memory
-template <int D>
-constexpr int kValues = D == 128 ? 3 : 4;  // of V
-template <int D>
-constexpr int kSmem = (2 + kKeys + kValues<D>) * kTileBytes<D> + 1024;  // and what the tiles' alignment costs
-constexpr uint32_t kColumns = 512;  // of TMEM: S of both tiles, then O
-constexpr int kO = 2 * kTile;
-constexpr int kNever = 0x7fffffff;
-
-struct Bars {
-  uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], k_full[4], v_full[4], v_used[4], odd_full[2], odd_clean[2], done;
-};
-
-template <int D>
-__global__ void __launch_bounds__(kThreads, 1)
-    long_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                         const __grid_constant__ Args a, uint32_t* err) {
-  constexpr int KS = kKeys, VS = kValues<D>, BYTES = kTileBytes<D>;
-  extern __shared__ unsigned char raw[];
-  __shared__ Bars bars;
-  __shared__ uint32_t tmem_slot;
-  __shared__ int found, any_odd;
-  __shared__ int odd_row[3][D];  // first row of a NaN, an infinity, a negative infinity in a column of V, where rows must not see all
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
-  const uint32_t q_at = base, k_at = base + 2 * BYTES, v_at = k_at + KS * BYTES;
-  const auto bar = [](uint64_t& b) { return smem_addr(&b); };
-
-  // on their way while the CTA sets itself up
-  int from = tid < a.n ? a.indptr[tid] : 0, to = tid < a.n ? a.indptr[tid + 1] : 0;
-  if (warp == kMmaWarp) tmem_alloc(smem_addr(&tmem_slot), kColumns);
-  if (tid == kCopyWarp * 32) {
-    prefetch_tensormap(&qmap), prefetch_tensormap(&kmap), prefetch_tensormap(&vmap);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(bars.q_full[i]), 1), mbar_init(bar(bars.s_full[i]), 1), mbar_init(bar(bars.o_full[i]), 1);
-      mbar_init(bar(bars.p_full[i][0]), 4), mbar_init(bar(bars.p_full[i][1]), 4);
-      mbar_init(bar(bars.odd_full[i]), 1), mbar_init(bar(bars.odd_clean[i]), 2);
-    }
-    for (int i = 0; i < 4; ++i) mbar_init(bar(bars.k_full[i]), 1), mbar_init(bar(bars.v_full[i]), 1), mbar_init(bar(bars.v_used[i]), 1);
-    mbar_init(bar(bars.done), 1);
-    mbar_init_fence();
-  }
-  // the block of rows and the heads; the last blocks, which have the most keys, first
-  const int units = a.q_heads >> a.apart;
-  const int slot = a.slots - 1 - (int)blockIdx.x / units, unit = blockIdx.x % units;
-  if (tid == 0) found = -1, any_odd = 0;
-  for (int i = tid; i < 3 * D; i += kThreads) (&odd_row[0][0])[i] = kNever;
-  tc_fence_before_sync();
-  __syncthreads();
-  // A sequence's blocks are behind those that the ones in front can have at most: from place (rows in front >> shift) + their number on.
-  for (int i = tid; i < a.n; i += kThreads) {
-    if (i != tid) from = a.indptr[i], to = a.indptr[i + 1];
-    const int place = slot - ((from >> a.shift) + i);
-    if (from < 0 || to > a.rows || from > to) {
-      if (unit == 0) raise(err, kErrBadIndex);
-    } else if (place >= 0 && ((int64_t)place << a.shift) < to - from) {
-      atomicMax(&found, i);  // there is one, where all ascend
-    }
-  }
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = tmem_slot;
-  const int seq = found;
-  if (seq < 0) {
-    if (warp == kMmaWarp) tmem_dealloc(tmem, kColumns);
-    return;
-  }
-  const int first = a.indptr[seq], len = a.indptr[seq + 1] - first, row0 = (slot - ((first >> a.shift) + seq)) << a.shift;
-
-  const int group = a.q_heads / a.kv_heads;
-  const int head0 = unit << a.apart, kv_head = head0 / group;
-  // tile i: head, first row, blocks of keys
-  const auto head_of = [&](int i) { return head0 + (a.apart ? i : 0); };
-  const auto begin_of = [&](int i) { return row0 + (a.apart ? 0 : i * kTile); };
-  const auto blocks_of = [&](int i) { return begin_of(i) < len ? begin_of(i) / kTile + 1 : 0; };
-  const int last_tile = blocks_of(1) > 0 ? 1 : 0, all = blocks_of(last_tile);
-  const int seen_by_all = row0 / kTile;  // blocks of keys before this one are; one block or two are not
-
-  // Blocks of V that are looked through have barriers of their own, since the warps that do it do not follow the ring.
-  const auto k_filled = [&](int j) { return mbar_wait(bar(bars.k_full[j % KS]), (j / KS) & 1, err); };
-  const auto v_filled = [&](int j) {
-    return j >= seen_by_all ? mbar_wait(bar(bars.odd_full[j - seen_by_all]), 0, err) : mbar_wait(bar(bars.v_full[j % VS]), (j / VS) & 1, err);
-  };
-  const auto v_clean = [&](int j) { return j >= seen_by_all ? mbar_wait(bar(bars.odd_clean[j - seen_by_all]), 0, err) : v_filled(j); };
-
-  // registers: 256 * 224 + 128 * 56 = 384 * 168, what the launch has
-  if (warp < kCopyWarp) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    const int i = warp >> 2, quarter = warp & 3;
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t s_at = lanes + i * kTile, o_at = lanes + kO + i * kTile;
-    const int begin = begin_of(i), blocks = blocks_of(i);
-    const int row = begin + quarter * 32 + lane;  // of the sequence
-    Row sums;
-    bool ok = true;
-    for (int j = 0; j < blocks; ++j) {
-      ok = __all_sync(0xffffffffu, mbar_wait(bar(bars.s_full[i]), j & 1, err));
-      if (!ok) break;
-      tc_fence_after_sync();
-      make_weights<D>(sums, s_at, o_at, a.scale, j == 0, j == blocks - 1, quarter * 32 + lane, [&](int half) {
-        if (lane == 0) mbar_arrive(bar(bars.p_full[i][half]));
-      });
-    }
-    ok = ok && blocks > 0 && mbar_wait(bar(bars.o_full[i]), 0, err);
-    for (int j = seen_by_all; j < all && ok; ++j) ok = v_clean(j);
-    if (__all_sync(0xffffffffu, ok)) {
-      tc_fence_after_sync();
-      const int row_w = begin + quarter * 32;
-      // the tile of Q is free now
-      write_rows<D>(o_at, sums.l, *reinterpret_cast<volatile int*>(&any_odd) != 0, [&](int kind, int c) { return row >= odd_row[kind][c]; },
-                    raw + (q_at - smem_addr(raw)) + i * BYTES + quarter * 2048,
-                    [&](int r) { return row_w + r < len ? a.out + (int64_t)(first + row_w + r) * a.ldo + (int64_t)head_of(i) * D : nullptr; }, lane);
-    }
-  } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == kCopyWarp) {
-      if (elect_one()) {
-        const auto fetch = [&](const CUtensorMap* map, uint32_t to, uint32_t full, int at_row, int at_head, uint64_t hint) {
-          mbar_expect_tx(full, BYTES);
-          tma_load_3d(to, map, full, 0, first + at_row, at_head * (D / 64), hint);
-        };
-        int k_n = 0, v_n = 0;  // blocks asked for
-        bool ok = true;
-        for (int j = 0; j < all; ++j) {
-          // With tile 0's scores against the block in front there, both tiles are done with the one before that, and a tile alone
-          // with this one, too: K's slot is free. V's is when v_used says so.
-          if (j > 0) ok = mbar_wait(bar(bars.s_full[0]), (j - 1) & 1, err);
-          if (!ok) break;
-          if (j == 0) fetch(&qmap, q_at, bar(bars.q_full[0]), begin_of(0), head_of(0), kEvictFirst);
-          fetch(&kmap, k_at + j % KS * BYTES, bar(bars.k_full[j % KS]), j * kTile, kv_head, kEvictLast);
-          ++k_n;
-          if (j == 0 && last_tile == 1) fetch(&qmap, q_at + BYTES, bar(bars.q_full[1]), begin_of(1), head_of(1), kEvictFirst);
-          if (j >= VS) ok = mbar_wait(bar(bars.v_used[(j - VS) % 4]), ((j - VS) / 4) & 1, err);
-          if (!ok) break;
-          fetch(&vmap, v_at + j % VS * BYTES, j >= seen_by_all ? bar(bars.odd_full[j - seen_by_all]) : bar(bars.v_full[j % VS]), j * kTile, kv_head, kEvictLast);
-          ++v_n;
-        }
-        if (!ok) {  // the copies under way land in shared memory
-          for (int j = max(0, k_n - KS); j < k_n; ++j) k_filled(j);
-          for (int j = max(0, v_n - VS); j < v_n; ++j) v_filled(j);
-          for (int i = 0; i <= last_tile; ++i) mbar_wait(bar(bars.q_full[i]), 0, err);
-        }
-      }
-    } else if (warp == kMmaWarp) {
-      // one thread for all tiles, in turns: it keeps two apart, so that one's products run under the other's exponentials
-      if (elect_one()) {
-        const auto scores = [&](int i, int j) {  // S of tile i against keys j
-          issue_scores<D>(tmem + i * kTile, q_at + i * BYTES, k_at + j % KS * BYTES);
-          mma_commit(bar(bars.s_full[i]));
-        };
-        // Turn j: P V(j) and S(j + 1) of the tiles. V was waited for in the turn before, K is between the weights' halves.
-        bool ok = k_filled(0);
-        for (int i = 0; i <= last_tile && ok; ++i) {
-          ok = mbar_wait(bar(bars.q_full[i]), 0, err);
-          if (!ok) break;
-          tc_fence_after_sync();
-          scores(i, 0);
-        }
-        ok = ok && v_clean(0);
-        for (int j = 0; j < all && ok; ++j) {
-          for (int i = 0; i <= last_tile && ok; ++i) {
-            const int blocks = blocks_of(i);
-            if (j < blocks) {
-              const uint32_t v = v_at + j % VS * BYTES;
-              for (int half = 0; half < 2 && ok; ++half) {  // of the block's keys, whose weights come in turn
-                ok = mbar_wait(bar(bars.p_full[i][half]), j & 1, err);
-                if (!ok) break;
-                tc_fence_after_sync();
-                issue_sums<D>(tmem + kO + i * kTile, tmem + i * kTile, v, half, j == 0);
-                if (half == 0 && i == 0 && j + 1 < all) ok = k_filled(j + 1);
-              }
-              if (!ok) break;
-              if (i == last_tile && j + VS < all) mma_commit(bar(bars.v_used[j % 4]));
-              if (j + 1 < blocks) scores(i, j + 1);
-              else mma_commit(bar(bars.o_full[i]));
-            }
-            if (ok && i == 0 && j + 1 < all) ok = v_clean(j + 1);
-          }
-        }
-        if (!ok) {  // what is under way uses shared memory and TMEM
-          mma_commit(bar(bars.done));
-          mbar_wait(bar(bars.done), 0, err);
-        }
-      }
-    } else {
-      const int t = tid - kGuardWarp * 32;
-      for (int j = seen_by_all; j < all; ++j) {
-        if (!v_filled(j)) break;
-        look_through<D>(raw + (v_at - smem_addr(raw)) + j % VS * BYTES, len - j * kTile, t, [&](int kind, int c, int r) {
-          atomicMin(&odd_row[kind][c], j * kTile + r);
-          any_odd = 1;
-        });
-        if (lane == 0) mbar_arrive(bar(bars.odd_clean[j - seen_by_all]));
-      }
-    }
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  if (warp == kMmaWarp) {
-    tc_fence_after_sync();
-    tmem_dealloc(tmem, kColumns);
-  }
-}
-
-}  // namespace wide
-
-// ---- short sequences -------------------------------------------------------------------------------------------------------
-
-namespace narrow {
-
-constexpr int kThreads = 256, kPerSm = 2;
-constexpr int kItemWarp = 4, kMmaWarp = 5, kGuardWarp = 6;
-constexpr uint32_t kColumns = 256;  // of TMEM: S, then O
-template <int D>
-constexpr int kSmem = 3 * kTileBytes<D> + 1024;  // Q, K and V, and what their alignment costs
+// ---- items -----------------------------------------------------------------------------------------------------------------
 
 struct Item {
   int first, len;  // of the sequence: first row, rows
   int row0, head;  // of the item: its first row, its first head; head < 0: there is none any more
 };
 
-// One of each of what an item or a block needs in turn: a barrier's phase is the item's or the block's number.
-struct Bars {
-  uint64_t item_full[2], item_empty[2];
-  uint64_t q_full, o_full, last_full, last_clean;  // by items; the last block of V has barriers of its own
-  uint64_t k_full, s_full, p_full[2], v_used;      // by blocks
-  uint64_t v_full;                                 // by blocks that are not an item's last
-  uint64_t done;
-};
-
 // The items in their order, for one warp: by blocks of keys, the most first, then by sequence, row and heads.
 struct Order {
   const Args& a;
   int lane;
-  int units = a.q_heads >> (7 - a.span);  // items of the same rows
+  int units = a.q_heads >> a.share;  // items of the same rows
   int level = -1;               // blocks of the items that come now but one
   int at_level = 0, longer = 0; // tiles of them; sequences that have any
   int until = 0;                // no sequence ends between this level and the one last counted
@@ -601,7 +368,7 @@ struct Order {
       const uint32_t has = __ballot_sync(0xffffffffu, from_k + incl > k);
       if (has) {
         const int l = __ffs(has) - 1, i = from_i + l, tile = k - from_k - __shfl_sync(0xffffffffu, incl - its, l), from = a.indptr[i];
-        return Item{from, a.indptr[i + 1] - from, level * kTile + (tile << a.span), unit << (7 - a.span)};
+        return Item{from, a.indptr[i + 1] - from, level * kTile + (tile << a.span), unit << a.share};
       }
       from_k += __shfl_sync(0xffffffffu, incl, 31);
     }
@@ -609,9 +376,28 @@ struct Order {
   }
 };
 
+// ---- one tile at a time ---------------------------------------------------------------------------------------------------
+
+namespace single {
+
+constexpr int kThreads = 256, kPerSm = 2;
+constexpr int kItemWarp = 4, kMmaWarp = 5, kGuardWarp = 6;
+constexpr uint32_t kColumns = 256;  // of TMEM: S, then O
+template <int D>
+constexpr int kSmem = 3 * kTileBytes<D> + 1024;  // Q, K and V, and what their alignment costs
+
+// One of each of what an item or a block needs in turn: a barrier's phase is the item's or the block's number.
+struct Bars {
+  uint64_t item_full[2], item_empty[2];
+  uint64_t q_full, o_full, last_full, last_clean;  // by items; the last block of V has barriers of its own
+  uint64_t k_full, s_full, p_full[2], v_used;      // by blocks
+  uint64_t v_full;                                 // by blocks that are not an item's last
+  uint64_t done;
+};
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, kPerSm)
-    short_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+    single_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                          const __grid_constant__ Args a, uint32_t* err) {
   constexpr int BYTES = kTileBytes<D>;
   extern __shared__ unsigned char raw[];
@@ -806,7 +592,267 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
   }
 }
 
-}  // namespace narrow
+}  // namespace single
+
+// ---- two tiles that share their keys ------------------------------------------------------------------------------------------
+
+namespace paired {
+
+constexpr int kThreads = 384;
+constexpr int kItemWarp = 8, kMmaWarp = 9, kGuardWarp = 10;
+constexpr uint32_t kColumns = 512;  // of TMEM: S of both tiles, then O
+constexpr int kO = 2 * kTile;
+template <int D>
+constexpr int kSmem = 6 * kTileBytes<D> + 1024;  // Q of both tiles, two blocks of K, two of V, and what their alignment costs
+
+// A barrier's phase is the number of what it stands for: an item (with two of them, half of it), a block, a use of a slot, or a block
+// that is not an item's last on a slot. With one for every item, the slowest of those that wait could be two phases behind.
+struct Bars {
+  uint64_t item_full[2], item_empty[2], last_full[2], last_clean[2];  // by every other item
+  uint64_t q_full, q_used, o_full[2];                                 // by items; o_full of each tile
+  uint64_t s_full[2], p_full[2][2];                                   // by blocks, of each tile
+  uint64_t k_full[2], k_used[2], v_used[2];                           // by uses of a slot
+  uint64_t v_full[2];                                                 // by uses by blocks that are not an item's last
+  uint64_t done;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    paired_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                  const __grid_constant__ Args a, uint32_t* err) {
+  constexpr int BYTES = kTileBytes<D>;
+  extern __shared__ unsigned char raw[];
+  __shared__ Bars bars;
+  __shared__ Item items[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int any_odd[2], odd_row[2][3][D];                // as in single_kernel
+  __shared__ __align__(16) unsigned char stages[8][32 * 64];  // 32 columns of a warp's rows on their way out
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
+  const uint32_t q_at = base, k_at = base + 2 * BYTES, v_at = base + 4 * BYTES;
+  const auto bar = [](uint64_t& b) { return smem_addr(&b); };
+  const auto wait = [&](uint64_t& b, int phase) { return mbar_wait(smem_addr(&b), phase & 1, err); };
+
+  if (warp == kMmaWarp) tmem_alloc(smem_addr(&tmem_slot), kColumns);
+  if (tid == kItemWarp * 32) {
+    prefetch_tensormap(&qmap), prefetch_tensormap(&kmap), prefetch_tensormap(&vmap);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(bars.item_full[i]), 1), mbar_init(bar(bars.item_empty[i]), 11);
+      mbar_init(bar(bars.last_full[i]), 1), mbar_init(bar(bars.last_clean[i]), 2);
+      mbar_init(bar(bars.o_full[i]), 1), mbar_init(bar(bars.s_full[i]), 1);
+      mbar_init(bar(bars.p_full[i][0]), 4), mbar_init(bar(bars.p_full[i][1]), 4);
+      mbar_init(bar(bars.k_full[i]), 1), mbar_init(bar(bars.k_used[i]), 1), mbar_init(bar(bars.v_full[i]), 1), mbar_init(bar(bars.v_used[i]), 1);
+    }
+    mbar_init(bar(bars.q_full), 1), mbar_init(bar(bars.q_used), 1), mbar_init(bar(bars.done), 1);
+    mbar_init_fence();
+  }
+  const int group = a.q_heads / a.kv_heads;
+  const auto fetch = [&](const CUtensorMap* map, uint32_t to, uint64_t& full, const Item& it, int j) {  // block j of K or V
+    mbar_expect_tx(bar(full), BYTES);
+    tma_load_3d(to, map, bar(full), 0, it.first + j * kTile, it.head / group * (D / 64), kEvictLast);
+  };
+  const auto fetch_q = [&](const Item& it) {  // rows of its heads, one head behind the other
+    mbar_expect_tx(bar(bars.q_full), 2 * BYTES);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c)
+        tma_load_4d(q_at + i * BYTES + c * (kTile * 128), &qmap, bar(bars.q_full), 0, it.first + it.row0, it.head + (i << (a.share - 1)), c, kEvictFirst);
+  };
+  const auto blocks_of = [](const Item& it) { return it.row0 / kTile + 1; };
+  // the first item, and the first of its copies, while the CTA sets itself up
+  Order order{a, lane};
+  Item it{0, 0, 0, -1};  // of the item warp
+  if (warp == kItemWarp) {
+    order.begin(err);
+    it = order.item(blockIdx.x);
+    if (lane == 0) {
+      items[0] = it;
+      mbar_arrive(bar(bars.item_full[0]));
+      if (it.head >= 0) {
+        fetch(&kmap, k_at, bars.k_full[0], it, 0);
+        fetch_q(it);
+        fetch(&vmap, v_at, it.row0 < kTile ? bars.last_full[0] : bars.v_full[0], it, 0);
+      }
+    }
+    __syncwarp();
+  }
+  for (int i = tid; i < 2 * 3 * D; i += kThreads) (&odd_row[0][0][0])[i] = -1;
+  if (tid < 2) any_odd[tid] = 0;
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+
+  const auto item_there = [&](int n) { return wait(bars.item_full[n & 1], n >> 1) && items[n & 1].head >= 0; };
+  const auto leave_item = [&](int n) { mbar_arrive(bar(bars.item_empty[n & 1])); };
+
+  // registers: 256 * 216 + 128 * 72 = 384 * 168, what the launch has
+  if (warp < kItemWarp) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int i = warp >> 2, quarter = warp & 3;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), s_at = lanes + i * kTile, o_at = lanes + kO + i * kTile;
+    const int local = (quarter * 32 + lane) & ((1 << a.span) - 1);  // row of its head's in the tile
+    int g = 0;  // blocks so far
+    for (int n = 0;; ++n) {
+      bool ok = __all_sync(0xffffffffu, item_there(n));
+      if (!ok) break;
+      const int blocks = blocks_of(items[n & 1]), seen = items[n & 1].row0 % kTile + local;  // the last key in the last block that the row sees
+      Row sums;
+      for (int j = 0; j < blocks; ++j, ++g) {
+        ok = __all_sync(0xffffffffu, wait(bars.s_full[i], g));
+        if (!ok) break;
+        tc_fence_after_sync();
+        const bool last = j == blocks - 1;
+        make_weights<D>(sums, s_at, o_at, a.scale, j == 0, last, seen, [&](int half) {
+          // behind the last block's look-through, which P V waits for as well: write_rows() below reads what it found
+          if (half == 1 && last) ok = __all_sync(0xffffffffu, wait(bars.last_clean[n & 1], n >> 1));
+          if (lane == 0) mbar_arrive(bar(bars.p_full[i][half]));
+        });
+      }
+      ok = ok && wait(bars.o_full[i], n);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after_sync();
+      const Item it = items[n & 1];
+      const auto sees = [&](int kind, int c) {
+        const int x = odd_row[n & 1][kind][c];
+        return x >> 8 == n && seen >= 127 - (x & 255);
+      };
+      const auto place = [&](int r) {
+        const int in_tile = quarter * 32 + r, row = it.row0 + (in_tile & ((1 << a.span) - 1)), head = it.head + (i << (a.share - 1)) + (in_tile >> a.span);
+        return row < it.len ? a.out + (int64_t)(it.first + row) * a.ldo + (int64_t)head * D : nullptr;
+      };
+      write_rows<D>(o_at, sums.l, *reinterpret_cast<volatile int*>(&any_odd[n & 1]) == n + 1, sees, stages[warp], place, lane);
+      if (lane == 0) leave_item(n);
+      tc_fence_before_sync();  // O has been read: in front of the next item's first weights
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == kItemWarp) {
+      int g = 0, v0 = 0, v1 = 0;                     // blocks so far; of those that are not an item's last, on each slot
+      int k_n = it.head >= 0, q_n = k_n, last_n = -1;  // copies of K and Q asked for; the item whose last V is
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        if (n > 0) it = order.item(n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x));
+        if (lane == 0) {
+          if (n > 0) {
+            ok = n < 2 || wait(bars.item_empty[n & 1], (n >> 1) - 1);
+            if (ok) items[n & 1] = it, mbar_arrive(bar(bars.item_full[n & 1]));
+          }
+          const int blocks = it.head < 0 ? 0 : blocks_of(it);
+          for (int j = 0; j < blocks && ok; ++j, ++g) {
+            const int slot = g & 1, use = g >> 1;
+            const bool last = j + 1 == blocks;
+            if (g > 0) {
+              ok = use == 0 || wait(bars.k_used[slot], use - 1);
+              if (!ok) break;
+              fetch(&kmap, k_at + slot * BYTES, bars.k_full[slot], it, j), ++k_n;
+              if (j == 0) {
+                ok = wait(bars.q_used, n - 1);
+                if (ok) fetch_q(it), ++q_n;
+              }
+              ok = ok && (use == 0 || wait(bars.v_used[slot], use - 1));
+              if (ok) fetch(&vmap, v_at + slot * BYTES, last ? bars.last_full[n & 1] : bars.v_full[slot], it, j);
+            }
+            if (ok && last) last_n = n;
+            else if (ok) ++(slot ? v1 : v0);
+          }
+          if (!ok) {  // the copies under way land in shared memory
+            for (int i = 0; i < 2; ++i) {
+              const int uses = (k_n + 1 - i) / 2, plain = i ? v1 : v0, item = last_n - i;
+              if (uses > 0) wait(bars.k_full[i], uses - 1);
+              if (plain > 0) wait(bars.v_full[i], plain - 1);
+              if (item >= 0) wait(bars.last_full[item & 1], item >> 1);
+            }
+            if (q_n > 0) wait(bars.q_full, q_n - 1);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (it.head < 0) break;
+      }
+    } else if (warp == kMmaWarp) {
+      if (elect_one()) {
+        const auto scores = [&](int i, int g, bool frees_q) {  // of tile i against block g
+          issue_scores<D>(tmem + i * kTile, q_at + i * BYTES, k_at + (g & 1) * BYTES);
+          mma_commit(bar(bars.s_full[i]));
+          if (i == 0) return;
+          mma_commit(bar(bars.k_used[g & 1]));
+          if (frees_q) mma_commit(bar(bars.q_used));
+        };
+        int g = 0, v0 = 0, v1 = 0, blocks = 0;
+        bool more = item_there(0), ok = true;
+        if (more) {
+          blocks = blocks_of(items[0]);
+          leave_item(0);
+          ok = wait(bars.q_full, 0) && wait(bars.k_full[0], 0);
+          if (ok) {
+            tc_fence_after_sync();
+            scores(0, 0, false), scores(1, 0, blocks == 1);
+          }
+        }
+        for (int n = 0; more && ok; ++n) {
+          int next = 0;  // blocks of the next item
+          for (int j = 0; j < blocks && ok; ++j, ++g) {
+            const bool last = j + 1 == blocks;
+            const int slot = g & 1;
+            ok = last ? wait(bars.last_clean[n & 1], n >> 1) : wait(bars.v_full[slot], slot ? v1++ : v0++);
+            for (int i = 0; i < 2 && ok; ++i) {
+              for (int half = 0; half < 2 && ok; ++half) {  // of the block's keys, whose weights come in turn
+                ok = wait(bars.p_full[i][half], g);
+                if (!ok) break;
+                tc_fence_after_sync();
+                issue_sums<D>(tmem + kO + i * kTile, tmem + i * kTile, v_at + slot * BYTES, half, j == 0);
+              }
+              if (!ok) break;
+              if (last) mma_commit(bar(bars.o_full[i]));
+              if (i == 1) mma_commit(bar(bars.v_used[slot]));
+              if (i == 0) {  // what comes behind: the item's next block, or the next item's first
+                more = !last || item_there(n + 1);
+                if (last && more) {
+                  next = blocks_of(items[(n + 1) & 1]);
+                  leave_item(n + 1);
+                  ok = wait(bars.q_full, n + 1);
+                }
+                if (more && ok) ok = wait(bars.k_full[(g + 1) & 1], (g + 1) >> 1);
+                tc_fence_after_sync();
+              }
+              if (more && ok) scores(i, g + 1, last ? next == 1 : j + 2 == blocks);
+            }
+          }
+          blocks = next;
+        }
+        // what is under way uses shared memory and TMEM
+        mma_commit(bar(bars.done));
+        wait(bars.done, 0);
+      }
+    } else {
+      const int t = tid - kGuardWarp * 32;
+      int g = -1;  // the item's last block
+      for (int n = 0;; ++n) {
+        if (!__all_sync(0xffffffffu, item_there(n))) break;
+        const int keys = items[n & 1].len - items[n & 1].row0 / kTile * kTile;
+        g += blocks_of(items[n & 1]);
+        __syncwarp();
+        if (lane == 0) leave_item(n);
+        // Nobody looks at what was found two items ago any more: both tiles have left that item, or this one would not be here.
+        if (!__all_sync(0xffffffffu, wait(bars.last_full[n & 1], n >> 1))) break;
+        look_through<D>(raw + (v_at - smem_addr(raw)) + (g & 1) * BYTES, keys, t, [&](int kind, int c, int r) {
+          atomicMax(&odd_row[n & 1][kind][c], n * 256 + 127 - r);
+          any_odd[n & 1] = n + 1;
+        });
+        if (lane == 0) mbar_arrive(bar(bars.last_clean[n & 1]));
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, kColumns);
+  }
+}
+
+}  // namespace paired
 
 }  // namespace
 
@@ -817,39 +863,45 @@ cudaError_t launch_packed_attend(const PackedAttend& p, int sm_count, uint32_t* 
   a.indptr = p.indptr, a.n = p.n, a.rows = p.rows, a.q_heads = p.q_heads, a.kv_heads = p.kv_heads;
   a.scale = p.scale * 1.44269504088896340736f;
   a.out = p.out, a.ldo = p.ldo;
-  a.apart = p.q_heads / p.kv_heads % 2 == 0;
-  a.shift = a.apart ? 7 : 8;
-  a.slots = (p.rows >> a.shift) + p.n;
-  // heads of a group share a tile's keys as far as their number halves, up to sixteen (eight rows of each, what a swizzled tile's
-  // pattern repeats after)
-  const int group = p.q_heads / p.kv_heads;
-  a.span = 7 - std::min(4, __builtin_ctz(group));
+  // Heads of a group share an item's keys as far as their number halves: up to sixteen a tile, eight rows of each, which a swizzled
+  // tile's pattern repeats after. Pairs of tiles where the group is even, there is work for every SM and a half more, and sequences have
+  // two items' rows in the mean. us, single | paired, 16 heads of 128 over 8: 1 of 2,048 tokens (0.9 items an SM) 36 | 38, 2 of 2,048 (1.8) 45 |
+  // 42, 1 of 8,192 250 | 229; 30 of 130 tokens (1 item's rows) 24 | 30, 28 of 32 to 512 (2.1) 36 | 35, 16 of 512 (4) 40 | 37.
+  const int halves = __builtin_ctz(p.q_heads / p.kv_heads);
+  const auto items_of = [&](int share, int tiles) {  // at most
+    a.share = share, a.span = 6 + tiles - share;
+    return (((int64_t)p.rows >> a.span) + p.n) * (p.q_heads >> share);
+  };
+  int64_t items = items_of(std::min(5, halves), 2);
+  const bool in_pairs = halves > 0 && items * 2 >= (int64_t)sm_count * 3 && p.rows / p.n >> a.span >= 2;
+  if (!in_pairs) items = items_of(std::min(4, halves), 1);
   CUtensorMap maps[3];
   const bf16* at[3] = {p.q, p.k, p.v};
   const int64_t ld[3] = {p.ldq, p.ldk, p.ldv};
-  const uint32_t box[3] = {64, kTile, (uint32_t)(D / 64)};
-  const bool is_long = p.rows / p.n >= 2048;
-  for (int i = is_long ? 0 : 1; i < 3; ++i) {
-    const uint64_t dims[3] = {64, (uint64_t)p.rows, (uint64_t)(i ? p.kv_heads : p.q_heads) * (D / 64)};
-    const uint64_t strides[2] = {(uint64_t)ld[i] * 2, 128};
-    if (tc_encode_bf16(&maps[i], at[i], 3, dims, strides, box) != 0) return cudaErrorInvalidValue;
+  for (int i = 0; i < 3; ++i) {
+    const uint64_t heads = i ? p.kv_heads : p.q_heads;
+    int rc;
+    if (i > 0) {
+      const uint64_t dims[3] = {64, (uint64_t)p.rows, heads * (D / 64)}, strides[2] = {(uint64_t)ld[i] * 2, 128};
+      const uint32_t box[3] = {64, kTile, (uint32_t)(D / 64)};
+      rc = tc_encode_bf16(&maps[i], at[i], 3, dims, strides, box);
+    } else {
+      const uint64_t dims[4] = {64, (uint64_t)p.rows, heads, (uint64_t)(D / 64)}, strides[3] = {(uint64_t)ld[i] * 2, (uint64_t)D * 2, 128};
+      const uint32_t box[4] = {64, 1u << a.span, (uint32_t)kTile >> a.span, 1};
+      rc = tc_encode_bf16(&maps[i], at[i], 4, dims, strides, box);
+    }
+    if (rc != 0) return cudaErrorInvalidValue;
   }
   const auto go = [&](auto d) {
     constexpr int kD = decltype(d)::value;
-    if (is_long) {
-      const cudaError_t e = allow_large<wide::long_kernel<kD>>(wide::kSmem<kD>);
-      if (e != cudaSuccess) return e;
-      wide::long_kernel<kD><<<(unsigned)a.slots * (a.q_heads >> a.apart), wide::kThreads, wide::kSmem<kD>, s>>>(maps[0], maps[1], maps[2], a, err);
+    cudaError_t e;
+    if (in_pairs) {
+      if ((e = allow_large<paired::paired_kernel<kD>>(paired::kSmem<kD>)) != cudaSuccess) return e;
+      paired::paired_kernel<kD><<<(unsigned)std::min<int64_t>(items, sm_count), paired::kThreads, paired::kSmem<kD>, s>>>(maps[0], maps[1], maps[2], a, err);
     } else {
-      const cudaError_t e = allow_large<narrow::short_kernel<kD>>(narrow::kSmem<kD>);
-      if (e != cudaSuccess) return e;
-      const uint64_t dims[4] = {64, (uint64_t)p.rows, (uint64_t)p.q_heads, (uint64_t)(kD / 64)};
-      const uint64_t strides[3] = {(uint64_t)p.ldq * 2, (uint64_t)kD * 2, 128};
-      const uint32_t tile[4] = {64, 1u << a.span, (uint32_t)kTile >> a.span, 1};
-      if (tc_encode_bf16(&maps[0], p.q, 4, dims, strides, tile) != 0) return cudaErrorInvalidValue;
-      const int64_t items = (((int64_t)p.rows >> a.span) + p.n) * (p.q_heads >> (7 - a.span));  // at most
-      const unsigned ctas = (unsigned)std::min<int64_t>(items, (int64_t)sm_count * narrow::kPerSm);
-      narrow::short_kernel<kD><<<ctas, narrow::kThreads, narrow::kSmem<kD>, s>>>(maps[0], maps[1], maps[2], a, err);
+      if ((e = allow_large<single::single_kernel<kD>>(single::kSmem<kD>)) != cudaSuccess) return e;
+      const unsigned ctas = (unsigned)std::min<int64_t>(items, (int64_t)sm_count * single::kPerSm);
+      single::single_kernel<kD><<<ctas, single::kThreads, single::kSmem<kD>, s>>>(maps[0], maps[1], maps[2], a, err);
     }
     return cudaGetLastError();
   };

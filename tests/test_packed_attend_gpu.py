@@ -201,6 +201,21 @@ def test_heads_that_share_a_tile(ops, hq, hk, d, lens):
     agree(run(ops, q, k, v, ptr, hq, hk, d, 0.1), *attend_of(q, k, v, ptr, hq, hk, d, 0.1), ptr)
 
 
+@pytest.mark.parametrize("hq,hk,d", [(64, 32, 128), (64, 16, 64), (96, 16, 64), (48, 2, 128), (64, 2, 64), (32, 2, 128)])
+@pytest.mark.parametrize("lens", [[300, 257, 513, 260], [700, 1000, 0, 333], [1, 2050, 3], [384] * 5])
+@pytest.mark.parametrize("odd", [False, True])
+def test_tiles_in_pairs(ops, hq, hk, d, lens, odd):
+    """As many heads as it takes for two tiles a block: sizes around its tiles, what is not finite, rows of nobody."""
+    q, k, v, ptr = case(hq, hk, d, lens, seed=hq + d, before=2, behind=9)
+    if odd:
+        for x in (q, k, v):
+            x[:2], x[int(ptr[-1]):] = float("nan"), float("inf")
+        last = int(ptr[2]) - 1  # of the second sequence
+        v[last, 3], v[last - 9, 5], v[last - 200 if lens[1] > 200 else last, 7], v[last - 1, 5] = float("nan"), -float("inf"), float("inf"), float("inf")
+        v[int(ptr[0]), d - 1] = float("nan")
+    agree(run(ops, q, k, v, ptr, hq, hk, d, 0.1), *attend_of(q, k, v, ptr, hq, hk, d, 0.1), ptr)
+
+
 def test_sequences_over_one_another_end(ops):
     """Many sequences of all the rows: more work than rows and sequences can make is not begun."""
     from pega_omni_b200.ops import OpsError
