@@ -278,8 +278,8 @@ int32_t omni_op_packed_attend(omni_ops* ctx, const void* q, int64_t ldq, const v
  * come behind tokens that the page holds, whose scale then only grows, and whose codes are rounded again when it does. Codes
  * are the nearest, ties to even; infinities become +-448 * 2^e, a NaN stays one. Rows of one page are neighbours in the call, in
  * ascending slots without a gap, as omni_op_kv_tables lays them: a row that is on the page of the row in front of it but not its
- * next token is left out and raises the device error word, and a page that occurs in two places further apart is written in an
- * undefined order. */
+ * next token is left out and raises the device error word (those behind it on that page may be left out too), and a page that
+ * occurs in two places further apart is written in an undefined order. */
 int32_t omni_op_kv8_append(omni_ops* ctx, const void* k, int64_t ldk, const void* v, int64_t ldv, const int32_t* slot,
                            int32_t rows, void* kv, float* scales, int32_t kv_pages, int32_t kv_heads, int32_t head_dim);
 

@@ -164,8 +164,8 @@ __global__ void __launch_bounds__(kTablesThreads) kv_tables_kernel(const TablesC
 // head, D / 16 neighbouring lanes a head, and a warp takes up to kRopeBatch such loads of one row at a time, all under way before
 // the first is used. The angle of a pair is the same for all heads of a row, so a warp makes each once, under its loads, and a
 // lane keeps its eight: in turns and in f64, since f32 would be off by 2^-24 of a far position's whole angle, and only what is left
-// of a turn goes to f32 and sincospi. All else is f32 with one rounding. 8,192 rows of 40 heads of 128: 32.1 us, 5.2 TB/s, where a
-// plain copy of them takes 27.6 us; angles and norms are 40 % of what the SMs can issue meanwhile. 64 rows of 24 heads: 2.3 us.
+// of a turn goes to f32 and sincospi. All else is f32 with one rounding. 8,192 rows of 40 heads of 128: 29.3 us, 5.7 TB/s, where a
+// plain copy of them takes 27.6 us; angles and norms are half of what the SMs can issue meanwhile. 64 rows of 24 heads: 2.3 us.
 
 struct Turns {
   double per_pos[64];
@@ -220,7 +220,9 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 14) qk_norm_rope_kernel(const
   if (my_pos < 0) return;
 #pragma unroll
   for (int p = lane; p < D / 2; p += 32) {
-    const double t = (double)my_pos * turns.per_pos[p];
+    double per_pos;  // through a generic address: as a constant, each lane's would be read by itself (32 us instead of 29 for the case above)
+    asm("ld.f64 %0, [%1];" : "=d"(per_pos) : "l"(&turns.per_pos[p]));
+    const double t = (double)my_pos * per_pos;
     float2 f;
     sincospif(2.f * (float)(t - rint(t)), &f.y, &f.x);
     rot[warp][(((p >> 1) & 3) * LANES + (p >> 3)) * 2 + (p & 1)] = f;  // the lanes' pairs side by side, so that no banks collide
@@ -267,11 +269,13 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 14) qk_norm_rope_kernel(const
 
 // ---- append ---------------------------------------------------------------------------------------------------------------
 // A run is what a call puts into one page: neighbouring rows in ascending slots. A warp takes the runs that begin in 16 rows (up to
-// 31 rows then: sixteen and what the last run has behind them), of K or V of one kv head, and holds their elements in
-// registers: rows of a prompt make one run of them, those of a decode step sixteen of one row, and no warp waits for another. Lane r
-// keeps what there is to know of row r: its slot, the row that begins its run, that run's largest magnitude and scale.
-// Bound by HBM where there are many rows (2 bytes in, 1 out an element), but a warp's page is a chain of load, maximum and store, and
-// registers hold two waves of them: 7,600 rows of 8 heads of 128 take 14.5 us, 3.2 TB/s. 61 rows of as many sequences: 4.2 us.
+// 31 rows then: sixteen and what the last run has behind them), of K or V of one kv head. A run by itself, as prompts make them, is
+// held in registers as sixteen rows from its first on; several are taken row by row, from memory again where they are more than
+// sixteen rows. No warp waits for another. Lane r keeps what there is to know of row r: its slot, the row that begins its run, that
+// run's largest magnitude and scale.
+// Bound by HBM where there are many rows (2 bytes in, 1 out an element), but a warp's page is a chain of slots, rows, maximum and store:
+// 7,600 rows of 8 heads of 128 take 13.7 us, 3.4 TB/s; the first sixteen rows are under way before the slots are known (14.1 otherwise), and
+// more warps at fewer registers make it no faster. 61 rows of as many sequences: 4.3 us.
 
 // The smallest 2^e >= 2^-100 with amax <= 448 * 2^e; amax finite, not negative. 448 = 1.75 * 2^8.
 __device__ __forceinline__ float page_scale(float amax) {
@@ -321,14 +325,13 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 12) kv8_append_kernel(const
   const int sub = lane / LANES, at = lane % LANES * 8;
   const bf16* const src = (w ? v : k) + head * D + at;
   const int64_t ld = w ? ldv : ldk;
-  // x[pass][i]: row base + 16 pass + i * TOGETHER + sub; the first sixteen are under way before the slots are known
-  uint4 x[2][STEPS];
-  const auto load = [&](int pass, int i) {
-    const int r = base + 16 * pass + i * TOGETHER + sub;
-    x[pass][i] = r < rows ? __ldg(reinterpret_cast<const uint4*>(src + r * ld)) : make_uint4(0, 0, 0, 0);
-  };
+  uint4 x[STEPS];  // rows base + from + i * TOGETHER + sub
+  const auto fetch = [&](int i, int r) { x[i] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)(base + r) * ld)); };
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i) load(0, i);
+  for (int i = 0; i < STEPS; ++i) {
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (base + i * TOGETHER + sub < rows) fetch(i, i * TOGETHER + sub);  // under way before the slots are known
+  }
   const int64_t limit = (int64_t)kv_pages * 16;
   const auto slot_of = [&](int r) {  // -2: none
     const int s = r >= 0 && r < rows ? slot[r] : -2;
@@ -345,68 +348,76 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 12) kv8_append_kernel(const
   }
   const uint32_t leaders = __ballot_sync(0xffffffffu, s >= 0 && ((s & 15) == 0 || before + 1 != s));
   const int l = 31 - __clz(leaders & (2u << lane) - 1u);  // that begins no later; -1 where the run begins in front of the window
-  const int run = s >= 0 && lane < 31 && l < 16 ? l : -1;
+  const int run = s >= 0 && l < 16 ? l : -1;
   const bool mine = run == lane;  // this lane's row begins a run of this warp
   float* const at_scale = scales + ((int64_t)(max(s, 0) >> 4) * hk + head) * 2 + w;
   const bool held = mine && (s & 15);  // the page holds tokens of this sequence
   const float old = held ? *at_scale : 0.f;
   const uint32_t ours = __ballot_sync(0xffffffffu, run >= 0);
-  const uint32_t its_ours = ours >> sub;  // bit 16 pass + i * TOGETHER: the row of x[pass][i] is this warp's
-  const int passes = ours >> 16 ? 2 : 1;
-  const auto is_ours = [&](int pass, int i) { return (its_ours >> (16 * pass + i * TOGETHER) & 1) != 0; };
-  if (passes == 2) {
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-      x[1][i] = make_uint4(0, 0, 0, 0);
-      if (is_ours(1, i)) load(1, i);
-    }
-  }
-  // the largest magnitudes: of the warp's one run as a prompt gives it, otherwise row by row and run by run
+  if (ours == 0) return;
   const uint32_t runs = leaders & 0xffffu;
-  const bool one = (runs & (runs - 1)) == 0;
+  // one run as a prompt gives it: sixteen rows from its first on, in slots that follow one another
+  const int first = __ffs(runs) - 1, from_first = __shfl_sync(0xffffffffu, s - lane, first);
+  const bool one = (runs & (runs - 1)) == 0 && __all_sync(0xffffffffu, run < 0 || s - lane == from_first);
+  const int lead = one ? first : 0;
+  const int passes = !one && ours >> 16 ? 2 : 1;
+  const auto is_ours = [&](int from, int i) { return (ours >> (from + i * TOGETHER + sub) & 1) != 0; };
+  const auto load = [&](int from) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+      if (is_ours(from, i)) fetch(i, from + i * TOGETHER + sub);
+  };
+  const auto finite_max = [&](int i) {
+    float f[8], most = 0.f;
+    unpack8v(x[i], f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = fabsf(f[e]) < kInf ? fmaxf(most, fabsf(f[e])) : most;
+    return most;
+  };
+  if (lead > 0) load(lead);
+  // the largest magnitudes: of the one run, otherwise row by row and run by run
   float m = 0.f;
-  __nv_bfloat162 m2 = __floats2bfloat162_rn(0.f, 0.f);
-#pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {
-    if (pass == passes) break;
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-      const __nv_bfloat162 its = is_ours(pass, i) ? abs_max(x[pass][i]) : __floats2bfloat162_rn(0.f, 0.f);
-      m2 = one ? __hmax2(m2, its) : its;
-      if (!one) {
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) m2 = __hmax2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
-        if (at == 0) row_max[warp][16 * pass + i * TOGETHER + sub] = fmaxf(__low2float(m2), __high2float(m2));
-      }
-    }
-  }
   if (one) {
+    __nv_bfloat162 m2 = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+      if (is_ours(lead, i)) m2 = __hmax2(m2, abs_max(x[i]));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m2 = __hmax2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
     m = fmaxf(__low2float(m2), __high2float(m2));
-  } else {
-    __syncwarp();
-    if (run >= 0) m = row_max[warp][lane];
-  }
-  if (__any_sync(0xffffffffu, m == kInf)) {  // infinities do not count: once more without
-    __syncwarp();
+    if (m == kInf) {  // infinities do not count: once more without
+      m = 0.f;
 #pragma unroll
-    for (int pass = 0; pass < 2; ++pass) {
-      if (pass == passes) break;
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        float f[8], its = 0.f;
-        unpack8v(x[pass][i], f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) its = fabsf(f[e]) < kInf ? fmaxf(its, fabsf(f[e])) : its;
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) its = fmaxf(its, __shfl_xor_sync(0xffffffffu, its, o));
-        if (at == 0) row_max[warp][16 * pass + i * TOGETHER + sub] = its;
-      }
+      for (int i = 0; i < STEPS; ++i)
+        if (is_ours(lead, i)) m = fmaxf(m, finite_max(i));
+      m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
     }
-    __syncwarp();
-    m = run >= 0 ? row_max[warp][lane] : 0.f;
-    if (one) m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+  } else {
+    for (int again = 0; again < 2; ++again) {
+#pragma unroll 1
+      for (int pass = 0; pass < passes; ++pass) {
+        if (passes == 2 && pass + again > 0) load(16 * pass);
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+          float its;
+          if (again) {
+            its = finite_max(i);
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) its = fmaxf(its, __shfl_xor_sync(0xffffffffu, its, o));
+          } else {
+            __nv_bfloat162 m2 = abs_max(x[i]);
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) m2 = __hmax2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
+            its = fmaxf(__low2float(m2), __high2float(m2));
+          }
+          if (at == 0) row_max[warp][16 * pass + i * TOGETHER + sub] = its;
+        }
+      }
+      __syncwarp();
+      m = run >= 0 ? row_max[warp][lane] : 0.f;
+      if (!__any_sync(0xffffffffu, m == kInf)) break;
+      __syncwarp();
+    }
   }
   const uint32_t my_max = __float_as_uint(fmaxf(m, 0.f));  // magnitudes order as their bits do; a row of NaN: 0
   uint32_t top = my_max;
@@ -420,27 +431,22 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 12) kv8_append_kernel(const
   if (mine) *at_scale = scale;
   const int64_t to = (((int64_t)(max(s, 0) >> 4) * hk + head) * 32 + w * 16 + (s & 15)) * D;  // of lane r's row
   if (one) {  // one row behind the other
-    const int lead = runs ? __ffs(runs) - 1 : 0;
     const float by = __shfl_sync(0xffffffffu, 1.f / scale, lead);
-    uint8_t* const dst = kv + (__shfl_sync(0xffffffffu, to, lead) + (sub - lead) * D + at);
+    uint8_t* const dst = kv + (__shfl_sync(0xffffffffu, to, lead) + sub * D + at);
 #pragma unroll
-    for (int pass = 0; pass < 2; ++pass) {
-      if (pass == passes) break;
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i)
-        if (is_ours(pass, i)) *reinterpret_cast<uint2*>(dst + (16 * pass + i * TOGETHER) * D) = e4m3_of8(x[pass][i], by);
-    }
+    for (int i = 0; i < STEPS; ++i)
+      if (is_ours(lead, i)) *reinterpret_cast<uint2*>(dst + i * TOGETHER * D) = e4m3_of8(x[i], by);
   } else {
     const float mul = __shfl_sync(0xffffffffu, 1.f / scale, max(run, 0));
-#pragma unroll
-    for (int pass = 0; pass < 2; ++pass) {
-      if (pass == passes) break;
+#pragma unroll 1
+    for (int pass = 0; pass < passes; ++pass) {
+      if (passes == 2) load(16 * pass);
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
         const int r = 16 * pass + i * TOGETHER + sub;
         const float by = __shfl_sync(0xffffffffu, mul, r);
         uint8_t* const dst = kv + (__shfl_sync(0xffffffffu, to, r) + at);
-        if (is_ours(pass, i)) *reinterpret_cast<uint2*>(dst) = e4m3_of8(x[pass][i], by);
+        if (is_ours(16 * pass, i)) *reinterpret_cast<uint2*>(dst) = e4m3_of8(x[i], by);
       }
     }
   }

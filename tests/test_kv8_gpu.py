@@ -384,12 +384,16 @@ def test_append_outside_the_cache_is_reported(ops, bad):
 
 
 @pytest.mark.parametrize("front", [0, 13, 15, 31])
-def test_append_leaves_out_rows_that_are_not_their_pages_next(ops, front):
+@pytest.mark.parametrize("given,out", [
+    ([0, 0, 1, 2, 20, 20, 20, 37, 36, 50, 53, 64, 65, 64], {1, 5, 6, 8, 10, 13}),
+    ([638, 638, 639], {1}), ([637, 639, 638], {1, 2}),  # at the end of the last page
+    ([0] + list(range(16)), {1}),
+])
+def test_append_leaves_out_rows_that_are_not_their_pages_next(ops, front, given, out):
     """The same slot twice, slots that descend or skip one, behind one another and where the kernel changes warps."""
     from pega_omni_b200.ops import OpsError
-    given = [16 * (i + 6) for i in range(front)] + [0, 0, 1, 2, 20, 20, 20, 37, 36, 50, 53, 64, 65, 64]
-    out = {front + i for i in (1, 5, 6, 8, 10, 13)}
-    kept = [i for i in range(len(given)) if i not in out]
+    given = [16 * (i + 6) for i in range(front)] + given
+    kept = [i for i in range(len(given)) if i - front not in out]
     rng = np.random.default_rng(front)
     kv, scales = cache(40, 2, 64, 2)
     k, v = bf16(rng.standard_normal((len(given), 128))), bf16(rng.standard_normal((len(given), 128)))
