@@ -121,7 +121,7 @@ struct Cut {
 constexpr int kCutRows = 1024;  // rows at most of a call in pieces
 
 __device__ __forceinline__ int pages_of_row(const Kv8Attend& a, int row) {
-  const int pos = a.pos[row];
+  const int pos = __ldcg(a.pos + row);
   return pos < 0 ? 0 : min((pos >> 4) + 1, a.n_pages);
 }
 
@@ -182,7 +182,8 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Part parts[kWarps][NT * 8], joined[NT * 8];
   __shared__ float factor[8][NT * 8];  // of the sums of warps, then of CTAs
-  grid_trigger();  // of the second kernel, if there is one
+  grid_wait();
+  grid_trigger();  // behind the wait: the second kernel, if there is one, looks at the rows' lengths before it waits itself
   const cg::cluster_group cluster = cg::this_cluster();
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = warp_index(), g = lane >> 2, t = lane & 3;
@@ -204,12 +205,12 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int j = 0; j < D / 32; ++j)
-      raw[nt][j] = __ldg(reinterpret_cast<const uint4*>(a.q + row * a.ldq + (int64_t)(head0 + min(nt * 8 + g, nq - 1)) * D + t * (D / 4)) + j);
+      raw[nt][j] = __ldcg(reinterpret_cast<const uint4*>(a.q + row * a.ldq + (int64_t)(head0 + min(nt * 8 + g, nq - 1)) * D + t * (D / 4)) + j);
 
   // the row's tokens and pages
-  const int s_of = a.seq ? a.seq[row] : row, pos = a.pos[row];
+  const int s_of = a.seq ? __ldcg(a.seq + row) : row, pos = __ldcg(a.pos + row);
   const bool named = s_of >= 0 && s_of < a.n_seqs;
-  const int first = named ? a.indptr[s_of] : 0, last = named ? a.indptr[s_of + 1] : 0;
+  const int first = named ? __ldcg(a.indptr + s_of) : 0, last = named ? __ldcg(a.indptr + s_of + 1) : 0;
   int len = pos < 0 || pos == 0x7fffffff ? 0 : pos + 1;
   if (pos >= 0 && !(named && len > 0 && first >= 0 && last <= a.n_pages && (int64_t)last - first >= ((int64_t)len + 15) / 16)) {
     if (tid == 0) raise(err, kErrBadIndex);
@@ -231,14 +232,14 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
   const auto fetch_id = [&](int b) {
     const int i = b * 32 + lane;
     if (i >= mine) return 0;
-    const int id = __ldg(my_pages + (int64_t)i * workers);
+    const int id = __ldcg(my_pages + (int64_t)i * workers);
     if (id >= 0 && id < a.kv_pages) return id;
     raise(err, kErrBadIndex);
     return -1;
   };
   const float2* const scales = reinterpret_cast<const float2*>(a.scales) + kh;
   int ids = fetch_id(0), ids_next = mine > 32 ? fetch_id(1) : 0;
-  float2 sc = __ldg(scales + (int64_t)max(ids, 0) * a.kv_heads), sc_next = sc;
+  float2 sc = __ldcg(scales + (int64_t)max(ids, 0) * a.kv_heads), sc_next = sc;
   if (ids < 0) sc.x = -1.f;  // no tokens on it
 
   const uint32_t ring = sm100::smem_addr(smem) + warp * (S * kPageBytes<D>);
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
     if (i < mine) {
       if ((i & 31) == 0 && i > 0) {
         ids = ids_next;
-        sc_next = __ldg(scales + (int64_t)max(ids, 0) * a.kv_heads);
+        sc_next = __ldcg(scales + (int64_t)max(ids, 0) * a.kv_heads);
         if (ids < 0) sc_next.x = -1.f;
         if (i + 32 < mine) ids_next = fetch_id(i / 32 + 1);
       }
@@ -493,6 +494,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4) kv8_join_kernel(const __gr
   const int groups = a.kv_heads * cut.subgroups, part = kh * cut.subgroups + head % group / cut.per;
   const Piece piece = find_piece<kJoinWarps>(a, cut, row, true);
   grid_wait();  // on every path: with this kernel the one in front has ended
+  grid_trigger();
   if (piece.count < 2) return;
   const int64_t step = (int64_t)groups * cut.per, at = (piece.before * (int64_t)groups + part) * cut.per + n;
   const float4* const parts = reinterpret_cast<const float4*>(cut.parts) + at;
@@ -559,10 +561,12 @@ cudaError_t go(const Kv8Attend& a, Cut cut, int ctas, int sm_count, cudaMemPool_
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(units * ctas), cfg.blockDim = dim3(kWarps * 32), cfg.dynamicSmemBytes = smem, cfg.stream = s;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = ctas, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr, cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr, cfg.numAttrs = cut.room ? 1 : 2;  // with pieces there is an allocation in front, not a kernel
   e = cudaLaunchKernelEx(&cfg, kv8_attend_kernel<D, NT>, a, cut, err);
   if (cut.room) {
     if (e == cudaSuccess) e = launch_pdl(kv8_join_kernel<D>, dim3((unsigned)a.rows * a.q_heads), dim3(kJoinWarps * 32), 0, s, a, cut);

@@ -7,6 +7,7 @@
 
 #include "f32x2.cuh"
 #include "kv8.h"
+#include "pdl.cuh"
 
 namespace omni {
 namespace {
@@ -55,7 +56,9 @@ __global__ void __launch_bounds__(kTablesThreads) kv_tables_kernel(const TablesC
   int* const need = rows + n + 1;       // [n + 1] pages to be taken
   int* const back = need + n + 1;       // [n + 1] pages given back
   int* const held = back + n + 1;       // [n] tokens held
-  const int count = *c.free_count;
+  grid_wait();
+  grid_trigger();
+  const int count = __ldcg(c.free_count);
 
   const int per = (n + block - 1) / block, begin = min(n, tid * per), end = min(n, begin + per);
   bool bad = false;
@@ -83,7 +86,7 @@ __global__ void __launch_bounds__(kTablesThreads) kv_tables_kernel(const TablesC
     for (int s = begin; s < end; ++s) {
       int len, add;
       if (pass == 0) {
-        len = c.lens[s], add = c.add[s];
+        len = __ldcg(c.lens + s), add = __ldcg(c.add + s);
         const bool wrong = len < 0 || add < -1 || (int64_t)len + max(add, 0) > (int64_t)c.width * kPageTokens;
         bad |= wrong;
         if (wrong) len = 0, add = 0;
@@ -116,11 +119,11 @@ __global__ void __launch_bounds__(kTablesThreads) kv_tables_kernel(const TablesC
 
   const auto returned = [&](int k) {  // the k-th page given back
     const int s = owner_of(back, n, k);
-    return c.table[(int64_t)s * c.width + (k - back[s])];
+    return __ldcg(c.table + (int64_t)s * c.width + (k - back[s]));
   };
   const auto taken = [&](int j) {  // the j-th page from the top of the stack
     const int i = count + back_n - 1 - j;
-    return i >= count ? returned(i - count) : c.free_pages[i];
+    return i >= count ? returned(i - count) : __ldcg(c.free_pages + i);
   };
   // a warp takes kChunk pages and rows of a sequence at a time, so a long one among many is shared
   const int chunks = ok ? (c.width + kChunk - 1) / kChunk : 0;
@@ -129,7 +132,7 @@ __global__ void __launch_bounds__(kTablesThreads) kv_tables_kernel(const TablesC
     const int32_t* const mine = c.table + (int64_t)s * c.width;
     const int p0 = chunk * kChunk, p1 = min(total, p0 + kChunk), own = min(had, p1);
 #pragma unroll 4
-    for (int p = p0 + lane; p < own; p += 32) c.pages[want[s] + p] = mine[p];
+    for (int p = p0 + lane; p < own; p += 32) c.pages[want[s] + p] = __ldcg(mine + p);
     for (int p = max(p0, had) + lane; p < p1; p += 32) {
       const int page = taken(need[s] + p - had);
       c.pages[want[s] + p] = page, c.table[(int64_t)s * c.width + p] = page;
@@ -150,8 +153,8 @@ __global__ void __launch_bounds__(kTablesThreads) kv_tables_kernel(const TablesC
   for (int s = first; s <= n; s += threads) c.indptr[s] = ok ? want[s] : 0, c.row_ptr[s] = ok ? rows[s] : 0;
   cluster.barrier_wait(std::move(all_read));
   for (int s = first; s < n; s += threads) {
-    const int len = c.lens[s];  // this thread alone writes it
-    c.lens_out[s] = !ok ? len : c.add[s] < 0 ? 0 : len + (rows[s + 1] - rows[s]);
+    const int len = __ldcg(c.lens + s);  // this thread alone writes it
+    c.lens_out[s] = !ok ? len : __ldcg(c.add + s) < 0 ? 0 : len + (rows[s + 1] - rows[s]);
   }
   if (first == 0) {
     *c.free_count_out = ok ? count + back_n - need_n : count;
@@ -191,12 +194,14 @@ __device__ __forceinline__ uint4 packed_of(const float2 (&v)[4]) {
 
 // Block y of a row's y_blocks: heads of q where y < q_blocks, otherwise of k.
 template <int D>
-__global__ void __launch_bounds__(kRopeWarps * 32, 14) qk_norm_rope_kernel(const bf16* x, int64_t ldx, const bf16* __restrict__ q_norm,
-                                                                       const bf16* __restrict__ k_norm, const int32_t* __restrict__ pos,
+__global__ void __launch_bounds__(kRopeWarps * 32, 14) qk_norm_rope_kernel(const bf16* x, int64_t ldx, const bf16* q_norm,
+                                                                       const bf16* k_norm, const int32_t* pos,
                                                                        int rows, int hq, int heads, int q_blocks, int y_blocks, float eps,
                                                                        const __grid_constant__ Turns turns, bf16* out, int64_t ldo) {
   constexpr int LANES = D / 16, HEADS = 32 / LANES;  // lanes of a head, heads of a warp's access
   __shared__ __align__(16) float2 rot[kRopeWarps][D / 2];
+  grid_wait();
+  grid_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = (int64_t)(blockIdx.x / y_blocks) * kRopeWarps + warp;
   const int y = blockIdx.x % y_blocks;
@@ -204,19 +209,19 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 14) qk_norm_rope_kernel(const
   const bool is_q = y < q_blocks;
   const int end = is_q ? hq : heads, at = lane % LANES * 8;
   const int head0 = (is_q ? y : y - q_blocks) * (HEADS * kRopeBatch) + (is_q ? 0 : hq) + lane / LANES;
-  const int my_pos = pos[row];
+  const int my_pos = __ldcg(pos + row);
   const bf16* const src = x + row * ldx + head0 * D + at;
   uint4 lo_raw[kRopeBatch], hi_raw[kRopeBatch];
 #pragma unroll
   for (int b = 0; b < kRopeBatch; ++b) {
     lo_raw[b] = hi_raw[b] = make_uint4(0, 0, 0, 0);
     if (head0 + b * HEADS < end) {
-      lo_raw[b] = *reinterpret_cast<const uint4*>(src + b * HEADS * D), hi_raw[b] = *reinterpret_cast<const uint4*>(src + b * HEADS * D + D / 2);
+      lo_raw[b] = __ldcg(reinterpret_cast<const uint4*>(src + b * HEADS * D)), hi_raw[b] = __ldcg(reinterpret_cast<const uint4*>(src + b * HEADS * D + D / 2));
     }
   }
   const bf16* const gain = is_q ? q_norm : k_norm;
   uint4 lo_gain = {}, hi_gain = {};
-  if (gain) lo_gain = __ldg(reinterpret_cast<const uint4*>(gain + at)), hi_gain = __ldg(reinterpret_cast<const uint4*>(gain + D / 2 + at));
+  if (gain) lo_gain = __ldcg(reinterpret_cast<const uint4*>(gain + at)), hi_gain = __ldcg(reinterpret_cast<const uint4*>(gain + D / 2 + at));
   if (my_pos < 0) return;
 #pragma unroll
   for (int p = lane; p < D / 2; p += 32) {
@@ -312,12 +317,14 @@ __device__ __forceinline__ __nv_bfloat162 abs_max(const uint4& u) {
 constexpr int kAppendWarps = 2;
 
 template <int D>
-__global__ void __launch_bounds__(kAppendWarps * 32, 12) kv8_append_kernel(const bf16* __restrict__ k, int64_t ldk, const bf16* __restrict__ v,
-                                                                       int64_t ldv, const int32_t* __restrict__ slot, int rows, uint8_t* kv,
+__global__ void __launch_bounds__(kAppendWarps * 32, 12) kv8_append_kernel(const bf16* k, int64_t ldk, const bf16* v,
+                                                                       int64_t ldv, const int32_t* slot, int rows, uint8_t* kv,
                                                                        float* scales, int kv_pages, int hk, int head_blocks, uint32_t* err) {
   constexpr int LANES = D / 8, TOGETHER = 32 / LANES, STEPS = 16 / TOGETHER;  // lanes of a row, rows of an access, accesses of 16 rows
   constexpr float kInf = __builtin_huge_valf();
   __shared__ float row_max[kAppendWarps][32];
+  grid_wait();
+  grid_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // blocks of the same rows follow one another: neighbouring heads are neighbours in DRAM
   const int base = blockIdx.x / head_blocks * 16, what = blockIdx.x % head_blocks * kAppendWarps + warp, head = what >> 1, w = what & 1;
@@ -326,7 +333,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 12) kv8_append_kernel(const
   const bf16* const src = (w ? v : k) + head * D + at;
   const int64_t ld = w ? ldv : ldk;
   uint4 x[STEPS];  // rows base + from + i * TOGETHER + sub
-  const auto fetch = [&](int i, int r) { x[i] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)(base + r) * ld)); };
+  const auto fetch = [&](int i, int r) { x[i] = __ldcg(reinterpret_cast<const uint4*>(src + (int64_t)(base + r) * ld)); };
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
     x[i] = make_uint4(0, 0, 0, 0);
@@ -334,7 +341,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 12) kv8_append_kernel(const
   }
   const int64_t limit = (int64_t)kv_pages * 16;
   const auto slot_of = [&](int r) {  // -2: none
-    const int s = r >= 0 && r < rows ? slot[r] : -2;
+    const int s = r >= 0 && r < rows ? __ldcg(slot + r) : -2;
     if (s >= limit) raise(err, kErrBadIndex);
     return s < 0 || s >= limit ? -2 : s;
   };
@@ -352,7 +359,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 12) kv8_append_kernel(const
   const bool mine = run == lane;  // this lane's row begins a run of this warp
   float* const at_scale = scales + ((int64_t)(max(s, 0) >> 4) * hk + head) * 2 + w;
   const bool held = mine && (s & 15);  // the page holds tokens of this sequence
-  const float old = held ? *at_scale : 0.f;
+  const float old = held ? __ldcg(at_scale) : 0.f;
   const uint32_t ours = __ballot_sync(0xffffffffu, run >= 0);
   if (ours == 0) return;
   const uint32_t runs = leaders & 0xffffu;
@@ -455,7 +462,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 12) kv8_append_kernel(const
     const float by = __shfl_sync(0xffffffffu, ratio, r);
     for (int t = sub; t < (its_slot & 15); t += TOGETHER) {
       uint2* const word = reinterpret_cast<uint2*>(kv + (((int64_t)(its_slot >> 4) * hk + head) * 32 + w * 16 + t) * D + at);
-      const uint2 u = *word;
+      const uint2 u = __ldcg(word);
       const float4 a = static_cast<float4>(*reinterpret_cast<const __nv_fp8x4_e4m3*>(&u.x));
       const float4 b = static_cast<float4>(*reinterpret_cast<const __nv_fp8x4_e4m3*>(&u.y));
       const float codes[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
@@ -480,10 +487,12 @@ cudaError_t launch_kv_tables(const TablesCall& c, cudaStream_t s) {
   const unsigned block = in_place && warps > 16 * 16 ? kTablesThreads : kTablesThreads / 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(block), cfg.dynamicSmemBytes = smem, cfg.stream = s;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = in_place ? ctas : 1, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr, cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = in_place ? ctas : 1, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr, cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kv_tables_kernel, c);
 }
 
@@ -501,8 +510,8 @@ cudaError_t launch_qk_norm_rope(const bf16* x, int64_t ldx, const bf16* q_norm, 
   const int q_blocks = (q_heads + per_warp - 1) / per_warp, k_blocks = (kv_heads + per_warp - 1) / per_warp;
   const unsigned grid = (unsigned)((rows + kRopeWarps - 1) / kRopeWarps) * (q_blocks + k_blocks);
   const auto go = [&](auto kernel) {
-    kernel<<<grid, kRopeWarps * 32, 0, s>>>(x, ldx, q_norm, k_norm, pos, rows, q_heads, q_heads + kv_heads, q_blocks, q_blocks + k_blocks, eps, turns, out, ldo);
-    return cudaGetLastError();
+    return launch_pdl(kernel, dim3(grid), dim3(kRopeWarps * 32), 0, s, x, ldx, q_norm, k_norm, pos, rows, q_heads, q_heads + kv_heads, q_blocks,
+                      q_blocks + k_blocks, eps, turns, out, ldo);
   };
   if (head_dim == 128) return go(qk_norm_rope_kernel<128>);
   if (head_dim == 64) return go(qk_norm_rope_kernel<64>);
@@ -514,8 +523,7 @@ cudaError_t launch_kv8_append(const bf16* k, int64_t ldk, const bf16* v, int64_t
   const int head_blocks = (2 * kv_heads + kAppendWarps - 1) / kAppendWarps;
   const unsigned grid = (unsigned)((rows + 15) / 16) * head_blocks;
   const auto go = [&](auto kernel) {
-    kernel<<<grid, kAppendWarps * 32, 0, s>>>(k, ldk, v, ldv, slot, rows, kv, scales, kv_pages, kv_heads, head_blocks, err);
-    return cudaGetLastError();
+    return launch_pdl(kernel, dim3(grid), dim3(kAppendWarps * 32), 0, s, k, ldk, v, ldv, slot, rows, kv, scales, kv_pages, kv_heads, head_blocks, err);
   };
   if (head_dim == 128) return go(kv8_append_kernel<128>);
   if (head_dim == 64) return go(kv8_append_kernel<64>);

@@ -32,6 +32,7 @@
 #include "f32x2.cuh"
 #include "gemm.h"
 #include "kv8.h"
+#include "pdl.cuh"
 #include "sm100.cuh"
 
 namespace omni {
@@ -314,7 +315,7 @@ struct Order {
 
   __device__ __forceinline__ int rows(int i) const {  // of sequence i
     if (i >= a.n) return 0;
-    const int from = a.indptr[i], to = a.indptr[i + 1];
+    const int from = __ldcg(a.indptr + i), to = __ldcg(a.indptr + i + 1);
     return from < 0 || to > a.rows || from > to ? 0 : to - from;
   }
   __device__ __forceinline__ static int blocks(int rows) { return (rows + kTile - 1) / kTile; }
@@ -338,7 +339,7 @@ struct Order {
     constexpr int kMany = 1 << 25;  // more than there can be
     int most = 0, sum = 0;
     for (int i = lane; i < a.n; i += 32) {
-      const int from = a.indptr[i], to = a.indptr[i + 1], its = blocks(rows(i));
+      const int from = __ldcg(a.indptr + i), to = __ldcg(a.indptr + i + 1), its = blocks(rows(i));
       if ((from < 0 || to > a.rows || from > to) && blockIdx.x == 0) raise(err, kErrBadIndex);
       most = max(most, its), sum = min(sum + its, kMany);
     }
@@ -367,8 +368,8 @@ struct Order {
       }
       const uint32_t has = __ballot_sync(0xffffffffu, from_k + incl > k);
       if (has) {
-        const int l = __ffs(has) - 1, i = from_i + l, tile = k - from_k - __shfl_sync(0xffffffffu, incl - its, l), from = a.indptr[i];
-        return Item{from, a.indptr[i + 1] - from, level * kTile + (tile << a.span), unit << a.share};
+        const int l = __ffs(has) - 1, i = from_i + l, tile = k - from_k - __shfl_sync(0xffffffffu, incl - its, l), from = __ldcg(a.indptr + i);
+        return Item{from, __ldcg(a.indptr + i + 1) - from, level * kTile + (tile << a.span), unit << a.share};
       }
       from_k += __shfl_sync(0xffffffffu, incl, 31);
     }
@@ -414,7 +415,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
   const auto bar = [](uint64_t& b) { return smem_addr(&b); };
   const auto wait = [&](uint64_t& b, int phase) { return mbar_wait(smem_addr(&b), phase & 1, err); };
 
-  if (warp == kMmaWarp) tmem_alloc(smem_addr(&tmem_slot), kColumns);
+  if (warp == kMmaWarp) {
+    grid_wait();  // columns only then: the kernel in front may want them for CTAs that have not begun
+    tmem_alloc(smem_addr(&tmem_slot), kColumns);
+  }
   if (tid == kItemWarp * 32) {
     prefetch_tensormap(&qmap), prefetch_tensormap(&kmap), prefetch_tensormap(&vmap);
     for (int i = 0; i < 2; ++i) mbar_init(bar(bars.item_full[i]), 1), mbar_init(bar(bars.item_empty[i]), 7), mbar_init(bar(bars.p_full[i]), 4);
@@ -437,12 +441,14 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
   Order order{a, lane};
   Item it{0, 0, 0, -1};  // of the item warp
   if (warp == kItemWarp) {
+    grid_wait();
     order.begin(err);
     it = order.item(blockIdx.x);
     if (lane == 0) {
       items[0] = it;
       mbar_arrive(bar(bars.item_full[0]));
       if (it.head >= 0) {
+        fence_async_global();
         fetch_q(it);
         fetch(&kmap, k_at, bars.k_full, it.first, it.head / group, kEvictLast);
         fetch(&vmap, v_at, it.row0 < kTile ? bars.last_full : bars.v_full, it.first, it.head / group, kEvictLast);
@@ -456,6 +462,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
+  grid_trigger();
 
   const auto item_there = [&](int n) { return wait(bars.item_full[n & 1], n >> 1) && items[n & 1].head >= 0; };
   const auto leave_item = [&](int n) { mbar_arrive(bar(bars.item_empty[n & 1])); };
@@ -633,7 +640,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const auto bar = [](uint64_t& b) { return smem_addr(&b); };
   const auto wait = [&](uint64_t& b, int phase) { return mbar_wait(smem_addr(&b), phase & 1, err); };
 
-  if (warp == kMmaWarp) tmem_alloc(smem_addr(&tmem_slot), kColumns);
+  if (warp == kMmaWarp) {
+    grid_wait();  // columns only then: the kernel in front may want them for CTAs that have not begun
+    tmem_alloc(smem_addr(&tmem_slot), kColumns);
+  }
   if (tid == kItemWarp * 32) {
     prefetch_tensormap(&qmap), prefetch_tensormap(&kmap), prefetch_tensormap(&vmap);
     for (int i = 0; i < 2; ++i) {
@@ -664,12 +674,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   Order order{a, lane};
   Item it{0, 0, 0, -1};  // of the item warp
   if (warp == kItemWarp) {
+    grid_wait();
     order.begin(err);
     it = order.item(blockIdx.x);
     if (lane == 0) {
       items[0] = it;
       mbar_arrive(bar(bars.item_full[0]));
       if (it.head >= 0) {
+        fence_async_global();
         fetch(&kmap, k_at, bars.k_full[0], it, 0);
         fetch_q(it);
         fetch(&vmap, v_at, it.row0 < kTile ? bars.last_full[0] : bars.v_full[0], it, 0);
@@ -683,6 +695,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
+  grid_trigger();
 
   const auto item_there = [&](int n) { return wait(bars.item_full[n & 1], n >> 1) && items[n & 1].head >= 0; };
   const auto leave_item = [&](int n) { mbar_arrive(bar(bars.item_empty[n & 1])); };
@@ -897,13 +910,13 @@ cudaError_t launch_packed_attend(const PackedAttend& p, int sm_count, uint32_t* 
     cudaError_t e;
     if (in_pairs) {
       if ((e = allow_large<paired::paired_kernel<kD>>(paired::kSmem<kD>)) != cudaSuccess) return e;
-      paired::paired_kernel<kD><<<(unsigned)std::min<int64_t>(items, sm_count), paired::kThreads, paired::kSmem<kD>, s>>>(maps[0], maps[1], maps[2], a, err);
+      return launch_pdl(paired::paired_kernel<kD>, dim3((unsigned)std::min<int64_t>(items, sm_count)), dim3(paired::kThreads), paired::kSmem<kD>, s,
+                        maps[0], maps[1], maps[2], a, err);
     } else {
       if ((e = allow_large<single::single_kernel<kD>>(single::kSmem<kD>)) != cudaSuccess) return e;
       const unsigned ctas = (unsigned)std::min<int64_t>(items, (int64_t)sm_count * single::kPerSm);
-      single::single_kernel<kD><<<ctas, single::kThreads, single::kSmem<kD>, s>>>(maps[0], maps[1], maps[2], a, err);
+      return launch_pdl(single::single_kernel<kD>, dim3(ctas), dim3(single::kThreads), single::kSmem<kD>, s, maps[0], maps[1], maps[2], a, err);
     }
-    return cudaGetLastError();
   };
   return D == 128 ? go(std::integral_constant<int, 128>()) : go(std::integral_constant<int, 64>());
 }

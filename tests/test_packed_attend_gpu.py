@@ -262,6 +262,46 @@ def plain_rope(x, gain, pos, d, theta):
     return torch.cat([lo * a.cos() - hi * a.sin(), hi * a.cos() + lo * a.sin()], -1)
 
 
+@pytest.mark.parametrize("hq,hk,d,n", [(16, 8, 128, 24), (10, 2, 64, 3), (16, 1, 128, 70)])
+def test_calls_behind_one_another(ops, hq, hk, d, n):
+    """Steps in which every call takes what the one in front has written give the same with and without a wait between the calls."""
+    rng = np.random.default_rng(n)
+    steps, width, prompt = 12, 40, 60
+    adds = [i32(rng.integers(1, prompt, n))] + [i32(rng.choice([-1, 0, 1, 1, 1], n) if k % 4 == 3 else np.ones(n)) for k in range(1, steps)]
+    rows = [prompt * n] + [n] * (steps - 1)
+    xs = [bf16(rng.standard_normal((r, (hq + 2 * hk) * d))) for r in rows]
+    gain = bf16(1 + 0.1 * rng.standard_normal(d))
+
+    def go(wait):
+        outs = []
+        done = torch.cuda.synchronize if wait else lambda: None
+        lens, count, free, table = i32([0] * n), i32([n * width]), i32(np.arange(n * width)), i32(np.zeros((n, width)))
+        kv, scales = torch.zeros((n * width, hk, 2, 16, d), dtype=torch.uint8, device="cuda"), torch.ones((n * width, hk, 2), device="cuda")
+        indptr, row_ptr, pages, status = i32([0] * (n + 1)), i32([0] * (n + 1)), i32([0] * (n * width)), i32([0])
+        pos, slot, seq = (i32([0] * max(rows)) for _ in range(3))
+        states = [x.clone() for x in xs]
+        torch.cuda.synchronize()
+        for k, r in enumerate(rows):
+            x, out = states[k], torch.full((r, hq * d), 2.0, dtype=torch.bfloat16, device="cuda")
+            at = pos[:r], slot[:r], seq[:r]
+            ops.kv_tables(lens, adds[k], table, free, count, lens, count, indptr, pages, row_ptr, *at, status), done()
+            ops.qk_norm_rope(x, gain, gain, at[0], hq, hk, d, 1e-6, 1e6, x), done()
+            q, key, v = x[:, :hq * d], x[:, hq * d:(hq + hk) * d], x[:, (hq + hk) * d:]
+            ops.kv8_append(key, v, at[1], kv, scales), done()
+            if k == 0:
+                ops.packed_attend(q, key, v, row_ptr, hq, hk, d, 0.1, out), done()
+            else:
+                ops.kv8_attend(q, kv, scales, at[0], indptr, pages, hq, 0.1, out, at[2]), done()
+            outs += [x, out]
+        ops.sync()
+        return outs + [lens, count, table, kv, scales, status]
+
+    want = go(True)
+    for _ in range(6):
+        for a, b in zip(go(False), want):
+            assert torch.equal(a.view(torch.int16) if a.dtype is torch.bfloat16 else a, b.view(torch.int16) if b.dtype is torch.bfloat16 else b)
+
+
 @pytest.mark.parametrize("hq,hk,d", [(16, 8, 128), (10, 2, 64)])
 def test_a_server_runs_them_together(ops, hq, hk, d):
     """Prompts come, sequences step and end, others take their pages; the steps are one captured graph. Every row's attention is that
