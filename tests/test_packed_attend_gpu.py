@@ -252,6 +252,35 @@ def test_the_same_every_time_and_from_a_graph(ops, lens):
         assert torch.equal(out, want)
 
 
+def test_side_by_side(ops):
+    """Calls of both kernels and both head sizes on streams of their own, all under way at once."""
+    cases = [(16, 8, 128, [5000]), (16, 8, 128, [300, 77, 512]), (64, 32, 64, [700, 300]), (4, 4, 64, [64] * 50), (5, 1, 128, [2000, 9])]
+    graphs, streams, outs, want, held = [], [], [], [], []
+    for n, (hq, hk, d, lens) in enumerate(cases):
+        q, k, v, ptr = case(hq, hk, d, lens, seed=n)
+        want.append(run(ops, q, k, v, ptr, hq, hk, d, 0.1).clone())
+        held.append((q, k, v, i32(ptr)))
+        outs.append(torch.zeros_like(want[-1], memory_format=torch.contiguous_format))
+        streams.append(torch.cuda.Stream())
+        graphs.append(torch.cuda.CUDAGraph())
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graphs[-1], stream=streams[-1]):
+            ops.stream(streams[-1].cuda_stream)
+            for _ in range(3):
+                ops.packed_attend(*held[-1], hq, hk, d, 0.1, outs[-1])
+        ops.stream(0)
+    for _ in range(10):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    ops.sync()
+
+
 # ---- together ---------------------------------------------------------------------------------------------------------------
 
 def plain_rope(x, gain, pos, d, theta):
