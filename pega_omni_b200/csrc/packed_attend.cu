@@ -312,11 +312,13 @@ struct Order {
   int until = 0;                // no sequence ends between this level and the one last counted
   int base = 0;                 // items in front of them
   int from_i = 0, from_k = 0;   // sequences that need not be looked at again, and their tiles
+  int from = 0, to = 0;         // rows of this lane's sequence of the first thirty-two, which are all that most calls have
 
-  __device__ __forceinline__ int rows(int i) const {  // of sequence i
-    if (i >= a.n) return 0;
-    const int from = __ldcg(a.indptr + i), to = __ldcg(a.indptr + i + 1);
-    return from < 0 || to > a.rows || from > to ? 0 : to - from;
+  __device__ __forceinline__ int rows(int i0) const {  // of sequence i0 + lane
+    const int i = i0 + lane;
+    int x = from, y = to;
+    if (i0 > 0 && i < a.n) x = __ldcg(a.indptr + i), y = __ldcg(a.indptr + i + 1);
+    return i >= a.n || x < 0 || y > a.rows || x > y ? 0 : y - x;
   }
   __device__ __forceinline__ static int blocks(int rows) { return (rows + kTile - 1) / kTile; }
   __device__ __forceinline__ int tiles(int rows) const {  // of this level, of a sequence with so many rows
@@ -327,7 +329,7 @@ struct Order {
     int sum = 0, next = 0;  // next: blocks of the longest sequence that has no such item
     longer = 0;
     for (int i0 = 0; i0 < a.n; i0 += 32) {
-      const int its = rows(i0 + lane);
+      const int its = rows(i0);
       sum += tiles(its);
       longer += __popc(__ballot_sync(0xffffffffu, blocks(its) > level));
       if (blocks(its) <= level) next = max(next, blocks(its));
@@ -337,12 +339,18 @@ struct Order {
   }
   __device__ __forceinline__ void begin(uint32_t* err) {
     constexpr int kMany = 1 << 25;  // more than there can be
+    if (lane < a.n) from = __ldcg(a.indptr + lane), to = __ldcg(a.indptr + lane + 1);
     int most = 0, sum = 0;
-    for (int i = lane; i < a.n; i += 32) {
-      const int from = __ldcg(a.indptr + i), to = __ldcg(a.indptr + i + 1), its = blocks(rows(i));
-      if ((from < 0 || to > a.rows || from > to) && blockIdx.x == 0) raise(err, kErrBadIndex);
+    for (int i0 = 0; i0 < a.n; i0 += 32) {
+      int x = from, y = to;
+      if (i0 > 0 && i0 + lane < a.n) x = __ldcg(a.indptr + i0 + lane), y = __ldcg(a.indptr + i0 + lane + 1);
+      if (i0 + lane >= a.n) break;
+      const bool wrong = x < 0 || y > a.rows || x > y;
+      if (wrong && blockIdx.x == 0) raise(err, kErrBadIndex);
+      const int its = wrong ? 0 : blocks(y - x);
       most = max(most, its), sum = min(sum + its, kMany);
     }
+    __syncwarp();
     level = (int)__reduce_max_sync(0xffffffffu, (unsigned)most) - 1;
     // sequences that overlap, between which an end lies in front of a beginning: an error by now, and no end of work
     if ((int)__reduce_add_sync(0xffffffffu, (unsigned)sum) > a.rows / kTile + a.n) level = -1;
@@ -359,7 +367,7 @@ struct Order {
     }
     const int k = (t - base) / units, unit = t - base - k * units;
     for (; level >= 0 && from_i < a.n; from_i += 32) {  // the sequence that has the k-th tile
-      const int its = tiles(rows(from_i + lane));
+      const int its = tiles(rows(from_i));
       int incl = its;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -368,8 +376,10 @@ struct Order {
       }
       const uint32_t has = __ballot_sync(0xffffffffu, from_k + incl > k);
       if (has) {
-        const int l = __ffs(has) - 1, i = from_i + l, tile = k - from_k - __shfl_sync(0xffffffffu, incl - its, l), from = __ldcg(a.indptr + i);
-        return Item{from, __ldcg(a.indptr + i + 1) - from, level * kTile + (tile << a.span), unit << a.share};
+        const int l = __ffs(has) - 1, tile = k - from_k - __shfl_sync(0xffffffffu, incl - its, l);
+        int x = __shfl_sync(0xffffffffu, from, l), y = __shfl_sync(0xffffffffu, to, l);
+        if (from_i > 0) x = __ldcg(a.indptr + from_i + l), y = __ldcg(a.indptr + from_i + l + 1);
+        return Item{x, y - x, level * kTile + (tile << a.span), unit << a.share};
       }
       from_k += __shfl_sync(0xffffffffu, incl, 31);
     }
