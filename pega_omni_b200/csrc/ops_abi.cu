@@ -37,8 +37,9 @@ struct omni_ops {
 };
 
 // Nothing of the next launch starts before everything in front of it in the stream has ended. Attention kernels ask for their
-// pages, GEMMs for their weights and biases before they wait for the kernel in front of them, because no other kernel of a
-// model's call writes those; calls made one by one here may.
+// positions, slots and pages, GEMMs for their weights and biases, draws for their counts and forced tokens before they wait for the
+// kernel in front of them, because no other kernel of a model's call writes those; calls made one by one here may, and the kernel in
+// front lets the next one start as it begins itself.
 __global__ void order_kernel() {}
 static cudaError_t order(cudaStream_t s) {
   order_kernel<<<1, 1, 0, s>>>();
@@ -227,6 +228,7 @@ int32_t omni_op_rope_attend(omni_ops* c, void* qkv, const void* q_norm, const vo
   map.indptr = indptr;
   map.pages = pages;
   const AttnShape a{q_heads, kv_heads, head_dim, eps, theta};
+  OPS_CUDA(c, order(c->stream));  // positions, slots and sequences are read early, and a call in front may have made them
   const size_t head = (size_t)rows * head_dim * sizeof(bf16);
   OPS_CUDA(c, on_aligned_rows(qkv, head * (q_heads + 2 * kv_heads), out, head * q_heads, c->stream, [&](void* x, void* y) {
     const cudaError_t e = launch_rope_kv((bf16*)x, (const bf16*)q_norm, (const bf16*)k_norm, (bf16*)kv, map, rows, a, kv_pages,
@@ -346,6 +348,7 @@ int32_t omni_op_sample(omni_ops* c, const void* logits, int32_t vocab, float tem
   p.seen_words = (vocab + 31) / 32;
   if (top_p < 1.f && (top_k <= 0 || top_k > 1024))
     return c->fail(OMNI_ERR_UNSUPPORTED, "top_p < 1 needs 0 < top_k <= 1024 (the nucleus filter ranks the survivors of the top-k cut)");
+  OPS_CUDA(c, order(c->stream));  // what is not drawn from - counts, uniforms, forced tokens - is read early
   OPS_CUDA(c, launch_sample((const bf16*)logits, p, frames, uniforms, force, SlotState{state, lines, stride}, codes,
                             rows, c->stream));
   return OMNI_OK;
@@ -419,6 +422,7 @@ int32_t omni_op_lm_dep_kv_attend(omni_ops* c, const void* qkv, void* ws, int32_t
 int32_t omni_op_lm_sample(omni_ops* c, const void* logits, int32_t vocab, int64_t ld, float temperature, int32_t top_k,
                           const int32_t* force, const int32_t* seeds, int32_t col, int32_t* drawn, int32_t rows) {
   if (!c || !logits || !force || !seeds || !drawn) return OMNI_ERR_INVALID;
+  OPS_CUDA(c, order(c->stream));  // forced tokens and seeds are read early
   OPS_CUDA(c, launch_lm_sample((const bf16*)logits, vocab, ld, temperature, top_k, force, seeds, col, drawn, rows,
                                c->stream));
   return OMNI_OK;
