@@ -33,7 +33,9 @@ void omni_ops_destroy(omni_ops* ctx);
 int32_t omni_ops_sync(omni_ops* ctx, uint32_t* word);
 /* The stream that the context's calls run on from here: given = 1: `stream`, a cudaStream_t of the context's device (NULL = the
  * default stream), which the caller may be capturing into a graph if the calls made are those of the 8-bit paged cache below;
- * given = 0: the context's own again, as after `omni_ops_create`. Calls on the one are not ordered against calls on the other. */
+ * given = 0: the context's own again, as after `omni_ops_create`. Calls on the one are not ordered against calls on the other, but
+ * for those that use the context's scratch (`omni_op_gemm` and the chain GEMMs): each waits for the one before it, wherever that
+ * ran, and is refused on a stream that is being captured. */
 int32_t omni_ops_stream(omni_ops* ctx, int32_t given, void* stream);
 /* Device time in ms between the two most recent omni_ops_mark calls (CUDA events on the context's stream). */
 int32_t omni_ops_mark(omni_ops* ctx, int32_t which /* 0 = begin, 1 = end */);

@@ -22,6 +22,8 @@ struct omni_ops {
   cudaStream_t stream = nullptr;  // what calls run on: `own` or the caller's
   cudaEvent_t ev[2] = {nullptr, nullptr};
   GemmScratch scratch;
+  cudaEvent_t scratch_used = nullptr;  // behind the last call that used it, if that ran on a stream of the caller's
+  bool scratch_on_own = true;          // it ran on `own` (or there is none)
   uint32_t* err = nullptr;
   cudaMemPool_t pool = nullptr;  // what a call needs for its own length, in its stream's order
   std::string error;
@@ -64,11 +66,33 @@ static cudaError_t on_aligned_rows(void* qkv, size_t qkv_bytes, void* out, size_
   return e != cudaSuccess ? e : done;
 }
 
+// Calls that use the context's scratch - the GEMMs' partial sums and the counters of their tiles - run one behind the other, on
+// whatever streams: scratch_begin() in front of their launches, scratch_end() behind them. Between two calls on the context's own
+// stream, which nobody else can capture or destroy, there is nothing to be done.
+static int scratch_begin(omni_ops* c);
+static cudaError_t scratch_end(omni_ops* c) {
+  c->scratch_on_own = c->stream == c->own;
+  return c->scratch_on_own ? cudaSuccess : cudaEventRecord(c->scratch_used, c->stream);
+}
+
 #define OPS_CUDA(ctx, expr)                                                                       \
   do {                                                                                            \
     cudaError_t e_ = (expr);                                                                      \
     if (e_ != cudaSuccess) return (ctx)->fail(OMNI_ERR_CUDA, "%s: %s", #expr, cudaGetErrorString(e_)); \
   } while (0)
+
+static int scratch_begin(omni_ops* c) {
+  if (c->stream == c->own && c->scratch_on_own) return OMNI_OK;
+  if (c->stream && c->stream != c->own) {  // two graphs that share scratch could be replayed side by side
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    OPS_CUDA(c, cudaStreamIsCapturing(c->stream, &capture));
+    if (capture != cudaStreamCaptureStatusNone)
+      return c->fail(OMNI_ERR_UNSUPPORTED, "calls that use the context's scratch (GEMMs and chains) cannot be captured");
+  }
+  if (c->scratch_on_own) OPS_CUDA(c, cudaEventRecord(c->scratch_used, c->own));
+  OPS_CUDA(c, cudaStreamWaitEvent(c->stream, c->scratch_used, 0));
+  return OMNI_OK;
+}
 
 extern "C" {
 
@@ -86,6 +110,7 @@ int32_t omni_ops_create(int32_t device, omni_ops** out) {
   c->stream = c->own;
   OPS_CUDA(c, cudaEventCreate(&c->ev[0]));
   OPS_CUDA(c, cudaEventCreate(&c->ev[1]));
+  OPS_CUDA(c, cudaEventCreateWithFlags(&c->scratch_used, cudaEventDisableTiming));
   if (tc_init() != 0) return c->fail(OMNI_ERR_CUDA, "cuTensorMapEncodeTiled entry point not found");
   tc_configure();
   stream_configure();
@@ -115,6 +140,7 @@ void omni_ops_destroy(omni_ops* c) {
   if (c->pool) cudaMemPoolDestroy(c->pool);
   if (c->ev[0]) cudaEventDestroy(c->ev[0]);
   if (c->ev[1]) cudaEventDestroy(c->ev[1]);
+  if (c->scratch_used) cudaEventDestroy(c->scratch_used);
   if (c->own) cudaStreamDestroy(c->own);
   delete c;
 }
@@ -191,7 +217,10 @@ int32_t omni_op_gemm(omni_ops* c, const void* w, int32_t N, int32_t K, const voi
   TcGemmPlan plan;
   const int rc = tc_plan(&plan, (const bf16*)w, N, K, (const bf16*)x, rows, (bf16*)y, ldy, epi, c->sm_count, splits);
   if (rc != 0) return c->fail(OMNI_ERR_CUDA, "tensor-map encode failed (%d)", rc);
-  OPS_CUDA(c, tc_launch(plan, c->scratch, c->err, c->stream));
+  if (const int busy = scratch_begin(c)) return busy;
+  const cudaError_t e = tc_launch(plan, c->scratch, c->err, c->stream);
+  OPS_CUDA(c, scratch_end(c));
+  OPS_CUDA(c, e);
   return OMNI_OK;
 }
 
@@ -265,16 +294,22 @@ int32_t omni_op_chain_gemm(omni_ops* c, const void* w, int32_t N, int32_t K, con
   if (!swiglu) {
     Epilogue epi;
     epi.bias = static_cast<const bf16*>(bias), epi.kind = epilogue;
-    OPS_CUDA(c, order(c->stream));
-    OPS_CUDA(c, chain.gemm((const bf16*)w, N, K, (const bf16*)x, rows, kStreamBf16, (bf16*)y, ldy, nullptr, 0, epi));
+    if (const int busy = scratch_begin(c)) return busy;
+    cudaError_t e = order(c->stream);
+    if (e == cudaSuccess) e = chain.gemm((const bf16*)w, N, K, (const bf16*)x, rows, kStreamBf16, (bf16*)y, ldy, nullptr, 0, epi);
+    OPS_CUDA(c, scratch_end(c));
+    OPS_CUDA(c, e);
     return OMNI_OK;
   }
   if (!wide_fuses(N, K, kGateGroup)) return c->fail(OMNI_ERR_UNSUPPORTED, "gate and up rows are no groups of %d", kGateGroup);
+  if (const int busy = scratch_begin(c)) return busy;
   bf16* grouped = nullptr;
   OPS_CUDA(c, cudaMalloc((void**)&grouped, (size_t)N * K * sizeof(bf16)));
   cudaError_t e = launch_interleave_gate_up((const bf16*)w, grouped, N / 2, K, kGateGroup, c->stream);
   if (e == cudaSuccess) e = order(c->stream);  // the GEMM asks for its weights before it waits
   if (e == cudaSuccess) e = chain.gemm(grouped, N, K, (const bf16*)x, rows, kStreamSwiglu, (bf16*)y, ldy);
+  const cudaError_t used = scratch_end(c);
+  if (e == cudaSuccess) e = used;
   const cudaError_t done = cudaStreamSynchronize(c->stream);
   cudaFree(grouped);
   OPS_CUDA(c, e);
@@ -289,6 +324,7 @@ int32_t omni_op_chain_norm_gemm(omni_ops* c, const void* w1, int32_t D, int32_t 
   int launches = 0;
   ChainPlans plans;
   const Chain chain{c->stream, c->err, c->sm_count, c->scratch.partials, c->scratch.partial_floats, &launches, &plans};
+  if (const int busy = scratch_begin(c)) return busy;
   OPS_CUDA(c, order(c->stream));
   bf16* tmp = nullptr;  // the rows of a norm of its own, the other residual of a folded one
   const size_t row_bytes = (size_t)rows * D * sizeof(bf16);
@@ -305,6 +341,8 @@ int32_t omni_op_chain_norm_gemm(omni_ops* c, const void* w1, int32_t D, int32_t 
                         },
                         (const bf16*)w2, N, D, tmp, rows, kStreamBf16, (bf16*)y, N);
   if (e == cudaSuccess && in != (bf16*)res) e = cudaMemcpyAsync(res, in, row_bytes, cudaMemcpyDeviceToDevice, c->stream);
+  const cudaError_t used = scratch_end(c);
+  if (e == cudaSuccess) e = used;
   const cudaError_t done = cudaStreamSynchronize(c->stream);
   cudaFree(tmp);
   OPS_CUDA(c, e);
