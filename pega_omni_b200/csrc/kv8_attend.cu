@@ -10,8 +10,10 @@
 // order of the head's elements within a sum is free, so a lane's operands are whole words of a key's row (Q is held in the same
 // order), and those of V^T are bytes of two tokens put side by side. Queries go to f16 under a power of two of their own, which
 // loses nothing above 2^-39 of the largest. With s the score in powers of two and u the log2 of the page's V scale, the
-// weights of a row are 2^(s + u - R), R near the largest s + u: at most 2^8 and rounded to f16 (2^-11 relative, an eighth of what
-// the bf16 result is rounded by). Their sum is taken of 2^(s - r) in f32, r near the largest s.
+// weights of a row are 2^(s + u - R + 7) in f16, which reaches less far than a float: R is near the largest s + u, but goes down, and
+// the sums up, for a page all of whose weights of a query lie 2^16 or more below it (where one token has nearly all of the weight and
+// no value, as an attention sink does, such pages are the result). A weight is off by 2^-11 of itself or 2^-16 of its page's largest,
+// whichever is more, down to pages 2^60 below the largest. The weights' sum is taken of 2^(s - r) in f32, r near the largest s.
 //
 // 128 rows of 500 to 8,000 tokens, 16 heads of 128 over 8: 173 us, 6.46 TB/s, 99 % of what a copy reaches. Where the rows are few it
 // is the way through one page that takes the time, 0.3 us a warp (0.7 us with sixteen heads), and the start and the join, 5 us.
@@ -30,7 +32,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr float kSlack = 8.f;  // powers of two by which a score may pass its reference before the sums are rescaled
+// In powers of two: by how much a score may pass its reference before the sums are rescaled; what a weight at its reference is; between
+// what the largest of a page's weights of a query may lie; by how much a reference may be lowered. A sum is at most
+// 2^(kTop + kLowered) times a code (2^9) and the tokens (2^31) then, which a float holds.
+constexpr float kSlack = 8.f, kLift = 7.f, kTop = kLift + kSlack, kFar = 9.f, kLowered = 60.f;
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kLowest = -1e30f;  // reference in front of all scores: a number, so that no difference is infinite minus infinite
 constexpr float kNone = -1.f;  // what the sums of a row that is not attended to are to be multiplied by, in the first of its pieces' parts
@@ -286,6 +291,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
   }
 
   float r[NT][2], R[NT][2], l[NT][2], o[NT][STEPS][4];
+  uint32_t lowered = 0;  // by how many powers of two at most R lies below the largest s + u, a byte a column
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     r[nt][0] = r[nt][1] = R[nt][0] = R[nt][1] = kLowest, l[nt][0] = l[nt][1] = 0.f;
@@ -293,6 +299,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
     for (int j = 0; j < STEPS; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
   }
 
+  const uint32_t column = 0x11111111u << t;  // the lanes that share this one's columns
   int stage = 0;
   for (int i = 0; i < mine; ++i) {
     copy_wait<S - 2>();
@@ -323,33 +330,54 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
       }
       float lvs;
       asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lvs) : "f"(vs));
-      bool over = false;
+      float to[NT][2];   // from scores to weights
+      bool off = false;  // a score above its reference by more than kSlack, or a lane's largest weight of a column out of [2^-kFar, 2^kTop]
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        // scores above this pass one of their references by more than kSlack
-        const float most[2] = {fminf(r[nt][0], R[nt][0] - lvs) + kSlack, fminf(r[nt][1], R[nt][1] - lvs) + kSlack};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[nt][e] *= ks * unit_of[nt][e & 1];
           if (kPart && g + (e & 2) * 4 >= valid) s[nt][e] = kNegInf;
-          over |= s[nt][e] > most[e & 1];
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float most = fmaxf(s[nt][e], s[nt][e + 2]);
+          to[nt][e] = lvs + kLift - R[nt][e];
+          const float weight = most + to[nt][e];
+          off |= most - r[nt][e] > kSlack || weight > kTop || (weight < -kFar && (!kPart || g < valid));
         }
       }
-      if (__any_sync(0xffffffffu, over)) {
+      if (__any_sync(0xffffffffu, off)) {
+        bool go = false;  // is it more than a lane's part of a column that lies far below?
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float m = fmaxf(s[nt][e], s[nt][e + 2]);
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-            const float nr = fmaxf(r[nt][e], m), nR = fmaxf(R[nt][e], m + lvs);
-            l[nt][e] *= exp2_of(r[nt][e] - nr);
-            const float f = exp2_of(R[nt][e] - nR);
-            r[nt][e] = nr, R[nt][e] = nR;
-#pragma unroll
-            for (int j = 0; j < STEPS; ++j) o[nt][j][e] *= f, o[nt][j][e + 2] *= f;
+            const float most = fmaxf(s[nt][e], s[nt][e + 2]), weight = most + to[nt][e];
+            const uint32_t near = __ballot_sync(0xffffffffu, !(weight < -kFar));
+            go |= most - r[nt][e] > kSlack || weight > kTop || (near & column) == 0;
           }
+        if (__any_sync(0xffffffffu, go)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float m = fmaxf(s[nt][e], s[nt][e + 2]);
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+              const float nr = fmaxf(r[nt][e], m), below = R[nt][e] - lvs - m;
+              l[nt][e] *= exp2_of(r[nt][e] - nr);
+              r[nt][e] = nr;
+              float nR = fmaxf(R[nt][e], m + lvs);
+              const int at = 8 * (2 * nt + e);
+              const float low = (float)(lowered >> at & 255);
+              if (below > kFar + kLift && lvs > kNegInf) nR = R[nt][e] - fminf(floorf(below) - kSlack, kLowered - low);
+              const float by = R[nt][e] - nR, f = exp2_of(by);
+              R[nt][e] = nR, to[nt][e] = lvs + kLift - nR, lowered += (uint32_t)(int)fmaxf(by, -low) << at;
+#pragma unroll
+              for (int j = 0; j < STEPS; ++j) o[nt][j][e] *= f, o[nt][j][e + 2] *= f;
+            }
+        }
       }
       uint32_t p[NT][2];
 #pragma unroll
@@ -358,7 +386,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           l[nt][e & 1] += exp2_of(s[nt][e] - r[nt][e & 1]);
-          w[e] = exp2_of(s[nt][e] + (lvs - R[nt][e & 1]));
+          w[e] = exp2_of(s[nt][e] + to[nt][e & 1]);
         }
         p[nt][0] = transpose8(half2_of(w[0], w[1])), p[nt][1] = transpose8(half2_of(w[2], w[3]));
       }
@@ -407,7 +435,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
       if (n < nq) {
-        if (g == 0) parts[warp][n] = Part{r[nt][e], R[nt][e], l[nt][e], 0.f};
+        if (g == 0) parts[warp][n] = Part{r[nt][e], R[nt][e] - kLift, l[nt][e], R[nt][e] + (float)(lowered >> 8 * (2 * nt + e) & 255) - kLift};
         float* const dst = sums + (warp * NT * 8 + n) * D + g * (D / 8);
 #pragma unroll
         for (int j = 0; j < STEPS; j += 2)
@@ -418,7 +446,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
   if (tid < nq) {
     float r_top = kLowest, R_top = kLowest, l_sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) r_top = fmaxf(r_top, parts[w][tid].r), R_top = fmaxf(R_top, parts[w][tid].R);
+    for (int w = 0; w < kWarps; ++w) r_top = fmaxf(r_top, parts[w][tid].r), R_top = fmaxf(R_top, parts[w][tid].f);  // as if no reference had been lowered
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) l_sum += parts[w][tid].l * weight_of(parts[w][tid].r, r_top), factor[w][tid] = weight_of(parts[w][tid].R, R_top);
     joined[tid] = part_of(r_top, R_top, l_sum);
