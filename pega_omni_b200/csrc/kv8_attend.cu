@@ -10,10 +10,11 @@
 // order of the head's elements within a sum is free, so a lane's operands are whole words of a key's row (Q is held in the same
 // order), and those of V^T are bytes of two tokens put side by side. Queries go to f16 under a power of two of their own, which
 // loses nothing above 2^-39 of the largest. With s the score in powers of two and u the log2 of the page's V scale, the
-// weights of a row are 2^(s + u - R + 7) in f16, which reaches less far than a float: R is near the largest s + u, but goes down, and
-// the sums up, for a page all of whose weights of a query lie 2^16 or more below it (where one token has nearly all of the weight and
-// no value, as an attention sink does, such pages are the result). A weight is off by 2^-11 of itself or 2^-16 of its page's largest,
-// whichever is more, down to pages 2^60 below the largest. The weights' sum is taken of 2^(s - r) in f32, r near the largest s.
+// weights of a row are 2^(s - r + u - R + 7) in f16, which reaches less far than a float: r + R is near the largest s + u, but goes
+// down, and the sums up, for a page all of whose weights of a query lie 2^16 or more below it (where one token has nearly all of the
+// weight and no value, as an attention sink does, such pages are the result). A weight is off by 2^-11 of itself or 2^-16 of its page's
+// largest, whichever is more, down to pages 2^60 below the largest. The weights' sum is taken of 2^(s - r) in f32, r near the largest
+// s. Scores may be of any size: R is kept from r on, since u would be lost in a sum with a score beyond 2^24.
 //
 // 128 rows of 500 to 8,000 tokens, 16 heads of 128 over 8: 173 us, 6.46 TB/s, 99 % of what a copy reaches. Where the rows are few it
 // is the way through one page that takes the time, 0.3 us a warp (0.7 us with sixteen heads), and the start and the join, 5 us.
@@ -37,7 +38,8 @@ namespace cg = cooperative_groups;
 // 2^(kTop + kLowered) times a code (2^9) and the tokens (2^31) then, which a float holds.
 constexpr float kSlack = 8.f, kLift = 7.f, kTop = kLift + kSlack, kFar = 9.f, kLowered = 60.f;
 constexpr float kNegInf = -__builtin_huge_valf();
-constexpr float kLowest = -1e30f;  // reference in front of all scores: a number, so that no difference is infinite minus infinite
+// References in front of all scores and weights: numbers, so that no difference is infinite minus infinite.
+constexpr float kLowest = -3.402823466e38f, kLowestWeight = -1e30f;
 constexpr float kNone = -1.f;  // what the sums of a row that is not attended to are to be multiplied by, in the first of its pieces' parts
 
 constexpr int kWarps = 4;
@@ -100,13 +102,14 @@ __device__ __forceinline__ uint32_t piece_at(int row, int col) {
   return (uint32_t)(row * D + ((D == 128 ? col ^ (row & 7) : col ^ ((row >> 1) & 3)) << 4));
 }
 
-struct Part {  // of a query: reference of the scores, of the weights, sum of 2^(s - r), and what the weights' sums are to be multiplied by
+struct Part {  // of a query: reference of the scores, of the weights (from r on), sum of 2^(s - r), and what the weights' sums are to be multiplied by
   float r, R, l, f;
 };
+constexpr Part kNothing = {kLowest, kLowestWeight, 0.f, 0.f};
 // Weight of summands under reference x when the largest reference is `top`.
 __device__ __forceinline__ float weight_of(float x, float top) { return exp2_of(x - top); }
 // 0 where nothing was attended to: all of the row's pages lie outside the cache.
-__device__ __forceinline__ Part part_of(float r, float R, float l) { return Part{r, R, l, l == 0.f ? 0.f : exp2_of(R - r) / l}; }
+__device__ __forceinline__ Part part_of(float r, float R, float l) { return Part{r, R, l, l == 0.f ? 0.f : exp2_of(R) / l}; }
 __device__ __forceinline__ uint2 result_of(float4 v, float f) {
   const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x * f, v.y * f), hi = __floats2bfloat162_rn(v.z * f, v.w * f);
   return make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
@@ -294,7 +297,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
   uint32_t lowered = 0;  // by how many powers of two at most R lies below the largest s + u, a byte a column
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    r[nt][0] = r[nt][1] = R[nt][0] = R[nt][1] = kLowest, l[nt][0] = l[nt][1] = 0.f;
+    r[nt][0] = r[nt][1] = kLowest, R[nt][0] = R[nt][1] = kLowestWeight, l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
     for (int j = 0; j < STEPS; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
   }
@@ -330,7 +333,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
       }
       float lvs;
       asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lvs) : "f"(vs));
-      float to[NT][2];   // from scores to weights
+      float to[NT][2];   // from scores above their reference to weights
       bool off = false;  // a score above its reference by more than kSlack, or a lane's largest weight of a column out of [2^-kFar, 2^kTop]
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -341,10 +344,10 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float most = fmaxf(s[nt][e], s[nt][e + 2]);
+          const float most = fmaxf(s[nt][e], s[nt][e + 2]) - r[nt][e];
           to[nt][e] = lvs + kLift - R[nt][e];
           const float weight = most + to[nt][e];
-          off |= most - r[nt][e] > kSlack || weight > kTop || (weight < -kFar && (!kPart || g < valid));
+          off |= most > kSlack || weight > kTop || (weight < -kFar && (!kPart || g < valid));
         }
       }
       if (__any_sync(0xffffffffu, off)) {
@@ -353,9 +356,9 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float most = fmaxf(s[nt][e], s[nt][e + 2]), weight = most + to[nt][e];
+            const float most = fmaxf(s[nt][e], s[nt][e + 2]) - r[nt][e], weight = most + to[nt][e];
             const uint32_t near = __ballot_sync(0xffffffffu, !(weight < -kFar));
-            go |= most - r[nt][e] > kSlack || weight > kTop || (near & column) == 0;
+            go |= most > kSlack || weight > kTop || (near & column) == 0;
           }
         if (__any_sync(0xffffffffu, go)) {
 #pragma unroll
@@ -365,14 +368,15 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
               float m = fmaxf(s[nt][e], s[nt][e + 2]);
 #pragma unroll
               for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-              const float nr = fmaxf(r[nt][e], m), below = R[nt][e] - lvs - m;
-              l[nt][e] *= exp2_of(r[nt][e] - nr);
+              const float nr = fmaxf(r[nt][e], m), up = r[nt][e] - nr;
+              l[nt][e] *= exp2_of(up);
               r[nt][e] = nr;
-              float nR = fmaxf(R[nt][e], m + lvs);
+              const float was = fmaxf(R[nt][e] + up, kLowestWeight), top = m - nr + lvs, below = was - top;  // from the new r on
               const int at = 8 * (2 * nt + e);
               const float low = (float)(lowered >> at & 255);
-              if (below > kFar + kLift && lvs > kNegInf) nR = R[nt][e] - fminf(floorf(below) - kSlack, kLowered - low);
-              const float by = R[nt][e] - nR, f = exp2_of(by);
+              float nR = fmaxf(was, top);
+              if (below > kFar + kLift && lvs > kNegInf) nR = was - fminf(floorf(below) - kSlack, kLowered - low);
+              const float by = was - nR, f = exp2_of(by);
               R[nt][e] = nR, to[nt][e] = lvs + kLift - nR, lowered += (uint32_t)(int)fmaxf(by, -low) << at;
 #pragma unroll
               for (int j = 0; j < STEPS; ++j) o[nt][j][e] *= f, o[nt][j][e + 2] *= f;
@@ -385,8 +389,9 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          l[nt][e & 1] += exp2_of(s[nt][e] - r[nt][e & 1]);
-          w[e] = exp2_of(s[nt][e] + to[nt][e & 1]);
+          const float above = s[nt][e] - r[nt][e & 1];
+          l[nt][e & 1] += exp2_of(above);
+          w[e] = exp2_of(above + to[nt][e & 1]);
         }
         p[nt][0] = transpose8(half2_of(w[0], w[1])), p[nt][1] = transpose8(half2_of(w[2], w[3]));
       }
@@ -444,11 +449,16 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
     }
   __syncthreads();
   if (tid < nq) {
-    float r_top = kLowest, R_top = kLowest, l_sum = 0.f;
+    float r_top = kLowest, R_top = kNegInf, l_sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) r_top = fmaxf(r_top, parts[w][tid].r), R_top = fmaxf(R_top, parts[w][tid].f);  // as if no reference had been lowered
+    for (int w = 0; w < kWarps; ++w) r_top = fmaxf(r_top, parts[w][tid].r);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) l_sum += parts[w][tid].l * weight_of(parts[w][tid].r, r_top), factor[w][tid] = weight_of(parts[w][tid].R, R_top);
+    for (int w = 0; w < kWarps; ++w) R_top = fmaxf(R_top, parts[w][tid].f + (parts[w][tid].r - r_top));  // as if no reference had been lowered
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float to_top = parts[w][tid].r - r_top;
+      l_sum += parts[w][tid].l * exp2_of(to_top), factor[w][tid] = weight_of(parts[w][tid].R + to_top, R_top);
+    }
     joined[tid] = part_of(r_top, R_top, l_sum);
   }
   __syncthreads();
@@ -481,15 +491,19 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NT>) kv8_attend_kernel(con
   fetch(begin);
   {
     const int n = tid >> 3, c = tid & 7;
-    Part p = {kLowest, kLowest, 0.f, 0.f};
+    Part p = kNothing;
     if (n < nq && c < ctas) p = *cluster.map_shared_rank(&joined[n], c);
-    float r_top = p.r, R_top = p.R;
+    float r_top = p.r;
 #pragma unroll
-    for (int x = 1; x < 8; x <<= 1) r_top = fmaxf(r_top, __shfl_xor_sync(0xffffffffu, r_top, x)), R_top = fmaxf(R_top, __shfl_xor_sync(0xffffffffu, R_top, x));
-    float l_sum = p.l * weight_of(p.r, r_top);
+    for (int x = 1; x < 8; x <<= 1) r_top = fmaxf(r_top, __shfl_xor_sync(0xffffffffu, r_top, x));
+    const float to_top = p.r - r_top, R = p.R + to_top;
+    float R_top = R;
+#pragma unroll
+    for (int x = 1; x < 8; x <<= 1) R_top = fmaxf(R_top, __shfl_xor_sync(0xffffffffu, R_top, x));
+    float l_sum = p.l * exp2_of(to_top);
 #pragma unroll
     for (int x = 1; x < 8; x <<= 1) l_sum += __shfl_xor_sync(0xffffffffu, l_sum, x);
-    if (n < nq) factor[c][n] = part_of(r_top, R_top, l_sum).f * weight_of(p.R, R_top);
+    if (n < nq) factor[c][n] = part_of(r_top, R_top, l_sum).f * weight_of(R, R_top);
   }
   __syncthreads();
   for (int i = begin; i < end; i += step) {
@@ -527,7 +541,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4) kv8_join_kernel(const __gr
   const int64_t step = (int64_t)groups * cut.per, at = (piece.before * (int64_t)groups + part) * cut.per + n;
   const float4* const parts = reinterpret_cast<const float4*>(cut.parts) + at;
   const int g = tid / LANES, d = tid % LANES;
-  Part mine = {kLowest, kLowest, 0.f, 0.f};
+  Part mine = kNothing;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   const float first = __ldcg(parts).w;
   for (int c = g; c < piece.count; c += AHEAD * GROUPS) {
@@ -535,19 +549,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4) kv8_join_kernel(const __gr
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
       const int at_piece = c + k * GROUPS;
-      p[k] = make_float4(kLowest, kLowest, 0.f, 0.f), x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      p[k] = make_float4(kNothing.r, kNothing.R, 0.f, 0.f), x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (at_piece < piece.count) p[k] = __ldcg(parts + at_piece * step), x[k] = __ldcg(reinterpret_cast<const float4*>(cut.sums + (at + at_piece * step) * D) + d);
     }
-    float r = mine.r, R = mine.R;
+    float r = mine.r;
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) r = fmaxf(r, p[k].x), R = fmaxf(R, p[k].y);
+    for (int k = 0; k < AHEAD; ++k) r = fmaxf(r, p[k].x);
+    mine.l *= exp2_of(mine.r - r), mine.R += mine.r - r, mine.r = r;
+    float R = mine.R;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) R = fmaxf(R, p[k].y + (p[k].x - r));
     const float old = weight_of(mine.R, R);
-    mine.l *= weight_of(mine.r, r), mine.r = r, mine.R = R;
+    mine.R = R;
     v.x *= old, v.y *= old, v.z *= old, v.w *= old;
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      mine.l += p[k].z * weight_of(p[k].x, r);
-      const float f = weight_of(p[k].y, R);
+      const float to_top = p[k].x - r, f = weight_of(p[k].y + to_top, R);
+      mine.l += p[k].z * exp2_of(to_top);
       v.x += x[k].x * f, v.y += x[k].y * f, v.z += x[k].z * f, v.w += x[k].w * f;
     }
   }
@@ -556,16 +574,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4) kv8_join_kernel(const __gr
   if (d == 0) part_of_group[g] = mine;
   __syncthreads();
   if (g > 0) return;
-  Part all = {kLowest, kLowest, 0.f, 0.f};
+  Part all = {kLowest, kNegInf, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < GROUPS; ++i) all.r = fmaxf(all.r, part_of_group[i].r), all.R = fmaxf(all.R, part_of_group[i].R);
+  for (int i = 0; i < GROUPS; ++i) all.r = fmaxf(all.r, part_of_group[i].r);
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) all.R = fmaxf(all.R, part_of_group[i].R + (part_of_group[i].r - all.r));
   v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < GROUPS; ++i) {
     const Part p = part_of_group[i];
     const float4 x = v_of[i][d];
-    const float f = weight_of(p.R, all.R);
-    all.l += p.l * weight_of(p.r, all.r);
+    const float to_top = p.r - all.r, f = weight_of(p.R + to_top, all.R);
+    all.l += p.l * exp2_of(to_top);
     v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
   }
   *reinterpret_cast<uint2*>(a.out + row * a.ldo + (int64_t)head * D + d * 4) = result_of(v, part_of(all.r, all.R, all.l).f);
