@@ -261,7 +261,8 @@ int32_t omni_op_kv_tables(omni_ops* ctx, const int32_t* lens, const int32_t* add
 /* The first q_heads + kv_heads heads of every row of x with pos >= 0, normed (x / sqrt(mean x^2 + eps) * gain, q_norm for the
  * q heads, k_norm for the k heads; NULL: no norm) and rotated: elements i and i + head_dim / 2 by pos * theta^(-2 i / head_dim).
  * Computed in f32 from an angle in f64 and rounded once (the attention calls above round between the steps as the reference
- * does). Other rows of out stay as they are. out may be x, with the same stride, and must not overlap it otherwise. */
+ * does). Other rows of out stay as they are. out may be x, with the same stride if there is more than one row, and must not overlap it
+ * otherwise. */
 int32_t omni_op_qk_norm_rope(omni_ops* ctx, const void* x, int64_t ldx, const void* q_norm, const void* k_norm,
                              const int32_t* pos, int32_t rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                              float eps, float theta, void* out, int64_t ldo);

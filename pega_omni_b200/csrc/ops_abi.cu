@@ -574,7 +574,7 @@ int32_t omni_op_qk_norm_rope(omni_ops* c, const void* x, int64_t ldx, const void
     return c->fail(OMNI_ERR_UNSUPPORTED, "%d + %d heads of %d: heads of 64 or 128", q_heads, kv_heads, head_dim);
   if (rows == 0) return OMNI_OK;
   const int64_t width = ((int64_t)q_heads + kv_heads) * head_dim;
-  if (!x || !pos || !out || !rows_at16(x, ldx, width) || !rows_at16(out, ldo, width) || !at16(q_norm) || !at16(k_norm) || (x == out && ldx != ldo))
+  if (!x || !pos || !out || !rows_at16(x, ldx, width) || !rows_at16(out, ldo, width) || !at16(q_norm) || !at16(k_norm) || (x == out && ldx != ldo && rows > 1))
     return c->fail(OMNI_ERR_INVALID, "null, rows that are not at 16-byte addresses or overlap, or a row stride below %lld", (long long)width);
   const OnDevice on(c->device);
   OPS_CUDA(c, launch_qk_norm_rope((const bf16*)x, ldx, (const bf16*)q_norm, (const bf16*)k_norm, pos, rows, q_heads, kv_heads,
