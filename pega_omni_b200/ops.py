@@ -24,28 +24,38 @@ def _need(ok, what):
         raise OpsError(what)
 
 
-def _ints(*tensors):
-    """Their addresses: contiguous int32."""
+def _ints(device, *tensors):
+    """Their addresses: contiguous int32 on the device, or in pinned host memory, which it reaches too."""
     at = []
     for t in tensors:
         if t.dtype is not _I32 or not t.is_contiguous():
             raise OpsError("lengths, positions, slots and pages are contiguous int32")
+        if t.get_device() != device and not (t.device.type == "cpu" and t.is_pinned()):
+            raise OpsError(f"a tensor on {t.device} in a call on device {device}")
         at.append(t.data_ptr())
     return at
 
 
-def _rows(t, rows, width, at_least=False):
+def _on(device, t):
+    """t's address; it has to be on the device."""
+    if t.get_device() != device:
+        raise OpsError(f"a tensor on {t.device} in a call on device {device}")
+    return t.data_ptr()
+
+
+def _rows(device, t, rows, width, at_least=False):
     """(address, row stride) of bf16 rows, each contiguous."""
     shape, stride = t.shape, t.stride()
     if t.dtype is not _BF16 or (shape != (rows, width) and not (at_least and len(shape) == 2 and shape[0] == rows and shape[1] > width)) or \
             (stride[1] != 1 and width > 1):
         raise OpsError(f"rows are bf16 [{rows}, {width}], each contiguous: got {t.dtype} {tuple(shape)} with strides {stride}")
-    return t.data_ptr(), stride[0] if rows > 1 else shape[1] + 7 & ~7
+    return _on(device, t), stride[0] if rows > 1 else shape[1] + 7 & ~7
 
 
 class Ops:
     def __init__(self, device: int = 0):
         self._lib = L.load()
+        self._device = device
         h = C.c_void_p()
         rc = self._lib.omni_ops_create(device, C.byref(h))
         self._h = h
@@ -196,7 +206,8 @@ class Ops:
     def kv_tables(self, lens, add, table, free_pages, free_count, lens_out, free_count_out, indptr, pages, row_ptr, pos, slot,
                   seq, status):
         n, width = table.shape
-        at = _ints(lens, add, table, free_pages, free_count, lens_out, free_count_out, indptr, pages, row_ptr, pos, slot, seq, status)
+        at = _ints(self._device, lens, add, table, free_pages, free_count, lens_out, free_count_out, indptr, pages, row_ptr, pos, slot, seq,
+                   status)
         row_cap = pos.numel()
         _need(lens.numel() == add.numel() == lens_out.numel() == n and indptr.numel() == row_ptr.numel() == n + 1 and
               slot.numel() == seq.numel() == row_cap, "one length, addition and table row a sequence; pos, slot and seq of one size")
@@ -204,39 +215,42 @@ class Ops:
                                                 at[6], at[7], at[8], pages.numel(), at[9], at[10], at[11], at[12], row_cap, at[13]))
 
     def qk_norm_rope(self, x, q_norm, k_norm, pos, q_heads, kv_heads, head_dim, eps, theta, out):
-        rows, width = pos.numel(), (q_heads + kv_heads) * head_dim
+        dev, rows, width = self._device, pos.numel(), (q_heads + kv_heads) * head_dim
         for gain in (q_norm, k_norm):
             _need(gain is None or (gain.dtype is _BF16 and gain.shape == (head_dim,) and gain.is_contiguous()), "gains are bf16 [head_dim]")
-        self._check(self._lib.omni_op_qk_norm_rope(self._h, *_rows(x, rows, width, True), _p(q_norm), _p(k_norm), *_ints(pos), rows,
-                                                   q_heads, kv_heads, head_dim, eps, theta, *_rows(out, rows, width, True)))
+        self._check(self._lib.omni_op_qk_norm_rope(self._h, *_rows(dev, x, rows, width, True), None if q_norm is None else _on(dev, q_norm),
+                                                   None if k_norm is None else _on(dev, k_norm), *_ints(dev, pos), rows, q_heads, kv_heads,
+                                                   head_dim, eps, theta, *_rows(dev, out, rows, width, True)))
 
     def packed_attend(self, q, k, v, indptr, q_heads, kv_heads, head_dim, scale, out):
-        rows, width, kv_width = q.shape[0], q_heads * head_dim, kv_heads * head_dim
-        self._check(self._lib.omni_op_packed_attend(self._h, *_rows(q, rows, width), *_rows(k, rows, kv_width), *_rows(v, rows, kv_width),
-                                                    *_ints(indptr), indptr.numel() - 1, rows, q_heads, kv_heads, head_dim, scale,
-                                                    *_rows(out, rows, width)))
+        dev, rows, width, kv_width = self._device, q.shape[0], q_heads * head_dim, kv_heads * head_dim
+        self._check(self._lib.omni_op_packed_attend(self._h, *_rows(dev, q, rows, width), *_rows(dev, k, rows, kv_width),
+                                                    *_rows(dev, v, rows, kv_width), *_ints(dev, indptr), indptr.numel() - 1, rows, q_heads,
+                                                    kv_heads, head_dim, scale, *_rows(dev, out, rows, width)))
 
     def _cache(self, kv, scales):
+        """(pages, heads, head_dim, address of kv, of scales)."""
         pages, heads, two, page, head_dim = kv.shape
         _need(kv.element_size() == 1 and two == 2 and page == L.OMNI_PAGE and kv.is_contiguous() and scales.is_contiguous() and
               scales.dtype is _F32 and scales.shape == (pages, heads, 2),
               "a cache is [pages, kv_heads, 2, 16, head_dim] of bytes with f32 scales [pages, kv_heads, 2]")
-        return pages, heads, head_dim
+        return pages, heads, head_dim, _on(self._device, kv), _on(self._device, scales)
 
     def kv8_append(self, k, v, slot, kv, scales):
-        pages, heads, head_dim = self._cache(kv, scales)
-        rows, width = slot.numel(), heads * head_dim
-        self._check(self._lib.omni_op_kv8_append(self._h, *_rows(k, rows, width), *_rows(v, rows, width), *_ints(slot), rows,
-                                                 kv.data_ptr(), scales.data_ptr(), pages, heads, head_dim))
+        pages, heads, head_dim, at_kv, at_scales = self._cache(kv, scales)
+        dev, rows, width = self._device, slot.numel(), heads * head_dim
+        self._check(self._lib.omni_op_kv8_append(self._h, *_rows(dev, k, rows, width), *_rows(dev, v, rows, width), *_ints(dev, slot), rows,
+                                                 at_kv, at_scales, pages, heads, head_dim))
 
     def kv8_attend(self, q, kv, scales, pos, indptr, pages, q_heads, scale, out, seq=None):
-        kv_pages, kv_heads, head_dim = self._cache(kv, scales)
-        at_pos, at_indptr, at_pages = _ints(pos, indptr, pages)
+        kv_pages, kv_heads, head_dim, at_kv, at_scales = self._cache(kv, scales)
+        dev = self._device
+        at_pos, at_indptr, at_pages = _ints(dev, pos, indptr, pages)
         rows, width, n_seqs = pos.numel(), q_heads * head_dim, indptr.numel() - 1
         _need(n_seqs >= rows if seq is None else seq.numel() == rows, "a sequence for each row")
-        self._check(self._lib.omni_op_kv8_attend(self._h, *_rows(q, rows, width), kv.data_ptr(), scales.data_ptr(), kv_pages, at_pos,
-                                                 None if seq is None else _ints(seq)[0], at_indptr, n_seqs, at_pages, pages.numel(),
-                                                 rows, q_heads, kv_heads, head_dim, scale, *_rows(out, rows, width)))
+        self._check(self._lib.omni_op_kv8_attend(self._h, *_rows(dev, q, rows, width), at_kv, at_scales, kv_pages, at_pos,
+                                                 None if seq is None else _ints(dev, seq)[0], at_indptr, n_seqs, at_pages, pages.numel(),
+                                                 rows, q_heads, kv_heads, head_dim, scale, *_rows(dev, out, rows, width)))
 
     # ---- streaming codec decoder (state: a byte tensor; lines / pos: int32 tensors, one entry per stream) ----
     def codec_rvq(self, codes, books, out, book_rows):
