@@ -210,7 +210,8 @@ class Ops:
                    status)
         row_cap = pos.numel()
         _need(lens.numel() == add.numel() == lens_out.numel() == n and indptr.numel() == row_ptr.numel() == n + 1 and
-              slot.numel() == seq.numel() == row_cap, "one length, addition and table row a sequence; pos, slot and seq of one size")
+              slot.numel() == seq.numel() == row_cap and free_count.numel() and free_count_out.numel() and status.numel(),
+              "one length, addition and table row a sequence; pos, slot and seq of one size; a word for the count and the status")
         self._check(self._lib.omni_op_kv_tables(self._h, at[0], at[1], n, at[2], width, at[3], free_pages.numel(), at[4], at[5],
                                                 at[6], at[7], at[8], pages.numel(), at[9], at[10], at[11], at[12], row_cap, at[13]))
 

@@ -94,3 +94,12 @@ def test_pinned_host_memory(ops, name):
             else:
                 with pytest.raises(OpsError, match="cpu"):
                     getattr(ops, name)(*args)
+
+
+@pytest.mark.parametrize("which", [4, 6, 13])
+def test_a_word_for_counts_and_status(ops, which):
+    args = arguments("kv_tables")
+    args[which] = Tensor(0)
+    with pytest.raises(OpsError, match="a word"):
+        ops.kv_tables(*args)
+    assert ops._lib.calls == 0
