@@ -3,8 +3,6 @@ from __future__ import annotations
 
 import ctypes as C
 
-import torch
-
 from . import lib as L
 
 
@@ -16,7 +14,13 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
+_BF16 = _F32 = _I32 = None  # torch's, from the first call on that looks at a tensor's type: without such calls torch need not be there
+
+
+def _types():
+    global _BF16, _F32, _I32
+    import torch
+    _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 
 
 def _need(ok, what):
@@ -26,6 +30,8 @@ def _need(ok, what):
 
 def _ints(device, *tensors):
     """Their addresses: contiguous int32 on the device, or in pinned host memory, which it reaches too."""
+    if _I32 is None:
+        _types()
     at = []
     for t in tensors:
         if t.dtype is not _I32 or not t.is_contiguous():
@@ -45,6 +51,8 @@ def _on(device, t):
 
 def _rows(device, t, rows, width, at_least=False):
     """(address, row stride) of bf16 rows, each contiguous."""
+    if _BF16 is None:
+        _types()
     shape, stride = t.shape, t.stride()
     if t.dtype is not _BF16 or (shape != (rows, width) and not (at_least and len(shape) == 2 and shape[0] == rows and shape[1] > width)) or \
             (stride[1] != 1 and width > 1):
@@ -217,10 +225,11 @@ class Ops:
 
     def qk_norm_rope(self, x, q_norm, k_norm, pos, q_heads, kv_heads, head_dim, eps, theta, out):
         dev, rows, width = self._device, pos.numel(), (q_heads + kv_heads) * head_dim
+        at_pos, = _ints(dev, pos)
         for gain in (q_norm, k_norm):
             _need(gain is None or (gain.dtype is _BF16 and gain.shape == (head_dim,) and gain.is_contiguous()), "gains are bf16 [head_dim]")
         self._check(self._lib.omni_op_qk_norm_rope(self._h, *_rows(dev, x, rows, width, True), None if q_norm is None else _on(dev, q_norm),
-                                                   None if k_norm is None else _on(dev, k_norm), *_ints(dev, pos), rows, q_heads, kv_heads,
+                                                   None if k_norm is None else _on(dev, k_norm), at_pos, rows, q_heads, kv_heads,
                                                    head_dim, eps, theta, *_rows(dev, out, rows, width, True)))
 
     def packed_attend(self, q, k, v, indptr, q_heads, kv_heads, head_dim, scale, out):
@@ -231,6 +240,8 @@ class Ops:
 
     def _cache(self, kv, scales):
         """(pages, heads, head_dim, address of kv, of scales)."""
+        if _F32 is None:
+            _types()
         pages, heads, two, page, head_dim = kv.shape
         _need(kv.element_size() == 1 and two == 2 and page == L.OMNI_PAGE and kv.is_contiguous() and scales.is_contiguous() and
               scales.dtype is _F32 and scales.shape == (pages, heads, 2),

@@ -1,4 +1,8 @@
 """What the operators' Python side refuses before it calls the library: tensors that a kernel could not reach, arrays too small."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -103,3 +107,8 @@ def test_a_word_for_counts_and_status(ops, which):
     with pytest.raises(OpsError, match="a word"):
         ops.kv_tables(*args)
     assert ops._lib.calls == 0
+
+
+def test_torch_is_not_needed_to_import_them():
+    code = "import sys; sys.modules['torch'] = None; import pega_omni_b200.ops as o; assert o.Ops and o.gemm_noalloc"
+    subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], check=True, timeout=60)
