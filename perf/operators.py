@@ -210,16 +210,21 @@ def prepare(case, seed):
 
 # ---- the operators -----------------------------------------------------------------------------------------------------
 
-_context = []
+_contexts = {}  # device -> [its context, the stream that its calls run on]
 
 
 def _ops():
-    """The operators' context on the stream that the program works on."""
-    if not _context:
+    """The current device's context, on the stream that the program works on at the moment."""
+    device = torch.cuda.current_device()
+    if device not in _contexts:
         from pega_omni_b200.ops import Ops
-        _context.append(Ops(torch.cuda.current_device()))
-        _context[0].stream(torch.cuda.current_stream().cuda_stream)
-    return _context[0]
+        _contexts[device] = [Ops(device), None]
+    context = _contexts[device]
+    stream = torch._C._cuda_getCurrentRawStream(device)  # torch.cuda.current_stream() makes an object, which takes longer than some of the calls
+    if context[1] != stream:
+        context[0].stream(stream)
+        context[1] = stream
+    return context[0]
 
 
 def run(st):
