@@ -37,16 +37,13 @@ def _ints(device, *tensors):
         if t.dtype is not _I32 or not t.is_contiguous():
             raise OpsError("lengths, positions, slots and pages are contiguous int32")
         if t.get_device() != device and not (t.device.type == "cpu" and t.is_pinned()):
-            raise OpsError(f"a tensor on {t.device} in a call on device {device}")
+            raise _elsewhere(device, t)
         at.append(t.data_ptr())
     return at
 
 
-def _on(device, t):
-    """t's address; it has to be on the device."""
-    if t.get_device() != device:
-        raise OpsError(f"a tensor on {t.device} in a call on device {device}")
-    return t.data_ptr()
+def _elsewhere(device, t):
+    return OpsError(f"a tensor on {t.device} in a call on device {device}")
 
 
 def _rows(device, t, rows, width, at_least=False):
@@ -57,7 +54,9 @@ def _rows(device, t, rows, width, at_least=False):
     if t.dtype is not _BF16 or (shape != (rows, width) and not (at_least and len(shape) == 2 and shape[0] == rows and shape[1] > width)) or \
             (stride[1] != 1 and width > 1):
         raise OpsError(f"rows are bf16 [{rows}, {width}], each contiguous: got {t.dtype} {tuple(shape)} with strides {stride}")
-    return _on(device, t), stride[0] if rows > 1 else shape[1] + 7 & ~7
+    if t.get_device() != device:
+        raise _elsewhere(device, t)
+    return t.data_ptr(), stride[0] if rows > 1 else shape[1] + 7 & ~7
 
 
 class Ops:
@@ -227,10 +226,13 @@ class Ops:
         dev, rows, width = self._device, pos.numel(), (q_heads + kv_heads) * head_dim
         at_pos, = _ints(dev, pos)
         for gain in (q_norm, k_norm):
-            _need(gain is None or (gain.dtype is _BF16 and gain.shape == (head_dim,) and gain.is_contiguous()), "gains are bf16 [head_dim]")
-        self._check(self._lib.omni_op_qk_norm_rope(self._h, *_rows(dev, x, rows, width, True), None if q_norm is None else _on(dev, q_norm),
-                                                   None if k_norm is None else _on(dev, k_norm), at_pos, rows, q_heads, kv_heads,
-                                                   head_dim, eps, theta, *_rows(dev, out, rows, width, True)))
+            if gain is None:
+                continue
+            _need(gain.dtype is _BF16 and gain.shape == (head_dim,) and gain.is_contiguous(), "gains are bf16 [head_dim]")
+            if gain.get_device() != dev:
+                raise _elsewhere(dev, gain)
+        self._check(self._lib.omni_op_qk_norm_rope(self._h, *_rows(dev, x, rows, width, True), _p(q_norm), _p(k_norm), at_pos, rows, q_heads,
+                                                   kv_heads, head_dim, eps, theta, *_rows(dev, out, rows, width, True)))
 
     def packed_attend(self, q, k, v, indptr, q_heads, kv_heads, head_dim, scale, out):
         dev, rows, width, kv_width = self._device, q.shape[0], q_heads * head_dim, kv_heads * head_dim
@@ -246,7 +248,10 @@ class Ops:
         _need(kv.element_size() == 1 and two == 2 and page == L.OMNI_PAGE and kv.is_contiguous() and scales.is_contiguous() and
               scales.dtype is _F32 and scales.shape == (pages, heads, 2),
               "a cache is [pages, kv_heads, 2, 16, head_dim] of bytes with f32 scales [pages, kv_heads, 2]")
-        return pages, heads, head_dim, _on(self._device, kv), _on(self._device, scales)
+        for t in (kv, scales):
+            if t.get_device() != self._device:
+                raise _elsewhere(self._device, t)
+        return pages, heads, head_dim, kv.data_ptr(), scales.data_ptr()
 
     def kv8_append(self, k, v, slot, kv, scales):
         pages, heads, head_dim, at_kv, at_scales = self._cache(kv, scales)
