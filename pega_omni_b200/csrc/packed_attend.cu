@@ -40,6 +40,7 @@ namespace {
 
 constexpr int kTile = 128;
 constexpr float kLag = 8.f;  // powers of two
+constexpr float kFar = 268435456.f;  // 2^28 powers of two: references beyond are off by more than sixteen when they are rounded
 constexpr float kNegInf = -__builtin_huge_valf();
 
 struct Args {
@@ -136,7 +137,7 @@ __device__ __forceinline__ void issue_sums(uint32_t o, uint32_t p, uint32_t v, i
   }
 }
 
-// A row's reference and the sum of its weights.
+// A row's reference, a score as the product gives it, and the sum of its weights.
 struct Row {
   float m = kNegInf, l = 0.f;
 };
@@ -160,16 +161,23 @@ __device__ __forceinline__ void make_weights(Row& row, uint32_t s_at, uint32_t o
       for (int t = 0; t < 4; ++t) top[t] = max3_nan(top[t], s[c + t], s[c + 4 + t]);
 #pragma unroll
     for (int t = 0; t < 4; ++t) top[t] = max3_nan(top[t], s[kTile - 4 + t], s[kTile - 4 + t]);
-    return max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3])) * scale_to_2;
+    return max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3]));
   };
   float2 sum[2];
+  // A weight is 2^((s - off) * scale + minus_ref): near 0 the reference goes into the sum, rounded, which is a factor in common; far from
+  // it, where that factor would not fit, it is taken off the scores.
+  float off, minus_ref;
+  const auto refer = [&] {
+    const float ref = row.m == kNegInf ? 0.f : row.m * scale_to_2;
+    off = fabsf(ref) > kFar ? row.m : 0.f, minus_ref = fabsf(ref) > kFar ? 0.f : -ref;
+  };
   const auto weights = [&](int q) {  // of a quarter of the keys
-    const float2 scale = both(scale_to_2), minus_ref = both(row.m == kNegInf ? 0.f : -row.m);
+    const float2 scale = both(scale_to_2), minus = both(minus_ref);
     uint32_t p[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int c = q * 32 + 2 * e;
-      const float2 x = fma2(make_float2(s[c], s[c + 1]), scale, minus_ref), w = make_float2(exp2_of(x.x), exp2_of(x.y));
+      const float2 x = fma2(make_float2(s[c], s[c + 1]), scale, minus), w = make_float2(exp2_of(x.x), exp2_of(x.y));
       sum[e & 1] = add2(sum[e & 1], w);
       const __nv_bfloat162 h = __floats2bfloat162_rn(w.x, w.y);
       p[e] = *reinterpret_cast<const uint32_t*>(&h);
@@ -182,21 +190,12 @@ __device__ __forceinline__ void make_weights(Row& row, uint32_t s_at, uint32_t o
     __syncwarp();
     give(half);
   };
-  // The first half is made under the reference as it is, with the row's maximum beside it, and once more where that turns out to be
-  // too far off. In front of all a maximum comes first.
-  float now;
-  if (first) row.m = now = largest();
-#pragma unroll 1
-  for (;;) {
-    sum[0] = sum[1] = both(0.f);
-    weights(0), weights(1);
-    if (first) break;
-    now = largest();
-    const bool over = now > row.m + kLag;
-    if (!__any_sync(0xffffffffu, over)) break;
-    const float next = over ? now : row.m;
-    const float f = row.m == next ? 1.f : row.m == kNegInf ? 0.f : exp2_of(row.m - next);
-    row.m = next, row.l *= f;
+  const auto raise_to = [&](float next) {
+    const float was = row.m, was_off = off, was_minus = minus_ref;
+    row.m = next;
+    refer();
+    const float f = was == next ? 1.f : was == kNegInf ? 0.f : exp2_of(fmaf(was_off - off, scale_to_2, minus_ref - was_minus));
+    row.l *= f;
 #pragma unroll 1
     for (int c = 0; c < D; c += 16) {
       float o[16];
@@ -206,6 +205,29 @@ __device__ __forceinline__ void make_weights(Row& row, uint32_t s_at, uint32_t o
       for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(o[e] * f);
       tmem_st16(o_at + c, r);
     }
+  };
+  // The first half is made under the reference as it is, with the row's maximum beside it, and once more where that turns out to be
+  // too far off. In front of all a maximum comes first, and where a row's reference is far from 0.
+  float now;
+  if (first) row.m = now = largest();
+  refer();
+  bool far = __any_sync(0xffffffffu, off != 0.f), last = first;
+#pragma unroll 1
+  for (;;) {
+    if (far) {
+      if (!first) now = largest(), raise_to(fmaxf(row.m, now));
+#pragma unroll
+      for (int c = 0; c < kTile; ++c) s[c] -= off;
+      last = true;
+    }
+    sum[0] = sum[1] = both(0.f);
+    weights(0), weights(1);
+    if (last) break;
+    now = largest();
+    const bool over = (now - row.m) * scale_to_2 > kLag;
+    if (!__any_sync(0xffffffffu, over)) break;
+    raise_to(over ? now : row.m);
+    far = __any_sync(0xffffffffu, off != 0.f);
   }
   done(0);
   weights(2), weights(3);
