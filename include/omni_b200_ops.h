@@ -2,9 +2,11 @@
  * own, over caller-owned DEVICE buffers. The reference exposes its kernels as
  * named ops of a manifest (`Gen::launch` / `Gen::gemm_rows`,
  * crates/omni-kern/src/lib.rs:103-224); these entry points are the same ops as
- * plain calls, used by the parity tests and micro-benchmarks. All tensors are
+ * plain calls, for parity tests and micro-benchmarks, and the operators around
+ * an 8-bit paged cache, for a server's own steps. All tensors are
  * bf16 row-major unless stated; every call is asynchronous on the context's
- * stream, `omni_ops_sync` waits and returns the device error word.
+ * stream and reads what calls in front of it there wrote; `omni_ops_sync` waits
+ * and returns the device error word.
  */
 #ifndef OMNI_B200_OPS_H
 #define OMNI_B200_OPS_H
@@ -27,6 +29,7 @@ enum omni_gemm_path {
 enum omni_epilogue { OMNI_EPI_NONE = 0, OMNI_EPI_BIAS = 1, OMNI_EPI_BIAS_SILU = 2 };
 
 int32_t omni_ops_create(int32_t device, omni_ops** out);
+/* Graphs that captured calls of the context hold its error word: they are not replayed any more when it is destroyed. */
 void omni_ops_destroy(omni_ops* ctx);
 /* Waits for the context's stream; returns 0, OMNI_ERR_CUDA (-2) or, when a
  * kernel raised the device error word, OMNI_ERR_DEVICE (-3) with the word in *word. */
@@ -269,9 +272,11 @@ int32_t omni_op_qk_norm_rope(omni_ops* ctx, const void* x, int64_t ldx, const vo
 
 /* Causal attention within each of n packed sequences (16,384 at most): rows indptr[i] .. indptr[i + 1] of q, k and v, of which row r sees the
  * sequence's rows up to itself: out[r][h] = softmax(scale * q[r][h] . K) V, h over q_heads and K, V those of kv head
- * h / (q_heads / kv_heads). scale > 0. indptr ascends from any row on; sequences may be empty. Rows outside of the sequences stay
+ * h / (q_heads / kv_heads). scale > 0. Scores and sums are f32; the weights are rounded to bf16, by 2^-8 of each at most, before they
+ * meet V (`omni_op_rope_attend` spends more bits there). indptr ascends from any row on; sequences may be empty. Rows outside of the sequences stay
  * as they are in out, and nothing of them, of other sequences or of later rows reaches a row, not even as a NaN. out must not
- * overlap q, k or v. */
+ * overlap q, k or v. The kernel's waits end by themselves after 0.4 s, which a sequence of some ten million rows may need for one
+ * tile: the device error word tells. */
 int32_t omni_op_packed_attend(omni_ops* ctx, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
                               int64_t ldv, const int32_t* indptr, int32_t n, int32_t rows, int32_t q_heads,
                               int32_t kv_heads, int32_t head_dim, float scale, void* out, int64_t ldo);
@@ -289,7 +294,10 @@ int32_t omni_op_kv8_append(omni_ops* ctx, const void* k, int64_t ldk, const void
 /* out[n][h] = softmax(scale * q[n][h] . K) V over tokens 0 .. pos[n] of sequence seq[n] (NULL: sequence n) of n_seqs, whose pages
  * are pages[indptr[s] .. indptr[s + 1]) out of n_pages. Rows with pos < 0 become zeros. What a page holds behind the row's
  * last token is not looked at. Scales may be any numbers >= 0 here. A row whose sequence, range or number of pages is wrong becomes
- * zeros; a page outside the cache is left out. */
+ * zeros; a page outside the cache is left out. Weights (times their page's V scale) are rounded to f16 on the way to V: by 2^-11 of
+ * each or 2^-16 of its page's largest, whichever is more, and pages whose largest lies below 2^-60 of the row's may lose more. The host
+ * takes n_pages / n_seqs for the rows' length when it cuts the work: the answer does not depend on it, the time does where `pages` has
+ * much more room than the sequences have pages. */
 int32_t omni_op_kv8_attend(omni_ops* ctx, const void* q, int64_t ldq, const void* kv, const float* scales, int32_t kv_pages,
                            const int32_t* pos, const int32_t* seq, const int32_t* indptr, int32_t n_seqs,
                            const int32_t* pages, int32_t n_pages, int32_t rows, int32_t q_heads, int32_t kv_heads,

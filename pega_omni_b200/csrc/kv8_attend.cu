@@ -16,8 +16,9 @@
 // largest, whichever is more, down to pages 2^60 below the largest. The weights' sum is taken of 2^(s - r) in f32, r near the largest
 // s. Scores may be of any size: R is kept from r on, since u would be lost in a sum with a score beyond 2^24.
 //
-// 128 rows of 500 to 8,000 tokens, 16 heads of 128 over 8: 173 us, 6.46 TB/s, 99 % of what a copy reaches. Where the rows are few it
-// is the way through one page that takes the time, 0.3 us a warp (0.7 us with sixteen heads), and the start and the join, 5 us.
+// 128 rows of 500 to 8,000 tokens, 16 heads of 128 over 8: 175 to 177 us from a graph, 6.35 TB/s, 97 % of what a copy reaches (193 to
+// 197 call after call, when power takes a tenth of the clock). Where the rows are few it is the way through one page that takes the
+// time, 0.3 us a warp (0.7 us with sixteen heads), and the start and the join, 5 us.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -642,7 +643,7 @@ cudaError_t launch_kv8_attend(const Kv8Attend& a, int sm_count, cudaMemPool_t po
   //   12 x 8,  28,000 - 34,000  258 /  164 /  133 /  157 | 130 - 139
   //   20 x 8,  500 - 5,000       44 /   30 /   29 /   31 | 27
   //   64 x 8,  2,000 - 8,000    128 /  123 /  116 /  120 |
-  //   128 x 8, 500 - 8,000      207 /  194 /  187 /  206 |  (the clock at rest: 173 with 4)
+  //   128 x 8, 500 - 8,000      207 /  194 /  187 /  206 |  (the clock at rest: 175 with 4)
   //   256 x 8, 100 - 2,000       98 /  103 /  133 /  211 |
   int ctas = 1;
   if (a.rows <= kCutRows && units * 6 <= at_once && held >= 256) {

@@ -1,4 +1,5 @@
-"""Operator-level calls (include/omni_b200_ops.h) over torch CUDA tensors, for parity tests and micro-benchmarks."""
+"""Operator-level calls (include/omni_b200_ops.h) over torch CUDA tensors: for parity tests and micro-benchmarks, and the operators
+around the 8-bit paged cache for a server's own steps."""
 from __future__ import annotations
 
 import ctypes as C
@@ -205,7 +206,8 @@ class Ops:
                                                    _p(force), _p(state), _p(lines), stride, _p(codes), rows))
 
     # ---- 8-bit paged cache (rows: bf16 [rows, heads * head_dim] with any row stride; kv: one byte an element
-    # [pages, kv_heads, 2, 16, head_dim]; scales: f32 [pages, kv_heads, 2]; everything else contiguous int32) ----
+    # [pages, kv_heads, 2, 16, head_dim]; scales: f32 [pages, kv_heads, 2]; everything else contiguous int32, which may also lie in
+    # pinned host memory) ----
     def stream(self, stream=None):
         """Later calls run on `stream` (a cudaStream_t as an int, 0: the default stream); None: on the context's own again."""
         self._check(self._lib.omni_ops_stream(self._h, stream is not None, stream))
