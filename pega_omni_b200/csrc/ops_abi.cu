@@ -75,10 +75,14 @@ static cudaError_t scratch_end(omni_ops* c) {
   return c->scratch_on_own ? cudaSuccess : cudaEventRecord(c->scratch_used, c->stream);
 }
 
+// An error that is reported is taken off the runtime's record, where the next call's launches would find it.
 #define OPS_CUDA(ctx, expr)                                                                       \
   do {                                                                                            \
     cudaError_t e_ = (expr);                                                                      \
-    if (e_ != cudaSuccess) return (ctx)->fail(OMNI_ERR_CUDA, "%s: %s", #expr, cudaGetErrorString(e_)); \
+    if (e_ != cudaSuccess) {                                                                      \
+      cudaGetLastError();                                                                         \
+      return (ctx)->fail(OMNI_ERR_CUDA, "%s: %s", #expr, cudaGetErrorString(e_));                 \
+    }                                                                                             \
   } while (0)
 
 static int scratch_begin(omni_ops* c) {
@@ -142,6 +146,7 @@ void omni_ops_destroy(omni_ops* c) {
   if (c->ev[1]) cudaEventDestroy(c->ev[1]);
   if (c->scratch_used) cudaEventDestroy(c->scratch_used);
   if (c->own) cudaStreamDestroy(c->own);
+  cudaGetLastError();  // of a context that could not be set up
   delete c;
 }
 

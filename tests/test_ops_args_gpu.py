@@ -32,3 +32,17 @@ def test_norm_and_rope_in_place_on_parts_of_wider_rows(ops, rows, wider):
     ops.qk_norm_rope(x, gain, gain, pos, hq, hk, d, 1e-6, 1e4, x[:, :width])
     ops.sync()
     assert torch.equal(x[:, :width], want) and torch.equal(x[:, width:], rest)
+
+
+def test_an_error_is_reported_once(ops):
+    """A context for a device that is not there is refused; the calls behind it do not hear of it again."""
+    from pega_omni_b200.ops import Ops, OpsError
+    w, x = (torch.randn(*shape, device="cuda").to(torch.bfloat16) for shape in ((64, 128), (2, 128)))
+    y = torch.zeros(2, 64, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    for again in range(2):
+        with pytest.raises(OpsError, match="device"):
+            Ops(99)
+        ops.chain_gemm(w, x, y)
+        ops.sync()
+    assert y.abs().sum() > 0
