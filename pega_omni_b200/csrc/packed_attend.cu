@@ -16,7 +16,7 @@
 //  - single_kernel: two CTAs of a tile each, which read K and V twice as often, but are out of step at an item's end, and smaller.
 // Of a turn of paired_kernel (a block of keys for both tiles, 3,400 clocks) the tensor cores have work for 2,050, the exponentials' pipe as
 // much; the rest is the way from the last weights to the next scores, and an item's end. The clock is what power leaves at this rate: 8,192
-// tokens of 32 heads take 470 to 515 us from a graph, 520 call after call. A cubic for every eighth or fourth exponential, two threads a row, an issuing
+// tokens of 32 heads take 470 to 515 us from a graph, 520 to 540 call after call. A cubic for every eighth or fourth exponential, two threads a row, an issuing
 // warp a tile (which lets both tiles fall into step), weights in unequal parts, a first reference from part of a row and 32-byte stores of results made it no faster.
 //
 // Scores, maxima, sums and O are f32. Weights go to bf16 because V does (one type for both operands): 2^-8 at most of a weight,
